@@ -627,6 +627,63 @@ RD_API int rd_cache_commit(int dtype, void* cache, int B, int nkv, int max_len, 
 RD_API int rd_decode_advance(const int64_t* next_tok, int64_t* token_buf, int64_t buf_ld, const int32_t* buf_begin,
                       const int32_t* begin, int32_t* kv_len, int32_t* base_len, int32_t* slot, int limit, int B, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Keys, values and weights in fewer bits.  No counterpart in the reference.
+ *
+ * A cache held in codes.  A row (one token's key or value of one head, hd values x; hd a multiple of 8, at most 256), with
+ * Q = 2^bits - 1 (bits 4 or 8), low = min(0, min x) and high = max(0, max x): scale = bf16((high - low) / Q) (the difference in fp32),
+ * zero = rint(-low / scale), code = rint(x / scale) + zero, both cut to 0 .. Q; a code stands for scale * (code - zero).  A scale
+ * of 0 (a row of zeros, or of values too small) makes all codes 0; NaN, infinities, or a difference past fp32's largest number make
+ * the scale NaN, and with it all that the row stands for.  Divisions round correctly, ties go to even: the codes are those of exact arithmetic.
+ * k_codes / v_codes [B, nkv, max_len, hd * bits / 8] bytes, one code each or two (feature 2 i in the low half); k_params / v_params
+ * [B, nkv, max_len] 32-bit words, the scale's bf16 pattern in the lower half, zero in the upper.  All four 16-byte aligned. */
+
+/* Quantises the keys and values of new tokens as they are written: head g of token t at k + t*tok_stride + g*head_stride (strides in
+ * elements; k, v and strides 16-byte aligned), to slot tok_slot[t] of row tok_row[t].  Tokens whose row or slot lies outside the cache are
+ * left out; two tokens of a call must not have the same place. */
+RD_API int rd_cache_quant_append(int dtype, int bits, const void* k, const void* v, int64_t tok_stride, int64_t head_stride, uint8_t* k_codes,
+                          void* k_params, uint8_t* v_codes, void* v_params, const int32_t* tok_row, const int32_t* tok_slot, int m_max,
+                          const int32_t* m_dev, int B, int nkv, int hd, int max_len, void* stream);
+
+/* Reads back: slots begin[b] .. begin[b] + length[b] - 1 of row b to rows 0 .. of k_out / v_out [B, nkv, out_len, hd] in `dtype`, rounded
+ * once.  At most out_len rows, none past the cache; what lies behind a row's last is left as it was.  A row with begin < 0 is left out. */
+RD_API int rd_cache_quant_read(int dtype, int bits, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes, const void* v_params,
+                        const int32_t* begin, const int32_t* length, int B, int nkv, int hd, int max_len, void* k_out, void* v_out,
+                        int out_len, void* stream);
+
+/* rd_cache_commit for `planes` consecutive planes of codes [planes, B, nkv, max_len, hd * bits / 8] and their parameters at once. */
+RD_API int rd_cache_quant_commit(int bits, uint8_t* codes, void* params, int planes, int B, int nkv, int max_len, int hd,
+                          const int32_t* kv_begin, const int32_t* base_len, const int32_t* unpacker, int W, int Lb, const int32_t* n_accepted,
+                          const int32_t* seq_in_beam, void* stream);
+
+/* Attention over such a cache: as rd_attention in modes RD_ATTN_CAUSAL and RD_ATTN_TREE (the new tokens' keys and values are in the
+ * cache), with scores multiplied by `scale`.  q: head h of token t at q + t*ldq + h*hd; out [m_max, nh*hd], rows past the last new token
+ * are left as they were.  A token that sees no key gets zeros.  max_len a multiple of 16; q, out and ldq 16-byte aligned.  max_new and
+ * max_kv bound the new tokens of a row and its keys.  workspace: rd_attention_quant_workspace_bytes() of device memory, 16-byte aligned
+ * (NULL if that is 0); calls that may run at the same time need one each. */
+RD_API int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m_max, int B, int nh, int nkv, int hd, int max_new, int max_kv);
+RD_API int rd_attention_quant(int dtype, int bits, const void* q, int64_t ldq, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,
+                       const void* v_params, void* out, const int32_t* row_start, const int32_t* kv_begin, const int32_t* base_len, int m_max,
+                       int B, int nh, int nkv, int hd, int max_len, int max_new, int max_kv, int mode, const uint32_t* tree_mask,
+                       int mask_words, float scale, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Rows as 8-bit integers: scale = bf16(max |x| / 127) held in fp32, code = rint(x / scale) cut to -127 .. 127 (ties to even, exact as
+ * above); a row of zeros has scale 0, one with NaN or infinities scale NaN and codes 0.  Columns K .. ld_codes - 1 are set to 0.
+ * codes 16-byte aligned, ld_codes a multiple of 16. */
+RD_API int rd_quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max, const int32_t* m_dev,
+                  int K, void* stream);
+
+/* C[t, n] = a_scales[t] w_scales[n] sum_k A[t, k] W[n, k], the sums exact (K <= 131072, a multiple of 16; A and W rows 16-byte aligned).
+ * epilogue: RD_EPI_NONE, RD_EPI_RES (R [m, ldr] in out_dtype; R may be C) or RD_EPI_SWIGLU (N even, C has N / 2 columns). */
+RD_API int rd_gemm_int8(int out_dtype, const int8_t* A, int64_t lda, const float* a_scales, const int8_t* W, int64_t ldw, const float* w_scales,
+                 void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev, int N, int K, int epilogue,
+                 int32_t* status, void* stream);
+/* rd_quant_rows of x [m, K] into codes / scales (the caller's, kept until the product has run), then rd_gemm_int8 of these with K rounded up
+ * to a multiple of 16 (columns of W past K are zeros). */
+RD_API int rd_linear_int8(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, const int8_t* W, int64_t ldw,
+                   const float* w_scales, int out_dtype, void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev,
+                   int N, int K, int epilogue, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

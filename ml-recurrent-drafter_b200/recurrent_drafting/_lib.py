@@ -106,6 +106,14 @@ SIGNATURES = {
     "rd_mlstm_scan": (_I, [_I, _P, _L, _P, _L, _P, _P, _F, _P, _F, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P]),
     "rd_cache_commit": (_I, [_I, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P]),
     "rd_decode_advance": (_I, [_P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "rd_cache_quant_append": (_I, [_I, _I, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
+    "rd_cache_quant_read": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P]),
+    "rd_cache_quant_commit": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P]),
+    "rd_attention_quant_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
+    "rd_attention_quant": (_I, [_I, _I, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _L, _P, _P]),
+    "rd_quant_rows": (_I, [_I, _P, _L, _P, _L, _P, _I, _P, _I, _P]),
+    "rd_gemm_int8": (_I, [_I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _L, _I, _P, _I, _I, _I, _P, _P]),
+    "rd_linear_int8": (_I, [_I, _P, _L, _P, _L, _P, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _I, _P, _P]),
     "rd_cache_unpack_static": (_I, [_I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P]),
 }
 

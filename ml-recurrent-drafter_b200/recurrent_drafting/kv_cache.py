@@ -6,8 +6,9 @@ it and only grows: row b occupies slots [kv_begin[b], kv_begin[b] + kv_len[b]). 
 are device int32 vectors owned by the decode loop; the View/Cache surface below keeps the
 reference's scalar `length` semantics for callers that use the cache the reference's way.
 """
+import math
 from dataclasses import dataclass
-from typing import List, Sequence, Tuple, Union
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -102,6 +103,141 @@ class Cache:
                   n_heads, max_length, head_dim, prompt_length, _lib.ptr(idx), n_flat, _lib.stream())
         for k, v in self.sliced:
             k.length = v.length = prompt_length + n_flat
+
+
+class LayerCodes(NamedTuple):
+    """One layer of a QuantizedCache: codes [batch, heads, capacity, head_dim * bits / 8] (uint8) and parameters [batch, heads, capacity, 2]
+    (int16: the bf16 pattern of the scale, zero)."""
+
+    k_codes: torch.Tensor
+    k_params: torch.Tensor
+    v_codes: torch.Tensor
+    v_params: torch.Tensor
+
+
+class QuantizedCache:
+    """Keys and values in codes of 8 or 4 bits, with a scale and a zero for each token of a head: a half or a quarter of a bf16 cache's
+    memory, and of the bytes that attention reads.  Rows are quantised as they are written (append), read back in a plain type (read), and
+    attended to where they lie (attend); slots and rows as in Cache.  A code stands for scale * (code - zero), zero being exact; see
+    rd_cache_quant_append in include/redrafter_b200.h for the rounding.
+
+    A row of batch, head and slot holds its values alone, so a slot may be written again at any time, and what lies past a row's length
+    is never looked at."""
+
+    SLOTS = 64  # the storage has a multiple of these
+
+    def __init__(self, batch_size: int, max_length: int, n_layers: int, n_heads: int, head_dim: int, bits: int, device) -> None:
+        if bits not in (4, 8):
+            raise _lib.RedrafterError(f"a cache is held in 4 or 8 bits, not in {bits}")
+        if head_dim % 8 or not 8 <= head_dim <= 256:
+            raise _lib.RedrafterError(f"heads of {head_dim} features: a multiple of 8 up to 256 is wanted")
+        self.bits, self.head_dim, self.max_length, self.length = bits, head_dim, max_length, 0
+        capacity = (max_length + self.SLOTS - 1) // self.SLOTS * self.SLOTS
+        self._codes = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, head_dim * bits // 8, dtype=torch.uint8, device=device)
+        self._params = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, 2, dtype=torch.int16, device=device)
+        self.layers = [LayerCodes(c[0], p[0], c[1], p[1]) for c, p in zip(self._codes, self._params)]
+
+    @property
+    def storage(self) -> "QuantizedCache":
+        """What the model's backbone() takes."""
+        return self
+
+    def set_length(self, length: int) -> None:
+        self.length = length
+
+    def bytes_per_token(self) -> int:
+        n_layers, _, _, heads, _, row = self._codes.shape
+        return 2 * n_layers * heads * (row + 4)
+
+    def _here(self, **tensors) -> None:
+        """The tensors lie on the cache's device, which is the current one: kernels are launched on its current stream."""
+        dev = self._codes.device
+        if not self._codes.is_cuda:
+            raise _lib.RedrafterError("operator called with a CPU tensor: this library has no CPU path")
+        if dev.index != torch._C._cuda_getDevice():
+            raise _lib.RedrafterError(f"the cache lies on {dev}, which is not the current device")
+        for name, t in tensors.items():
+            if t is not None and t.device != dev:
+                raise _lib.RedrafterError(f"{name} lies on {t.device}, the cache on {dev}")
+
+    @staticmethod
+    def _indices(**tensors) -> None:
+        for name, (t, n) in tensors.items():
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
+                raise _lib.RedrafterError(f"{name} is a contiguous int32 vector of {n} elements")
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, tok_row: torch.Tensor, tok_slot: torch.Tensor,
+               m_dev: Optional[torch.Tensor] = None) -> None:
+        """Writes the keys and values [tokens, heads, head_dim] of new tokens (bf16 or fp32; any strides of tokens and heads, the same in
+        both) to slots tok_slot of batch rows tok_row.  Two tokens must not have the same place."""
+        l = self.layers[layer]
+        B, heads, capacity, _ = l.k_codes.shape
+        m = k.shape[0]
+        if k.shape != (m, heads, self.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
+            raise _lib.RedrafterError(f"keys {tuple(k.shape)} and values {tuple(v.shape)}: [tokens, {heads}, {self.head_dim}] of one type is wanted")
+        # the stride of a dimension of size 1 says nothing
+        strides = [tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)) for t in (k, v)]
+        if strides[0] != strides[1] or (self.head_dim > 1 and strides[0][2] != 1):
+            raise _lib.RedrafterError("keys and values need the same strides, and their features one after another")
+        self._here(k=k, v=v, tok_row=tok_row, tok_slot=tok_slot, m_dev=m_dev)
+        self._indices(tok_row=(tok_row, m), tok_slot=(tok_slot, m))
+        _lib.call("rd_cache_quant_append", _lib.dtype_code(k.dtype), self.bits, _lib.ptr(k), _lib.ptr(v), strides[0][0], strides[0][1],
+                  _lib.ptr(l.k_codes), _lib.ptr(l.k_params), _lib.ptr(l.v_codes), _lib.ptr(l.v_params), _lib.ptr(tok_row), _lib.ptr(tok_slot), m,
+                  _lib.ptr(m_dev), B, heads, self.head_dim, capacity, _lib.stream())
+
+    def read(self, layer: int, begin: torch.Tensor, length: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
+        """Slots begin[b] .. begin[b] + length[b] - 1 of every row b as plain keys and values: rows 0 .. of k_out and v_out [batch, heads,
+        rows, head_dim] (bf16 or fp32, contiguous).  What lies behind a row's last is left as it was."""
+        l = self.layers[layer]
+        B, heads, capacity, _ = l.k_codes.shape
+        rows = k_out.shape[2] if k_out.dim() == 4 else -1
+        if k_out.shape != (B, heads, rows, self.head_dim) or v_out.shape != k_out.shape or k_out.dtype != v_out.dtype:
+            raise _lib.RedrafterError(f"outputs {tuple(k_out.shape)} and {tuple(v_out.shape)}: [{B}, {heads}, rows, {self.head_dim}] of one type is wanted")
+        if not (k_out.is_contiguous() and v_out.is_contiguous()):
+            raise _lib.RedrafterError("the outputs are contiguous")
+        self._here(begin=begin, length=length, k_out=k_out, v_out=v_out)
+        self._indices(begin=(begin, B), length=(length, B))
+        _lib.call("rd_cache_quant_read", _lib.dtype_code(k_out.dtype), self.bits, _lib.ptr(l.k_codes), _lib.ptr(l.k_params), _lib.ptr(l.v_codes),
+                  _lib.ptr(l.v_params), _lib.ptr(begin), _lib.ptr(length), B, heads, self.head_dim, capacity, _lib.ptr(k_out), _lib.ptr(v_out), rows,
+                  _lib.stream())
+
+    def attend(self, layer: int, q: torch.Tensor, out: torch.Tensor, row_start: torch.Tensor, kv_begin: torch.Tensor, base_len: torch.Tensor,
+               max_new: int, max_kv: int, mode: int = _lib.ATTN_CAUSAL, tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+               status: Optional[torch.Tensor] = None) -> None:
+        """Attention of new tokens, whose keys and values have been appended.  q [tokens, query heads * head_dim] (bf16 or fp32; rows any
+        stride apart), out the same, contiguous; row b of the batch has tokens row_start[b] .. row_start[b + 1] - 1, its keys are slots
+        kv_begin[b] .. + base_len[b] (all visible) and its new tokens' own, visible causally or through tree_mask [tokens, words] (ATTN_TREE).
+        max_new, max_kv: upper bounds of a row's new tokens and keys.  scale: of the scores, 1 / sqrt(head_dim) unless given."""
+        l = self.layers[layer]
+        B, heads, capacity, _ = l.k_codes.shape
+        m, width = q.shape
+        if width % (heads * self.head_dim) or out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise _lib.RedrafterError(f"queries {tuple(q.shape)}, output {tuple(out.shape)}: [tokens, a multiple of {heads} heads * {self.head_dim}] of one type is wanted")
+        if width > 1 and q.stride(1) != 1:
+            raise _lib.RedrafterError("the features of a query lie one after another")
+        self._here(q=q, out=out, row_start=row_start, kv_begin=kv_begin, base_len=base_len, tree_mask=tree_mask, status=status)
+        self._indices(row_start=(row_start, B + 1), kv_begin=(kv_begin, B), base_len=(base_len, B))
+        words = 0
+        if mode == _lib.ATTN_TREE:
+            if tree_mask is None or tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] < m or not tree_mask.is_contiguous():
+                raise _lib.RedrafterError("tree_mask is a contiguous int32 matrix with a row for each token")
+            words = tree_mask.shape[1]
+        code = _lib.dtype_code(q.dtype)
+        nh = width // self.head_dim
+        need = _lib.load().rd_attention_quant_workspace_bytes(code, self.bits, m, B, nh, heads, self.head_dim, max_new, max_kv)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        _lib.call("rd_attention_quant", code, self.bits, _lib.ptr(q), q.stride(0) if m > 1 else width, _lib.ptr(l.k_codes), _lib.ptr(l.k_params),
+                  _lib.ptr(l.v_codes), _lib.ptr(l.v_params), _lib.ptr(out), _lib.ptr(row_start), _lib.ptr(kv_begin), _lib.ptr(base_len), m, B, nh, heads,
+                  self.head_dim, capacity, max_new, max_kv, mode, _lib.ptr(tree_mask) if words else None, words,
+                  1.0 / math.sqrt(self.head_dim) if scale is None else scale, _lib.ptr(workspace), max(need, 0), _lib.ptr(status), _lib.stream())
+
+    def commit_draft(self, fp, n_accepted: torch.Tensor, seq_in_beam: torch.Tensor, beam_shape, kv_begin: torch.Tensor) -> None:
+        """Moves the accepted tokens of a packed draft behind the rows' prefixes, in all layers."""
+        n_layers, _, B, heads, capacity, _ = self._codes.shape
+        self._here()
+        _lib.call("rd_cache_quant_commit", self.bits, _lib.ptr(self._codes), _lib.ptr(self._params), 2 * n_layers, B, heads, capacity, self.head_dim,
+                  _lib.ptr(kv_begin), _lib.ptr(fp.base_len), _lib.ptr(fp.unpacker), beam_shape.width, beam_shape.length, _lib.ptr(n_accepted),
+                  _lib.ptr(seq_in_beam), _lib.stream())
 
 
 @dataclass(frozen=True)

@@ -245,6 +245,78 @@ class Linear:
                       _lib.ptr(m_dev), n, k, epilogue, _lib.stream())
 
 
+class Int8Linear:
+    """y = epilogue(x W^T) with the weight's rows and, at each call, the rows of x in 8-bit integers, a scale for each row of both: half of
+    a bf16 weight's bytes.  The sums are exact; see rd_quant_rows in include/redrafter_b200.h for the rounding of the rows."""
+
+    def __init__(self, weight: torch.Tensor):
+        n, k = weight.shape
+        codes = torch.empty(n, (k + 15) // 16 * 16, dtype=torch.int8, device=weight.device)
+        scales = torch.empty(n, dtype=torch.float32, device=weight.device)
+        quantize_rows(weight, codes, scales)
+        self._hold(codes, scales, k)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8Linear":
+        """From a weight that is held in integers: codes [out, in] int8 (-127 .. 127), scales [out] fp32."""
+        n, k = codes.shape
+        if codes.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != (n,) or scales.device != codes.device:
+            raise _lib.RedrafterError("codes [out, in] int8 and scales [out] fp32 on one device are wanted")
+        if k % 16 or not codes.is_contiguous() or codes.data_ptr() % 16:
+            padded = torch.zeros(n, (k + 15) // 16 * 16, dtype=torch.int8, device=codes.device)
+            padded[:, :k] = codes
+            codes = padded
+        self = cls.__new__(cls)
+        self._hold(codes, scales.contiguous(), k)
+        return self
+
+    def _hold(self, codes: torch.Tensor, scales: torch.Tensor, k: int) -> None:
+        self.codes, self.scales, self.in_features, self.out_features = codes, scales, k, codes.shape[0]
+
+    def drop_plans(self) -> None:
+        """Nothing is kept between calls."""
+
+    def __call__(self, a: torch.Tensor, c: torch.Tensor, epilogue: int = _lib.EPI_NONE, residual: Optional[torch.Tensor] = None,
+                 m_dev: Optional[torch.Tensor] = None, m_max: Optional[int] = None, status: Optional[torch.Tensor] = None) -> None:
+        """c = epilogue(a W^T); a [rows, in] bf16 or fp32, c [rows, out] (out / 2 with EPI_SWIGLU) bf16 or fp32, residual as c (EPI_RES; it
+        may be c).  Rows may lie any stride apart."""
+        m = a.shape[0] if m_max is None else m_max
+        wide = self.out_features // 2 if epilogue == _lib.EPI_SWIGLU else self.out_features
+        if a.dim() != 2 or a.shape[0] < m or a.shape[1] != self.in_features or c.dim() != 2 or c.shape[0] < m or c.shape[1] != wide:
+            raise _lib.RedrafterError(f"input {tuple(a.shape)}, output {tuple(c.shape)}: [rows, {self.in_features}] and [rows, {wide}] are wanted")
+        for t in (a, c) + ((residual,) if residual is not None else ()):
+            if t.device != self.codes.device or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise _lib.RedrafterError("rows of consecutive features on the weight's device are wanted")
+        if residual is not None and (residual.dim() != 2 or residual.shape[0] < m or residual.shape[1] != wide or residual.dtype != c.dtype):
+            raise _lib.RedrafterError("the residual has the output's shape and type")
+        if self.codes.is_cuda and self.codes.device.index != torch._C._cuda_getDevice():
+            raise _lib.RedrafterError(f"the weight lies on {self.codes.device}, which is not the current device")
+        k16 = self.codes.shape[1]
+        codes = torch.empty(m, k16, dtype=torch.int8, device=a.device)
+        scales = torch.empty(m, dtype=torch.float32, device=a.device)
+
+        def ld(t: torch.Tensor) -> int:
+            return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+        _lib.call("rd_linear_int8", _lib.dtype_code(a.dtype), _lib.ptr(a), ld(a), _lib.ptr(codes), k16, _lib.ptr(scales), _lib.ptr(self.codes), k16,
+                  _lib.ptr(self.scales), _lib.dtype_code(c.dtype), _lib.ptr(c), ld(c), _lib.ptr(residual), 0 if residual is None else ld(residual), m,
+                  _lib.ptr(m_dev), self.out_features, self.in_features, epilogue, _lib.ptr(status), _lib.stream())
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, m_dev: Optional[torch.Tensor] = None) -> None:
+    """Rows x [rows, k] (bf16 or fp32) as 8-bit integers: codes [rows, at least k, a multiple of 16] int8, contiguous, and scales [rows] fp32;
+    columns past k become 0."""
+    m, k = x.shape
+    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[0] < m or codes.shape[1] < k or codes.shape[1] % 16 or not codes.is_contiguous():
+        raise _lib.RedrafterError(f"codes: contiguous int8 [{m}, a multiple of 16 from {k} on] is wanted")
+    if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] < m or not scales.is_contiguous() or (k > 1 and x.stride(1) != 1):
+        raise _lib.RedrafterError("scales: contiguous fp32, one for each row; the values of a row lie one after another")
+    if x.is_cuda and (x.device != codes.device or x.device != scales.device or x.device.index != torch._C._cuda_getDevice()):
+        raise _lib.RedrafterError("rows, codes and scales lie on the current device")
+    _lib.call("rd_quant_rows", _lib.dtype_code(x.dtype), _lib.ptr(x), x.stride(0) if m > 1 else k, _lib.ptr(codes), codes.shape[1], _lib.ptr(scales), m,
+              _lib.ptr(m_dev), k, _lib.stream())
+
+
 class PendingRows(NamedTuple):
     """Rows that a projection may have left as shares of K: residual + the shares in parts."""
 
