@@ -1,10 +1,15 @@
 // Attention over a key/value cache held in codes of 8 or 4 bits (cache_quant.cu): softmax(scale Q K^T) V with
 // K = scale_k (code - zero_k), V likewise, a scale and a zero for each token of a head.
 //
-// attention_quant_rows_kernel: one CTA per (new token, head).  A warp
+// attention_quant_rows_kernel: one CTA per (new token, head), for 32-bit queries and heads that the other kernels do not have.  A warp
 // takes 32 keys at a time, a key each for the scores, then all of them together for the values, a lane some features; running
 // maximum and sum in fp32.  The score is scale_k (q . code - zero_k sum q), the value's weight p scale_v.
+#include <atomic>
+
+#include <cuda_fp16.h>
+
 #include "quant.cuh"
+#include "umma.cuh"
 
 namespace {
 
@@ -130,11 +135,83 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const
   }
 }
 
+#include "attention_quant_few.cuh"
+
+// Lets a kernel have its dynamic shared memory on the current device; once for each.
+template <auto Kernel>
+bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) {
+    rd_set_last_cuda_error((int)err);
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+  }();
+  return n;
+}
+
+// The few-rows kernel serves 16-bit queries of heads of 64 or 128 features whose group has at most kFewRows rows.
+struct FewPlan {
+  int rows;          // of an item: 8 or 16; 0: not for this call
+  int keys, slots;   // of a tile; CTAs at most
+  int64_t items;     // bound of their number
+};
+FewPlan few_plan(int dtype, int bits, int B, int nh, int nkv, int hd, int max_new, int max_kv) {
+  FewPlan p{0, 0, 0, 0};
+  const int64_t rows = (int64_t)max_new * (nh / nkv);
+  if (dtype != RD_BF16 || (hd != 64 && hd != 128) || rows > kFewRows) return p;
+  p.rows = rows <= 8 ? 8 : 16;
+  p.keys = kTileBytes * 8 / (hd * bits);
+  p.slots = sm_count() * (p.rows == 8 ? 2 : 1);
+  const int64_t tiles = ((int64_t)max_kv + p.keys - 1) / p.keys + 1, chains = (int64_t)B * nkv;  // one more: rows begin inside a tile
+  const int64_t all = chains * ((tiles + kFewWarps - 1) / kFewWarps);
+  p.items = all < chains + 4 * p.slots ? all : chains + 4 * p.slots;
+  return p;
+}
+// chains that no call cuts need no workspace
+bool few_cut(const FewPlan& p, int B, int nkv) { return p.items > (int64_t)B * nkv; }
+
+template <int HD, int BITS, int NT>
+int launch_few(const Args& a, const FewPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
+  constexpr auto kernel = attention_quant_few_kernel<HD, BITS, NT>;
+  using Sm = FewSmem<HD, BITS, NT>;
+  RD_REQUIRE(allow_smem<kernel>(Sm::kBytes), RD_ERR_LAUNCH);
+  CUtensorMap mk, mv;
+  const int64_t lines = (int64_t)a.B * a.nkv * a.max_len * (HD * BITS / 8) / 128;
+  RD_REQUIRE(lines <= 0x7fffffff, RD_ERR_SIZE);
+  RD_REQUIRE(rd_umma::make_byte_map(&mk, a.k_codes, lines, 128, 128, kTileBytes / 128) && rd_umma::make_byte_map(&mv, a.v_codes, lines, 128, 128, kTileBytes / 128),
+             RD_ERR_ARG);
+  const bool cut = few_cut(p, a.B, a.nkv);
+  int* header = (int*)workspace;
+  float* partial = cut ? (float*)((uint8_t*)workspace + kFewHeader) : nullptr;
+  const unsigned grid = (unsigned)(p.items < p.slots ? p.items : p.slots);
+  cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kFewThreads), Sm::kBytes, s, 1, mk, mv, a, partial, p.slots, cut ? header : nullptr, status);
+  RD_CHECK_CHAINED(err);
+  if (!cut) return RD_OK;
+  err = rd::launch_chained(attention_quant_merge_kernel<HD>, dim3((unsigned)((a.nkv * p.rows + 7) / 8), (unsigned)a.B), dim3(256), 0, s, 1, a, (const float*)partial,
+                           (const int*)header, p.keys, p.rows);
+  RD_CHECK_CHAINED(err);
+  return RD_OK;
+}
+
 }  // namespace
 
 extern "C" int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m_max, int B, int nh, int nkv, int hd, int max_new, int max_kv) {
   if ((dtype != RD_F32 && dtype != RD_BF16) || (bits != 4 && bits != 8) || m_max < 0 || B < 0 || nh < 1 || nkv < 1 || hd < 1 || max_new < 0 || max_kv < 0) return RD_ERR_ARG;
   if (nh % nkv != 0 || B == 0 || m_max == 0 || max_new == 0) return 0;
+  const FewPlan p = few_plan(dtype, bits, B, nh, nkv, hd, max_new, max_kv);
+  if (p.rows && few_cut(p, B, nkv)) return kFewHeader + p.items * few_item_floats(hd, p.rows) * 4;
   return 0;
 }
 
@@ -161,7 +238,16 @@ extern "C" int rd_attention_quant(int dtype, int bits, const void* q, int64_t ld
   RD_REQUIRE(need <= workspace_bytes, RD_ERR_CAPACITY);
   RD_REQUIRE(need == 0 || workspace, RD_ERR_ARG);
   RD_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, RD_ERR_ALIGN);
-  (void)status;
+  const FewPlan few = few_plan(dtype, bits, B, nh, nkv, hd, max_new, max_kv);
+  if (few.rows != 0 && max_kv > 0) {
+    cudaStream_t s = (cudaStream_t)stream;
+    if (hd == 128) {
+      if (bits == 4) return few.rows == 8 ? launch_few<128, 4, 1>(a, few, workspace, status, s) : launch_few<128, 4, 2>(a, few, workspace, status, s);
+      return few.rows == 8 ? launch_few<128, 8, 1>(a, few, workspace, status, s) : launch_few<128, 8, 2>(a, few, workspace, status, s);
+    }
+    if (bits == 4) return few.rows == 8 ? launch_few<64, 4, 1>(a, few, workspace, status, s) : launch_few<64, 4, 2>(a, few, workspace, status, s);
+    return few.rows == 8 ? launch_few<64, 8, 1>(a, few, workspace, status, s) : launch_few<64, 8, 2>(a, few, workspace, status, s);
+  }
   const dim3 grid(max_new, nh, B);
   cudaError_t err;
   auto run = [&](auto kern) { err = rd::launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a); };

@@ -1,0 +1,572 @@
+// Attention over a cache in codes for few query rows to a key/value head (a decode step: the query heads of a group times the new tokens
+// of a row, up to 16): included by attention_quant.cu.
+//
+// Such a call is bound by the bytes of the codes.  A warp takes a tile of keys at a time (2 KB of key codes, 2 KB of value codes, brought by TMA into
+// a ring of its own) and multiplies it on the warp-level tensor cores, codes as they lie: a code in the low bits of a 16-bit word is
+// the fp16 number code * 2^-24, a code four bits higher 16 times that, so two of them are formed by one masking instruction.  (tcgen05 would want
+// the operands in shared memory or TMEM: writing the unpacked codes there costs more than these products, 8 columns wide.)
+//   S^T = K Q^T   A: 16 keys x 16 features of codes, B: 8 query rows, scaled by a power of two to fp16 (bf16's 8 bits fit) and, where the codes
+//                 are 16 times too large, by 1/16.  score = scale_k (S - zero_k sum q).
+//   O^T += V^T W  A: 16 features x 16 keys of codes minus their zeros (exact in fp16), B: W = p scale_v / r 2^14 in fp16, where r is the
+//                 largest value scale so far: weights keep fp16's 11 bits down to 2^-28 of the largest.
+// The accumulators' layouts fit: a lane holds the same query columns in S^T and in O^T, so the running maximum and sum need no
+// exchange but the maximum's over the 8 lanes of a column, and only where some lane's exceeds it; the weights become a B operand by
+// movmatrix.
+// Shared memory lies in TMA's 128-byte swizzle, and the 16 keys of a product are taken in an order (Shape::key) in which both the reads of K
+// (16 bytes of 8 keys) and of V (4 to 16 bytes of 4 keys) touch every bank once.
+//
+// Work is cut on the device, where the rows' lengths are known: chains (row, key/value head) in chunks of equal length.
+
+constexpr int kFewWarps = 8;
+constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kFewStages = 3;
+constexpr int kTileBytes = 2048;  // of key codes, and of value codes
+constexpr int kFewRows = 16;      // query rows at most
+
+template <int HD, int BITS>
+struct Shape {
+  static constexpr int kRowBytes = HD * BITS / 8;
+  static constexpr int kKeys = kTileBytes / kRowBytes;  // of a tile: 16, 32 or 64
+  static constexpr int kWords = kRowBytes / 16;         // 32-bit words of a key that a lane holds for S^T
+  static constexpr int kPer = 32 / BITS;                // codes of a word
+  static constexpr int kSteps = HD / 16;                // products along the features
+  static constexpr int kStage = 2 * kTileBytes + 2 * 64 * 4;  // codes, then the parameters of up to 64 keys and values
+  // the key of a sub-tile of 16 whose scores are row i of a product
+  static __device__ __forceinline__ int key(int i) {
+    const int i0 = i & 1, i1 = (i >> 1) & 1, i2 = (i >> 2) & 1, i3 = i >> 3;
+    if constexpr (kRowBytes == 128) return i0 | (i1 << 1) | ((i2 ^ i0) << 2) | (i3 << 3);
+    else if constexpr (kRowBytes == 64) return i0 | (i3 << 1) | (i1 << 2) | (i2 << 3);
+    else return i0 | (i1 << 1) | (i3 << 2) | (i2 << 3);
+  }
+  // byte `at` of key `k` of a tile, in the swizzled tile
+  static __device__ __forceinline__ uint32_t place(int k, int at) {
+    const uint32_t b = k * kRowBytes + at;
+    return b ^ ((b >> 3) & 0x70);
+  }
+  // first feature of word w of a lane with t = lane % 4
+  static __device__ __forceinline__ int feature(int t, int w) {
+    if constexpr (kWords == 8) return (w >> 2) * 64 + t * 16 + (w & 3) * 4;
+    else return t * (HD / 4) + w * kPer;
+  }
+};
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(rd_umma::smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(rd_umma::smem_u32(bar))
+               : "memory");
+}
+
+// Rounds of row b: its tiles (at multiples of `keys` slots) over the warps of a CTA.
+__device__ __forceinline__ int rounds_of(const Args& a, int b, int keys) {
+  const Row r = row_of(a, b);
+  if (r.n_new <= 0 || r.end <= 0) return 0;
+  const int tiles = (r.first + r.end + keys - 1) / keys - r.first / keys;
+  return (tiles + kFewWarps - 1) / kFewWarps;
+}
+// Items of all rows at this chunk; one warp.
+__device__ __forceinline__ int count_items(const Args& a, int keys, int chunk) {
+  int n = 0;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) n += (rounds_of(a, b, keys) + chunk - 1) / chunk;
+  return rd::warp_sum_i(n) * a.nkv;
+}
+// The chunk of a launch of `slots` CTAs; one warp, the same answer in every CTA.  One item to a CTA if that fills them evenly: the smallest chunk that
+// leaves no more items than CTAs is at most 1.25 times what an even share would be.  Otherwise four items to a CTA, one after another.
+__device__ __forceinline__ int choose_chunk(const Args& a, int keys, int slots) {
+  int total = 0, most = 0;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+    const int r = rounds_of(a, b, keys);
+    total += r;
+    most = max(most, r);
+  }
+  total = rd::warp_sum_i(total);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (most == 0) return 1;
+  const int64_t work = (int64_t)total * a.nkv;
+  int lo = (int)max((work + slots - 1) / slots, (int64_t)1), hi = min(most, lo + lo / 4);  // a chunk in (lo - 1, hi] is looked for
+  if (lo >= most) return most;
+  if (count_items(a, keys, hi) > slots) return (int)max((work + 4 * slots - 1) / (4 * slots), (int64_t)1);
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (count_items(a, keys, mid) <= slots) hi = mid;
+    else lo = mid + 1;
+  }
+  return hi;
+}
+struct Item {
+  int b, head, index, of, before;  // row, key/value head, chunk of the chain, chunks of the chain, items of the rows before
+};
+// Item i; one warp, all lanes the same answer.  b = -1: there are fewer.  The heads of a chunk come one after another.
+__device__ __forceinline__ Item find_item(const Args& a, int keys, int chunk, int i) {
+  Item it{-1, 0, 0, 0, 0};
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int chunks = b0 + lane < a.B ? (rounds_of(a, b0 + lane, keys) + chunk - 1) / chunk : 0;
+    int sum = chunks * a.nkv;
+    const int mine = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + sum > i);
+    if (past != 0) {
+      const int who = __ffs(past) - 1;
+      const int start = before + __shfl_sync(0xffffffffu, sum - mine, who);
+      it.of = __shfl_sync(0xffffffffu, chunks, who);
+      it.b = b0 + who;
+      it.before = start;
+      it.index = (i - start) / a.nkv;
+      it.head = (i - start) - it.index * a.nkv;
+      return it;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return it;
+}
+
+// The workspace: a header of one int (the chunk), then for every item its rows' unnormalised outputs, maxima (base 2) and sums.
+constexpr int kFewHeader = 256;
+__host__ __device__ constexpr int64_t few_item_floats(int hd, int rows) { return (int64_t)rows * (hd + 2); }
+
+template <int HD, int BITS, int NT>
+struct FewSmem {
+  static constexpr int kRing = kFewWarps * kFewStages * Shape<HD, BITS>::kStage;
+  static constexpr int kMerge = kFewWarps * 8 * NT * (HD + 4) * 4;  // outputs, then maxima and sums, of all warps
+  static constexpr int kBytes = 1024 + (kRing > kMerge ? kRing : kMerge) + kFewWarps * kFewStages * 8 + 64;
+};
+
+template <int HD, int BITS, int NT>
+__global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
+    attention_quant_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a, float* partial, int slots,
+                               int* header, int32_t* status) {
+  using S = Shape<HD, BITS>;
+  constexpr int kKeys = S::kKeys, kSub = kKeys / 16, kMT = HD / 16;
+  constexpr int kRows = 8 * NT;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  using Sm = FewSmem<HD, BITS, NT>;
+  constexpr int kData = Sm::kRing > Sm::kMerge ? Sm::kRing : Sm::kMerge;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kData);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(bars + kFewWarps * kFewStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint64_t* full = bars + warp * kFewStages;
+  // tiles of all warps first (their swizzle wants 1024 bytes of alignment), then the parameters
+  uint8_t* codes = smem + warp * kFewStages * 2 * kTileBytes;
+  uint32_t* params = reinterpret_cast<uint32_t*>(smem + kFewWarps * kFewStages * 2 * kTileBytes) + warp * kFewStages * 128;
+  rd::pdl_launch_dependents();
+  if (threadIdx.x == 0) *gave_up = 0;
+  if (lane == 0) {
+    for (int s = 0; s < kFewStages; ++s) rd_umma::mbar_init(&full[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  rd::pdl_wait();
+  const int chunk = choose_chunk(a, kKeys, slots);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && header != nullptr) *header = chunk;
+  const int group = a.nh / a.nkv;
+  const int64_t plane_rows = (int64_t)a.B * a.nkv * a.max_len;
+  uint32_t used = 0;  // tiles that this warp has waited for so far: stage and phase
+  bool ok = true;
+  for (int item = blockIdx.x; ok; item += gridDim.x) {
+    const Item it = find_item(a, kKeys, chunk, item);
+    if (it.b < 0) break;
+    const Row r = row_of(a, it.b);
+    const int64_t chain = (int64_t)it.b * a.nkv + it.head;
+    const int64_t slot0 = chain * a.max_len;  // row of the planes
+    const int tile_first = r.first / kKeys, tile_end = (r.first + r.end + kKeys - 1) / kKeys;
+    const int from = tile_first + it.index * chunk * kFewWarps, to = min(tile_end, from + chunk * kFewWarps);
+    const int mine = from + warp < to ? (to - from - warp + kFewWarps - 1) / kFewWarps : 0;
+    auto load = [&](int i) {  // tile i of this warp, one lane
+      const uint32_t stage = (used + i) % kFewStages;
+      const int64_t row = slot0 + (int64_t)(from + warp + i * kFewWarps) * kKeys;
+      const uint32_t n = (uint32_t)min((int64_t)kKeys, plane_rows - row) * 4;
+      rd_umma::mbar_expect_tx(&full[stage], 2 * kTileBytes + 2 * n);
+      const int line = (int)(row / (128 / S::kRowBytes));
+      rd_umma::tma_load_2d(codes + stage * 2 * kTileBytes, &map_k, &full[stage], 0, line);
+      rd_umma::tma_load_2d(codes + stage * 2 * kTileBytes + kTileBytes, &map_v, &full[stage], 0, line);
+      bulk_load(params + stage * 128, a.k_params + row, n, &full[stage]);
+      bulk_load(params + stage * 128 + 64, a.v_params + row, n, &full[stage]);
+    };
+    if (rd::elect_one())
+      for (int i = 0; i < kFewStages && i < mine; ++i) load(i);
+    __syncwarp();
+
+    // the queries: row n * 8 + g is head (row % group) of new token row / group; a lane holds its share of the features
+    const int rows = r.n_new * group;
+    uint32_t q[NT][S::kSteps][2];
+    float q_sum[NT][2], unit[NT][2];  // of the columns 2 t, 2 t + 1 of a block of rows: sum q, and what a score is to be multiplied with
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = n * 8 + g;
+      float x[HD / 4];
+      const bool live = row < rows;
+      const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + (int64_t)(r.start + (live ? row / group : 0)) * a.ldq + (it.head * group + (live ? row % group : 0)) * HD;
+#pragma unroll
+      for (int w = 0; w < S::kWords; ++w) {
+        const int d = S::feature(t, w);
+#pragma unroll
+        for (int e = 0; e < S::kPer; e += 4) {
+          const uint2 u = live ? *reinterpret_cast<const uint2*>(src + d + e) : make_uint2(0u, 0u);
+          x[w * S::kPer + e] = __uint_as_float(u.x << 16), x[w * S::kPer + e + 1] = __uint_as_float(u.x & 0xffff0000u);
+          x[w * S::kPer + e + 2] = __uint_as_float(u.y << 16), x[w * S::kPer + e + 3] = __uint_as_float(u.y & 0xffff0000u);
+        }
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the row's largest to [2^14, 2^15): what is below 2^-38 of it is lost.  2^(141 - e) and its inverse, in two factors each, because e
+      // runs over all of fp32's exponents.
+      const int e = top > 0.f && top < INFINITY ? (int)(__float_as_uint(top) >> 23) : 141;
+      const int up = 141 - e, h1 = up / 2, h2 = up - h1;
+      const float f1 = __uint_as_float((uint32_t)(127 + h1) << 23), f2 = __uint_as_float((uint32_t)(127 + h2) << 23);
+      const float i1 = __uint_as_float((uint32_t)(127 - h1) << 23), i2 = __uint_as_float((uint32_t)(127 - h2) << 23);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < S::kWords; ++w) {
+        float* y = x + w * S::kPer;
+#pragma unroll
+        for (int i = 0; i < S::kPer; ++i) y[i] = y[i] * f1 * f2;
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // codes i and i + 4 of a word share a register; those of odd i are 16 times too large
+            const float f = (i & 1) ? 0.0625f : 1.f;
+            const uint32_t u = pack_f16(y[i] * f, y[i + 4] * f);
+            q[n][2 * w + i / 2][i & 1] = u;
+            sum += (__half2float(__ushort_as_half((unsigned short)u)) + __half2float(__ushort_as_half((unsigned short)(u >> 16)))) / f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t u = pack_f16(y[i], y[i + 2]);
+            q[n][w][i] = u;
+            sum += __half2float(__ushort_as_half((unsigned short)u)) + __half2float(__ushort_as_half((unsigned short)(u >> 16)));
+          }
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      // log2(e) scale 2^24 / the queries' factor: scores in base 2
+      const float back = a.scale * 1.44269504f * 16777216.f * i1 * i2;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        q_sum[n][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + c));
+        unit[n][c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c));
+      }
+    }
+
+    float o[NT][kMT][4], m[NT][2], l[NT][2], ref = 0.f, inv_ref = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const uint32_t stage = (used + i) % kFewStages;
+      if (!rd_umma::mbar_wait(&full[stage], ((used + i) / kFewStages) & 1)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* kt = codes + stage * 2 * kTileBytes;
+      const uint8_t* vt = kt + kTileBytes;
+      const uint32_t *kp = params + stage * 128, *vp = kp + 64;
+      const int j0 = (from + warp + i * kFewWarps) * kKeys - r.first;  // key of the tile's first slot
+      const bool whole = j0 >= 0 && j0 + kKeys <= r.base;              // every row sees every key
+      float s[NT][kSub][4], sv[kSub][2];
+      bool more = false;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        const int key[2] = {u * 16 + S::key(g), u * 16 + S::key(g + 8)};
+        uint32_t w[2][S::kWords];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if constexpr (S::kWords == 2) {
+            *reinterpret_cast<uint2*>(w[x]) = *reinterpret_cast<const uint2*>(kt + S::place(key[x], t * 8));
+          } else {
+#pragma unroll
+            for (int y = 0; y < S::kWords / 4; ++y)
+              *reinterpret_cast<uint4*>(w[x] + 4 * y) = *reinterpret_cast<const uint4*>(kt + S::place(key[x], t * 16 + y * 64));
+          }
+        }
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+        for (int y = 0; y < S::kWords; ++y) {
+          if constexpr (BITS == 4) {
+            const uint32_t b0 = w[0][y] >> 8, b1 = w[1][y] >> 8;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_f16(acc[n], w[0][y] & 0x000f000fu, w[1][y] & 0x000f000fu, w[0][y] & 0x00f000f0u, w[1][y] & 0x00f000f0u, q[n][2 * y][0], q[n][2 * y][1]);
+              mma_f16(acc[n], b0 & 0x000f000fu, b1 & 0x000f000fu, b0 & 0x00f000f0u, b1 & 0x00f000f0u, q[n][2 * y + 1][0], q[n][2 * y + 1][1]);
+            }
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma_f16(acc[n], w[0][y] & 0x00ff00ffu, w[1][y] & 0x00ff00ffu, (w[0][y] >> 8) & 0x00ff00ffu, (w[1][y] >> 8) & 0x00ff00ffu, q[n][y][0], q[n][y][1]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t p = kp[key[x]];
+          const float sk = param_scale(p), zk = (float)param_zero(p) * 0x1p-24f;
+          sv[u][x] = param_scale(vp[key[x]]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) s[n][u][2 * x + c] = fmaf(-zk, q_sum[n][c], acc[n][2 * x + c]) * sk;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = j0 + key[x];
+            const bool there = j >= 0 && j < r.end;
+            if (!there) sv[u][x] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int row = n * 8 + 2 * t + c;
+                if (!(there && row < rows && (j < r.base || sees(a, r, row / group, j)))) s[n][u][2 * x + c] = -INFINITY;
+              }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          more |= sv[u][x] > ref;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) more |= s[n][u][2 * x] > m[n][0] || s[n][u][2 * x + 1] > m[n][1];
+        }
+      }
+      if (__any_sync(0xffffffffu, more)) {
+        // a larger maximum or a larger value scale: what has been summed so far is brought to it
+        float top = ref, mx[NT][2];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) top = fmaxf(top, fmaxf(sv[u][0], sv[u][1]));
+#pragma unroll
+        for (int o2 = 4; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+        const float back = ref * __frcp_rn(fmaxf(top, 0x1p-100f));
+        ref = top;
+        inv_ref = 16384.f / fmaxf(ref, 0x1p-100f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float f[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            mx[n][c] = m[n][c];
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) mx[n][c] = fmaxf(mx[n][c], fmaxf(s[n][u][c], s[n][u][2 + c]));
+#pragma unroll
+            for (int o2 = 4; o2 < 32; o2 <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], o2));
+            f[c] = m[n][c] == -INFINITY ? 0.f : ex2((m[n][c] - mx[n][c]) * unit[n][c]);
+            m[n][c] = mx[n][c];
+            l[n][c] *= f[c];
+            f[c] *= back;
+          }
+#pragma unroll
+          for (int k = 0; k < kMT; ++k) o[n][k][0] *= f[0], o[n][k][1] *= f[1], o[n][k][2] *= f[0], o[n][k][3] *= f[1];
+        }
+      }
+      float off[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) off[n][c] = m[n][c] == -INFINITY ? 0.f : -m[n][c] * unit[n][c];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float f = sv[u][x] * inv_ref;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float p0 = ex2(fmaf(s[n][u][2 * x], unit[n][0], off[n][0])), p1 = ex2(fmaf(s[n][u][2 * x + 1], unit[n][1], off[n][1]));
+            l[n][0] += p0;
+            l[n][1] += p1;
+            float w0 = p0 * f, w1 = p1 * f;
+            if (!whole) w0 = p0 == 0.f ? 0.f : w0, w1 = p1 == 0.f ? 0.f : w1;  // a hidden value counts for nothing, NaN or not
+            b[n][x] = transpose8x8(pack_f16(w0, w1));
+          }
+        }
+        // values of the keys whose weights this lane's B registers hold: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        uint32_t z[2], z16[2];
+        constexpr int kVWords = S::kRowBytes / 32;  // words of a key that a lane holds: features g * HD / 8 ..
+        uint32_t w[4][kVWords];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = u * 16 + S::key(2 * t + (x & 1) + 8 * (x >> 1));
+          uint32_t zero = param_zero(vp[key]);
+          if (!whole) {
+            const int j = j0 + key;
+            if (j < 0 || j >= r.end) zero = 0;  // whatever lies there
+          }
+          if (x & 1) z[x >> 1] |= zero << 16;
+          else z[x >> 1] = zero;
+          const uint8_t* src = vt + S::place(key, g * (S::kRowBytes / 8));
+          if constexpr (kVWords == 1) w[x][0] = *reinterpret_cast<const uint32_t*>(src);
+          else if constexpr (kVWords == 2) *reinterpret_cast<uint2*>(w[x]) = *reinterpret_cast<const uint2*>(src);
+          else *reinterpret_cast<uint4*>(w[x]) = *reinterpret_cast<const uint4*>(src);
+        }
+        z16[0] = z[0] << 4, z16[1] = z[1] << 4;
+#pragma unroll
+        for (int y = 0; y < kVWords; ++y) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // two bytes of each of two keys: four features of 4 bits, or two of 8
+            const uint32_t c0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), c1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
+            if constexpr (BITS == 4) {
+              const uint32_t d0 = c0 >> 8, d1 = c1 >> 8;
+              const uint32_t e0 = sub_f16x2(c0 & 0x000f000fu, z[0]), e1 = sub_f16x2(c0 & 0x00f000f0u, z16[0]);
+              const uint32_t e2 = sub_f16x2(c1 & 0x000f000fu, z[1]), e3 = sub_f16x2(c1 & 0x00f000f0u, z16[1]);
+              const uint32_t f0 = sub_f16x2(d0 & 0x000f000fu, z[0]), f1 = sub_f16x2(d0 & 0x00f000f0u, z16[0]);
+              const uint32_t f2 = sub_f16x2(d1 & 0x000f000fu, z[1]), f3 = sub_f16x2(d1 & 0x00f000f0u, z16[1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma_f16(o[n][4 * y + 2 * half], e0, e1, e2, e3, b[n][0], b[n][1]);
+                mma_f16(o[n][4 * y + 2 * half + 1], f0, f1, f2, f3, b[n][0], b[n][1]);
+              }
+            } else {
+              const uint32_t e0 = sub_f16x2(c0 & 0x00ff00ffu, z[0]), e1 = sub_f16x2((c0 >> 8) & 0x00ff00ffu, z[0]);
+              const uint32_t e2 = sub_f16x2(c1 & 0x00ff00ffu, z[1]), e3 = sub_f16x2((c1 >> 8) & 0x00ff00ffu, z[1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * y + half], e0, e1, e2, e3, b[n][0], b[n][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // every lane has read its part of the stage
+      if (i + kFewStages < mine && rd::elect_one()) load(i + kFewStages);
+      __syncwarp();
+    }
+    used += mine;
+    if (!ok) *gave_up = 1;
+
+    // The warps' results meet in shared memory, where the rings were: no copy is under way any more.
+    __syncthreads();
+    if (*gave_up) {
+      ok = false;
+      break;
+    }
+    float* so = reinterpret_cast<float*>(smem);                       // [warp][row][HD + 2]: a row's stride shifts the banks
+    float* ss = so + kFewWarps * kRows * (HD + 2);                    // [warp][row][2]
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float sum = l[n][c];
+#pragma unroll
+        for (int o2 = 4; o2 < 32; o2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+        const int row = n * 8 + 2 * t + c;
+        // 2^24 / 2^14: the codes' factor and the weights'
+        float* dst = so + (warp * kRows + row) * (HD + 2);
+#pragma unroll
+        for (int k = 0; k < kMT; ++k) {
+          dst[g * (HD / 8) + 2 * k] = o[n][k][c] * 1024.f * ref;
+          dst[g * (HD / 8) + 2 * k + 1] = o[n][k][2 + c] * (BITS == 4 ? 64.f : 1024.f) * ref;
+        }
+        if (g == 0) {
+          ss[(warp * kRows + row) * 2] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * unit[n][c];
+          ss[(warp * kRows + row) * 2 + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < min(rows, kRows) * HD; x += kFewThreads) {
+      const int row = x / HD, d = x - row * HD;
+      float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, ss[(w * kRows + row) * 2]);
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        const float mw = ss[(w * kRows + row) * 2];
+        const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
+        sum += f * ss[(w * kRows + row) * 2 + 1];
+        v += mw == -INFINITY ? 0.f : f * so[(w * kRows + row) * (HD + 2) + d];
+      }
+      if (it.of == 1) {
+        const int64_t at = ((int64_t)(r.start + row / group) * a.nh + it.head * group + row % group) * HD + d;
+        ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
+      } else {
+        float* dst = partial + item * few_item_floats(HD, kRows) + row * (HD + 2);
+        dst[d] = v;
+        if (d == 0) dst[HD] = top, dst[HD + 1] = sum;
+      }
+    }
+    __syncthreads();
+    // The next item's copies go where generic writes have just been
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+  }
+  if (!ok) {
+    if (status && threadIdx.x == 0) atomicExch(status, 41);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land
+  }
+}
+
+// Sums the chunks of the chains that have several.  A warp for each query row of each chain.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a, const float* partial, const int* header, int keys, int item_rows) {
+  rd::pdl_launch_dependents();
+  rd::pdl_wait();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, group = a.nh / a.nkv;
+  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5);  // (key/value head, row)
+  const int head = unit / item_rows, row = unit - head * item_rows;
+  const int chunk = *reinterpret_cast<const volatile int*>(header);
+  const Row r = row_of(a, b);
+  if (head >= a.nkv || row >= r.n_new * group) return;
+  const int n = (rounds_of(a, b, keys) + chunk - 1) / chunk;
+  if (n <= 1) return;
+  int before = 0;
+  for (int x = lane; x < b; x += 32) before += (rounds_of(a, x, keys) + chunk - 1) / chunk;
+  before = rd::warp_sum_i(before) * a.nkv;
+  const int64_t step = few_item_floats(HD, item_rows) * a.nkv;
+  const float* p = partial + (before + head) * few_item_floats(HD, item_rows) + row * (HD + 2);
+  float top = -INFINITY;
+  for (int c = lane; c < n; c += 32) top = fmaxf(top, p[c * step + HD]);
+  top = rd::warp_max(top);
+  float sum = 0.f, v[HD / 32] = {};
+#pragma unroll 4
+  for (int c = 0; c < n; ++c) {
+    const float* x = p + c * step;
+    const float mw = x[HD];
+    const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
+    sum += f * x[HD + 1];
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) v[k] += mw == -INFINITY ? 0.f : f * x[k * 32 + lane];
+  }
+  __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((int64_t)(r.start + row / group) * a.nh + head * group + row % group) * HD;
+#pragma unroll
+  for (int k = 0; k < HD / 32; ++k) dst[k * 32 + lane] = __float2bfloat16_rn(sum == 0.f ? 0.f : v[k] / sum);
+}
