@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const
 }
 
 #include "attention_quant_few.cuh"
+#include "attention_quant_many.cuh"
 
 // Lets a kernel have its dynamic shared memory on the current device; once for each.
 template <auto Kernel>
@@ -205,6 +206,40 @@ int launch_few(const Args& a, const FewPlan& p, void* workspace, int32_t* status
   return RD_OK;
 }
 
+// The many-rows kernel serves the other 16-bit calls of such heads.
+struct ManyPlan {
+  bool here;
+  int n_split;
+};
+ManyPlan many_plan(int dtype, int B, int nh, int nkv, int hd, int max_new, int max_kv) {
+  ManyPlan p{dtype == RD_BF16 && (hd == 64 || hd == 128) && (int64_t)max_new * (nh / nkv) > kFewRows, 1};
+  if (!p.here) return p;
+  // Shares of the keys where the query tiles leave CTAs idle: enough to fill two to an SM, each of at least four tiles.
+  const int64_t chains = (int64_t)B * nkv * (((int64_t)max_new * (nh / nkv) + kManyRows - 1) / kManyRows), slots = 2 * sm_count();
+  if (2 * chains >= slots) return p;
+  const int64_t by_fill = slots / chains, by_length = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys / 4;
+  int64_t n = by_fill < by_length ? by_fill : by_length;
+  n = n < kManyMaxSplit ? n : kManyMaxSplit;
+  p.n_split = n > 1 ? (int)n : 1;
+  return p;
+}
+
+template <int HD, int BITS>
+int launch_many(const Args& a, const ManyPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
+  constexpr auto kernel = attention_quant_many_kernel<HD, BITS>;
+  RD_REQUIRE(allow_smem<kernel>(ManySmem<HD>::kBytes), RD_ERR_LAUNCH);
+  const int64_t tiles = ((int64_t)a.max_new * (a.nh / a.nkv) + kManyRows - 1) / kManyRows * p.n_split;
+  RD_REQUIRE(tiles <= 0x7fffffff, RD_ERR_SIZE);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)tiles, a.nkv, a.B), dim3(kManyThreads), ManySmem<HD>::kBytes, s, 1, a, (float*)workspace, p.n_split,
+                                       status);
+  RD_CHECK_CHAINED(err);
+  if (p.n_split == 1) return RD_OK;
+  err = rd::launch_chained(attention_quant_merge_shares_kernel<HD>, dim3((unsigned)(((int64_t)a.max_new * a.nh + 7) / 8), a.B), dim3(256), 0, s, 1, a,
+                           (const float*)workspace, p.n_split);
+  RD_CHECK_CHAINED(err);
+  return RD_OK;
+}
+
 }  // namespace
 
 extern "C" int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m_max, int B, int nh, int nkv, int hd, int max_new, int max_kv) {
@@ -212,6 +247,8 @@ extern "C" int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m
   if (nh % nkv != 0 || B == 0 || m_max == 0 || max_new == 0) return 0;
   const FewPlan p = few_plan(dtype, bits, B, nh, nkv, hd, max_new, max_kv);
   if (p.rows && few_cut(p, B, nkv)) return kFewHeader + p.items * few_item_floats(hd, p.rows) * 4;
+  const ManyPlan q = many_plan(dtype, B, nh, nkv, hd, max_new, max_kv);
+  if (q.here && q.n_split > 1) return (int64_t)m_max * nh * q.n_split * (hd + 2) * 4;
   return 0;
 }
 
@@ -247,6 +284,12 @@ extern "C" int rd_attention_quant(int dtype, int bits, const void* q, int64_t ld
     }
     if (bits == 4) return few.rows == 8 ? launch_few<64, 4, 1>(a, few, workspace, status, s) : launch_few<64, 4, 2>(a, few, workspace, status, s);
     return few.rows == 8 ? launch_few<64, 8, 1>(a, few, workspace, status, s) : launch_few<64, 8, 2>(a, few, workspace, status, s);
+  }
+  const ManyPlan many = many_plan(dtype, B, nh, nkv, hd, max_new, max_kv);
+  if (many.here && max_kv > 0) {
+    cudaStream_t s = (cudaStream_t)stream;
+    if (hd == 128) return bits == 4 ? launch_many<128, 4>(a, many, workspace, status, s) : launch_many<128, 8>(a, many, workspace, status, s);
+    return bits == 4 ? launch_many<64, 4>(a, many, workspace, status, s) : launch_many<64, 8>(a, many, workspace, status, s);
   }
   const dim3 grid(max_new, nh, B);
   cudaError_t err;

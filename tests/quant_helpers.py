@@ -74,7 +74,12 @@ def fill(cache, layer, seed, scale=1.0):
 
 def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, scale, weight_step, exp_step=2.0 ** -20):
     """(out, bound): attention in 64 bits over the values that the codes stand for, [tokens, heads * dim], and how far a kernel may be off
-    whose softmax weights are rounded by at most weight_step (relative) beside what fp32 sums of scores cost; a row that sees nothing is 0."""
+    whose softmax weights are rounded by at most weight_step (relative) beside what fp32 sums of scores cost; a row that sees nothing is 0.
+
+    Weights in fp16 have a smallest step besides, which counts where a feature's large weights all meet values of 0.  A weight is p s / r
+    2^8 (2^14 in the kernel for few rows), s the value's scale, r a power of two (the scale) that is no more than the largest scale R of the keys;
+    the largest p is at least 1 and the sum l that the result is divided by too.  Half of fp16's smallest step is 2^-25, so a key adds at
+    most 2^-25 2^-8 r (code - zero) / l <= 2^-33 R (2^bits - 1)."""
     l = cache.layers[layer]
     B, heads, cap, _ = l.k_codes.shape
     hd = cache.head_dim
@@ -82,7 +87,8 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
     m = q.shape[0]
     nh = q.shape[1] // hd
     k, v = values(host(l.k_codes), host(l.k_params), cache.bits), values(host(l.v_codes), host(l.v_params), cache.bits)
-    ks, kz = scale_zero(host(l.k_params))
+    ks = scale_zero(host(l.k_params))[0]
+    vs = np.nan_to_num(scale_zero(host(l.v_params))[0])
     top = 2 ** cache.bits - 1
     out, bound = np.zeros((m, nh, hd)), np.zeros((m, nh, hd))
     for b in range(B):
@@ -105,6 +111,8 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
                 err = (hd + 4) * 2.0 ** -23 * np.abs(x).sum() * 2 * top * ks[b, g, seen].max() * abs(scale) + 2.0 ** -22 * np.abs(sc).max()
                 weight = weight_step + exp_step + 2 * err + seen.size * 2.0 ** -23
                 bound[s + i, h] = weight * (p @ np.abs(v[b, g, seen])) + weight * np.abs(out[s + i, h])
+                if weight_step > 2.0 ** -12:
+                    bound[s + i, h] += seen.size * 2.0 ** -33 * vs[b, g, seen].max() * top
     return out.reshape(m, -1), bound.reshape(m, -1)
 
 
