@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll 1
     for (int i = 0; i < mine; ++i) {
       const uint32_t stage = (used + i) % kFewStages;
-      if (!rd_umma::mbar_wait(&full[stage], ((used + i) / kFewStages) & 1)) {
+      if (!__all_sync(0xffffffffu, rd_umma::mbar_wait(&full[stage], ((used + i) / kFewStages) & 1))) {
         ok = false;
         break;
       }

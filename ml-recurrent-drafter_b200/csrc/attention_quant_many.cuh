@@ -36,6 +36,10 @@ __device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, vol
     if (*stop || clock64() - t0 > (1ll << 31)) return false;
   }
 }
+// by all lanes of a warp, the same answer for all
+__device__ __forceinline__ bool warp_wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, mbar_wait_or(bar, parity, stop));
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(rd_umma::smem_u32(bar)) : "memory");
 }
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       request_v(0);
     }
     for (int t = 0; t < n_tiles; ++t) {
-      if (t >= 2 && !mbar_wait_or(&s_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
+      if (t >= 2 && !warp_wait_or(&s_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 1;
         break;
       }
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         mbar_arrive(&scales_full[t & 3]);
         mbar_arrive(&k_full[t & 1]);
       }
-      if (t >= 2 && !mbar_wait_or(&o_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
+      if (t >= 2 && !warp_wait_or(&o_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 2;
         break;
       }
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
     const int all_see = a.mode == RD_ATTN_CAUSAL ? min(kv_end, r.base + first_token + 1) : min(kv_end, r.base);
     float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
     for (int t = 0; t < n_tiles; ++t) {
-      if (!mbar_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !mbar_wait_or(&s_full[t & 1], (t >> 1) & 1, stop)) {
+      if (!warp_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !warp_wait_or(&s_full[t & 1], (t >> 1) & 1, stop)) {
         ok = false, site = 4;
         break;
       }
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       }
       if (__any_sync(0xffffffffu, t > 0 && keep != 1.f)) {
         // O has to be quiet while it is brought to the new maximum or r
-        if (!mbar_wait_or(&o_full[(t - 1) & 1], ((t - 1) >> 1) & 1, stop)) {
+        if (!warp_wait_or(&o_full[(t - 1) & 1], ((t - 1) >> 1) & 1, stop)) {
           ok = false, site = 5;
           break;
         }
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       }
     }
     if (ok && n_tiles > 0) {
-      ok = mbar_wait_or(&o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, stop);
+      ok = warp_wait_or(&o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, stop);
       if (!ok) site = 6;
     }
     if (ok) {

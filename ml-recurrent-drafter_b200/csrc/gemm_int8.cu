@@ -1,28 +1,69 @@
 // Products of matrices held in 8-bit integers with a scale for each row: C[t, n] = sA[t] sW[n] sum_k A[t, k] W[n, k], and the quantiser of
 // their rows.  A row x of K values: scale = bf16(max |x| / 127) in fp32, code = rint(x / scale) cut to -127 .. 127; the scale's 8 significant
 // bits make fp32's division give the codes of exact arithmetic (cache_quant.cu has the argument).  The sums are integers and exact.
-#include "rd_common.cuh"
+#include <atomic>
+#include <type_traits>
+
+#include "umma.cuh"
 
 namespace {
 
 constexpr int kQuantThreads = 256;
 
-template <typename T>
+// One block a row, 8 values of a thread at a time; rows of up to kQuantHeld * 2048 values stay in registers between the maximum and the
+// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows.  VEC: rows on 16-byte boundaries, K a multiple of 8.
+constexpr int kQuantHeld = 6;
+
+__device__ __forceinline__ uint32_t int8_code(float x, float scale) {
+  return (uint32_t)(int)fminf(fmaxf(rintf(x / scale), -127.f), 127.f) & 0xffu;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int i, int K, float* x) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    const uint4 u = *reinterpret_cast<const uint4*>(row + i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+  } else if constexpr (VEC) {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row + i);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(row + i + 4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = i + e < K ? rd::Num<T>::to_f(row[i + e]) : 0.f;
+  }
+}
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max,
                                                                    const int32_t* m_dev, int K) {
   __shared__ float red[kQuantThreads / 32];
   rd::pdl_wait();
-  rd::pdl_launch_dependents();
+  rd::pdl_launch_dependents();  // after the wait: a product that follows may read what was complete before this kernel began
   const int t = blockIdx.x;
   if (t >= rd::live_rows(m_dev, m_max)) return;
   const T* row = x + (int64_t)t * ldx;
   int8_t* to = codes + (int64_t)t * ld_codes;
-  float top = 0.f;
+  constexpr int kStep = kQuantThreads * 8;
+  const int first = threadIdx.x * 8;
+  float held[kQuantHeld][8], top = 0.f;
   bool odd = false;
-  for (int i = threadIdx.x; i < K; i += kQuantThreads) {
-    const float v = fabsf(rd::Num<T>::to_f(row[i]));
-    odd |= !(v <= 3.402823466e38f);
-    top = fmaxf(top, v);
+  auto look = [&](const float* v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      odd |= !(fabsf(v[e]) <= 3.402823466e38f);
+      top = fmaxf(top, fabsf(v[e]));
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kQuantHeld; ++j)
+    if (first + j * kStep < K) load_row8<T, VEC>(row, first + j * kStep, K, held[j]);
+#pragma unroll
+  for (int j = 0; j < kQuantHeld; ++j)
+    if (first + j * kStep < K) look(held[j]);
+  for (int i = first + kQuantHeld * kStep; i < K; i += kStep) {
+    float v[8];
+    load_row8<T, VEC>(row, i, K, v);
+    look(v);
   }
   if (odd) top = INFINITY;
   top = rd::warp_max(top);
@@ -35,8 +76,23 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, i
   const float scale = __bfloat162float(__float2bfloat16_rn(top / 127.f));
   const bool some = fine && scale > 0.f;
   if (threadIdx.x == 0) scales[t] = fine ? scale : __int_as_float(0x7fffffff);
-  for (int i = threadIdx.x; i < ld_codes; i += kQuantThreads)
-    to[i] = some && i < K ? (int8_t)fminf(fmaxf(rintf(rd::Num<T>::to_f(row[i]) / scale), -127.f), 127.f) : (int8_t)0;
+  auto put = [&](int i, const float* v) {
+    uint2 w = make_uint2(0u, 0u);
+    if (some && v != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.x |= int8_code(v[e], scale) << (8 * e), w.y |= int8_code(v[4 + e], scale) << (8 * e);
+    }
+    *reinterpret_cast<uint2*>(to + i) = w;
+  };
+  // columns past K: codes of zeros; ld_codes is a multiple of 16
+#pragma unroll
+  for (int j = 0; j < kQuantHeld; ++j)
+    if (first + j * kStep < ld_codes) put(first + j * kStep, first + j * kStep < K ? held[j] : nullptr);
+  for (int64_t i = first + kQuantHeld * kStep; i < ld_codes; i += kStep) {
+    float v[8];
+    if (i < K) load_row8<T, VEC>(row, (int)i, K, v);
+    put((int)i, i < K ? v : nullptr);
+  }
 }
 
 struct Int8Args {
@@ -55,62 +111,490 @@ struct Int8Args {
   int N, K;
 };
 
-constexpr int BM = 64, BN = 64, BK = 16;  // BK: words of 4
+constexpr int kBlock = 128;  // bytes of K in a block: a row of a swizzled tile
+constexpr int kMmaK = 32;    // of one product
+constexpr int kEpiWarps = 4;
+
+// 8-bit signed operands, 32-bit integer accumulator, both K-major
+__host__ __device__ constexpr uint32_t int8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <int PAIR>
+__device__ __forceinline__ void mma_int8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  if (rd_umma::mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (rd_umma::mbar_try(bar, parity)) return true;
+    if (*stop || clock64() - t0 > (1ll << 31)) return false;
+  }
+}
+// by all lanes of a warp, the same answer for all
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, wait_or(bar, parity, stop));
+}
+__device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int* v) {
+  float f[32];
+  rd_umma::tmem_ld32(taddr, f);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
+}
+template <typename OutT>
+__device__ __forceinline__ float gated(float gate, float up) {
+  return (sizeof(OutT) == 2 ? rd::silu_f(gate) : rd::silu_exact(gate)) * up;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Few tokens (up to kFewTokens): bound by the weight's bytes.  A CTA owns `slab` rows of the weight, all of K and all tokens; the weight rows
+// ride the products' M, the tokens their N.  In a chain that begins with the row quantiser the first ring of weights is asked
+// for before the codes of the tokens are there (`early`: the quantiser starts its successors only when all before it is complete).
+constexpr int kFewTokens = 128;
+constexpr int kFewRing = 94 * 1024, kFewStagesMost = 16, kFewThreads = 192;
+constexpr int kFewSmem = 1024 + kFewRing + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512;
+struct FewShape {
+  int slab, tokens, blocks, stages, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
+};
 
 template <typename OutT, int EPI>
-__global__ void __launch_bounds__(256) gemm_int8_kernel(const Int8Args a) {
-  __shared__ int As[BK][BM + 4], Ws[BK][BN + 4];
+__global__ void __launch_bounds__(kFewThreads)
+    int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Int8Args a, const FewShape sh, int32_t* status) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFewRing + 16 * 1024);
+  uint64_t* empty = full + kFewStagesMost;
+  uint64_t* acc_full = empty + kFewStagesMost;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.x * sh.slab;
+  const int w_bytes = sh.slab * kBlock, a_bytes = sh.tokens * kBlock, stage_bytes = sh.blocks * (w_bytes + a_bytes);
+  const int k_blocks = (a.K + kBlock - 1) / kBlock, steps = (k_blocks + sh.blocks - 1) / sh.blocks;
   rd::pdl_launch_dependents();
+  if (warp == 0 && rd::elect_one()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    for (int s = 0; s < kFewStagesMost; ++s) {
+      rd_umma::mbar_init(&full[s], 2);
+      rd_umma::mbar_init(&empty[s], 1);
+    }
+    rd_umma::mbar_init(acc_full, 1);
+    *stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) rd_umma::tmem_alloc(tmem_slot, sh.tmem_cols);
+  rd_umma::fence_before();
+  __syncthreads();
+  rd_umma::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+  int site = 0;
+  if (warp == 0) {
+    if (rd::elect_one()) {
+      // blocks of a step: weights, then tokens; blocks past K are not loaded and not multiplied
+      auto load = [&](int step, bool weights) {
+        const int s = step % sh.stages, n = min(sh.blocks, k_blocks - step * sh.blocks);
+        uint8_t* to = smem + s * stage_bytes + (weights ? 0 : sh.blocks * w_bytes);
+        rd_umma::mbar_expect_tx(&full[s], n * (weights ? w_bytes : a_bytes));
+        for (int i = 0; i < n; ++i)
+          rd_umma::tma_load_2d(to + i * (weights ? w_bytes : a_bytes), weights ? &map_w : &map_a, &full[s], (step * sh.blocks + i) * kBlock, weights ? row0 : 0);
+      };
+      const int ahead = min(steps, sh.stages);
+      if (!sh.early) rd::pdl_wait();
+      for (int i = 0; i < ahead; ++i) load(i, true);
+      if (sh.early) rd::pdl_wait();
+      for (int i = 0; i < ahead; ++i) load(i, false);
+      for (int i = ahead; i < steps; ++i) {
+        if (!wait_or(&empty[i % sh.stages], (i / sh.stages - 1) & 1, stop)) {
+          ok = false, site = 1;
+          break;
+        }
+        load(i, true);
+        load(i, false);
+      }
+    }
+  } else if (warp == 1) {
+    if (rd::elect_one()) {
+      rd::pdl_wait();
+      const int M = rd::live_rows(a.m_dev, a.m_max);
+      const uint32_t idesc = int8_idesc(128, max(16, (M + 15) / 16 * 16));
+      for (int i = 0; i < steps; ++i) {
+        const int s = i % sh.stages, n = min(sh.blocks, k_blocks - i * sh.blocks);
+        if (!wait_or(&full[s], (i / sh.stages) & 1, stop)) {
+          ok = false, site = 2;
+          break;
+        }
+        rd_umma::fence_after();
+        const uint32_t w = rd_umma::smem_u32(smem + s * stage_bytes), t = w + sh.blocks * w_bytes;
+        for (int b = 0; b < n; ++b) {
+          const uint64_t dw = rd_umma::desc_k_major(w + b * w_bytes), dt = rd_umma::desc_k_major(t + b * a_bytes);
+#pragma unroll
+          for (int k = 0; k < kBlock / kMmaK; ++k) mma_int8<0>(tmem, dw + 2 * k, dt + 2 * k, idesc, i | b | k);
+        }
+        rd_umma::commit(&empty[s]);
+      }
+      if (ok) rd_umma::commit(acc_full);
+    }
+  } else {
+    rd::pdl_wait();
+    const int M = rd::live_rows(a.m_dev, a.m_max), quarter = warp & 3;
+    const int f = row0 + quarter * 32 + lane;
+    // the lane's feature; rows of the product past the slab are the next slab's
+    const bool mine = quarter * 32 + lane < sh.slab && f < a.N;
+    const float sw = mine ? a.w_scales[f] : 0.f;
+    const int64_t col = EPI == RD_EPI_SWIGLU ? f >> 1 : f;
+    ok = warp_wait(acc_full, 0, stop);
+    if (!ok) site = 3;
+    rd_umma::fence_after();
+    for (int c = 0; ok && quarter * 32 < sh.slab && c < M; c += 32) {
+      int v[32];
+      tmem_ld32i(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+      const int n = min(32, M - c);
+      const OutT* res = (const OutT*)a.R + (int64_t)c * a.ldr + col;
+      OutT* out = (OutT*)a.C + (int64_t)c * a.ldc + col;
+      float r[32];
+      if (EPI == RD_EPI_RES) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = mine && i < n ? rd::Num<OutT>::to_f(res[i * a.ldr]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (i >= n) break;
+        float y = (float)v[i] * (a.a_scales[c + i] * sw);
+        if (EPI == RD_EPI_SWIGLU) {
+          const float up = __shfl_xor_sync(0xffffffffu, y, 1);
+          if (mine && !(lane & 1)) out[i * a.ldc] = rd::Num<OutT>::from_f(gated<OutT>(y, up));
+        } else {
+          if (EPI == RD_EPI_RES) y += r[i];
+          if (mine) out[i * a.ldc] = rd::Num<OutT>::from_f(y);
+        }
+      }
+    }
+  }
+  if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 510 + site);
+  __syncwarp();
+  rd_umma::fence_before();
+  __syncthreads();
+  if (*stop)
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land
+  if (warp == 1) {
+    rd_umma::fence_after();
+    rd_umma::tmem_dealloc(tmem, sh.tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Many tokens: bound by the tensor cores and by the operands' way from L2.  Persistent, CTAs in clusters of two that share products of 256
+// tokens (the products' M, 128 to a CTA) x `width` features (their N; each CTA stages half of them):
+//   warp 0     loads of both operands, six stages of a block of K each; both CTAs' loads complete on the leader's barrier;
+//   warp 1     of the leader: issues the products into one of two accumulators;
+//   warps 2-5  epilogue, a token to a lane: scales, gate; 32 output features at a time through shared memory, from where rows go out
+//              (and residual rows come in) in 16-byte pieces of consecutive addresses.
+constexpr int kManyStages = 6, kManyThreads = 192, kTileTokens = 256, kMostWidth = 256;
+struct ManySmem {
+  static constexpr int kTokens = 128 * kBlock, kFeatures = kMostWidth / 2 * kBlock;
+  static constexpr int kScratch = kEpiWarps * 32 * 32 * 4, kScales = 2 * kMostWidth * 4;
+  static constexpr int kBytes = 1024 + kManyStages * (kTokens + kFeatures) + kScratch + kScales + 256;
+};
+struct ManyMaps {
+  CUtensorMap a, w;
+};
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_leader(void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(rd_umma::smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(rd_umma::smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(rd_umma::smem_u32(bar)), "h"((uint16_t)3)
+               : "memory");
+}
+
+template <typename OutT, int EPI>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    int8_many_kernel(const __grid_constant__ ManyMaps maps, const Int8Args a, int width, int32_t* status) {
+  using L = ManySmem;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sW = sA + kManyStages * L::kTokens;
+  float* scratch = reinterpret_cast<float*>(sW + kManyStages * L::kFeatures);
+  float* s_scale = scratch + kEpiWarps * 32 * 32;  // [2][256]: the weight scales of a tile
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + 2 * kMostWidth);
+  uint64_t* empty = full + kManyStages;
+  uint64_t* acc_full = empty + kManyStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  rd::pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w) : "memory");
+    for (int s = 0; s < kManyStages; ++s) {
+      rd_umma::mbar_init(&full[s], 1);
+      rd_umma::mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      rd_umma::mbar_init(&acc_full[i], 1);
+      rd_umma::mbar_init(&acc_empty[i], 2 * kEpiWarps);
+    }
+    *stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(rd_umma::smem_u32(tmem_slot)), "r"(2 * kMostWidth) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  rd_umma::fence_before();
+  __syncthreads();
+  cluster_sync();
+  rd_umma::fence_after();
+  const uint32_t tmem = *tmem_slot;
   rd::pdl_wait();
   const int M = rd::live_rows(a.m_dev, a.m_max);
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
-  if (m0 >= M) return;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int lr = threadIdx.x >> 2, lk = (threadIdx.x & 3) * 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 4 * BK) {
-    const int k = k0 + 4 * lk;
-    int4 u = make_int4(0, 0, 0, 0), w = u;
-    if (k < a.K && m0 + lr < M) u = *reinterpret_cast<const int4*>(a.A + (int64_t)(m0 + lr) * a.lda + k);
-    if (k < a.K && n0 + lr < a.N) w = *reinterpret_cast<const int4*>(a.W + (int64_t)(n0 + lr) * a.ldw + k);
-    As[lk][lr] = u.x, As[lk + 1][lr] = u.y, As[lk + 2][lr] = u.z, As[lk + 3][lr] = u.w;
-    Ws[lk][lr] = w.x, Ws[lk + 1][lr] = w.y, Ws[lk + 2][lr] = w.z, Ws[lk + 3][lr] = w.w;
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < BK; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(As[kk][ty * 4 + i], Ws[kk][tx * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty * 4 + i;
-    if (m >= M) continue;
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      v[j] = n < a.N ? (float)acc[i][j] * (a.a_scales[m] * a.w_scales[n]) : 0.f;
-    }
-    OutT* C = (OutT*)a.C + (int64_t)m * a.ldc;
-    if (EPI == RD_EPI_SWIGLU) {
-#pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const int n = n0 + tx * 4 + j;
-        if (n + 1 < a.N) C[n / 2] = rd::Num<OutT>::from_f(rd::silu_exact(v[j]) * v[j + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + tx * 4 + j;
-        if (n >= a.N) continue;
-        if (EPI == RD_EPI_RES) v[j] += rd::Num<OutT>::to_f(((const OutT*)a.R)[(int64_t)m * a.ldr + n]);
-        C[n] = rd::Num<OutT>::from_f(v[j]);
+  const int t_tiles = (M + kTileTokens - 1) / kTileTokens, f_tiles = (a.N + width - 1) / width, tiles = t_tiles * f_tiles;
+  const int k_blocks = (a.K + kBlock - 1) / kBlock;
+  bool ok = true;
+  int site = 0;
+  // tiles that run at the same time share features: those are read from memory once, the tokens lie in L2
+  if (warp == 0) {
+    if (rd::elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int tile = pair; ok && tile < tiles; tile += n_pairs) {
+        const int t0 = tile % t_tiles * kTileTokens + (int)rank * 128, f0 = tile / t_tiles * width + (int)rank * (width / 2);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!wait_or(&empty[stage], phase ^ 1, stop)) {
+            ok = false, site = 1;
+            break;
+          }
+          const uint32_t bar = in_leader(&full[stage]);
+          if (rank == 0) rd_umma::mbar_expect_tx(&full[stage], 2 * (L::kTokens + width / 2 * kBlock));
+          load_pair(sA + stage * L::kTokens, &maps.a, bar, kb * kBlock, t0);
+          load_pair(sW + stage * L::kFeatures, &maps.w, bar, kb * kBlock, f0);
+          if (++stage == kManyStages) stage = 0, phase ^= 1;
+        }
       }
     }
+  } else if (warp == 1) {
+    if (rank == 0 && rd::elect_one()) {
+      const uint32_t idesc = int8_idesc(256, width);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      for (int tile = pair; ok && tile < tiles; tile += n_pairs, ++local) {
+        const int acc = local & 1;
+        if (!wait_or(&acc_empty[acc], ((local >> 1) & 1) ^ 1, stop)) {
+          ok = false, site = 2;
+          break;
+        }
+        rd_umma::fence_after();
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!wait_or(&full[stage], phase, stop)) {
+            ok = false, site = 3;
+            break;
+          }
+          rd_umma::fence_after();
+          const uint64_t da = rd_umma::desc_k_major(rd_umma::smem_u32(sA + stage * L::kTokens)), dw = rd_umma::desc_k_major(rd_umma::smem_u32(sW + stage * L::kFeatures));
+#pragma unroll
+          for (int k = 0; k < kBlock / kMmaK; ++k) mma_int8<1>(tmem + acc * kMostWidth, da + 2 * k, dw + 2 * k, idesc, kb | k);
+          commit_both(&empty[stage]);
+          if (++stage == kManyStages) stage = 0, phase ^= 1;
+        }
+        if (ok) commit_both(&acc_full[acc]);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    float* scr = scratch + (warp - 2) * 32 * 32;
+    constexpr bool kGated = EPI == RD_EPI_SWIGLU;
+    constexpr int kEach = 16 / (int)sizeof(OutT), kLanes = 32 / kEach, kRowsAtOnce = 32 / kLanes;  // values of a 16-byte piece; lanes of a row of 32 outputs
+    const bool vec = ((uintptr_t)a.C % 16 == 0) && (a.ldc * sizeof(OutT)) % 16 == 0 && (EPI != RD_EPI_RES || ((uintptr_t)a.R % 16 == 0 && (a.ldr * sizeof(OutT)) % 16 == 0));
+    const int wide = kGated ? a.N / 2 : a.N;
+    int local = 0;
+    for (int tile = pair; tile < tiles; tile += n_pairs, ++local) {
+      const int t0 = tile % t_tiles * kTileTokens + (int)rank * 128 + quarter * 32, f0 = tile / t_tiles * width;
+      float* sw = s_scale + (local & 1) * kMostWidth;
+      for (int i = threadIdx.x - 64; i < width; i += kEpiWarps * 32) sw[i] = f0 + i < a.N ? a.w_scales[f0 + i] : 0.f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const float sa = t0 + lane < M ? a.a_scales[t0 + lane] : 0.f;
+      const int acc = local & 1;
+      if (!warp_wait(&acc_full[acc], (local >> 1) & 1, stop)) {
+        ok = false, site = 4;
+        break;
+      }
+      rd_umma::fence_after();
+      const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + acc * kMostWidth;
+      for (int c = 0; c < width; c += kGated ? 64 : 32) {
+        const int o0 = kGated ? (f0 + c) >> 1 : f0 + c;  // first of 32 outputs
+        if (o0 >= wide) break;
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < (kGated ? 2 : 1); ++half) {
+          int v[32];
+          tmem_ld32i(taddr + c + 32 * half, v);
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sw + c + 32 * half + i);
+            y[i] = (float)v[i] * (sa * s.x), y[i + 1] = (float)v[i + 1] * (sa * s.y), y[i + 2] = (float)v[i + 2] * (sa * s.z), y[i + 3] = (float)v[i + 3] * (sa * s.w);
+          }
+          if (kGated) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = gated<OutT>(y[2 * i], y[2 * i + 1]);
+          }
+#pragma unroll
+          for (int i = 0; i < (kGated ? 4 : 8); ++i) {
+            const int piece = (half * 4 + i) ^ (lane & 7);
+            *reinterpret_cast<float4*>(scr + lane * 32 + piece * 4) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          }
+        }
+        __syncwarp();
+        if (vec && o0 + 32 <= wide) {
+          const int part = lane % kLanes * kEach;
+#pragma unroll
+          for (int i = 0; i < 32; i += kRowsAtOnce) {
+            const int row = i + lane / kLanes;
+            float x[kEach];
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4) *reinterpret_cast<float4*>(x + e) = *reinterpret_cast<const float4*>(scr + row * 32 + ((((part + e) >> 2) ^ (row & 7)) << 2));
+            if (t0 + row >= M) continue;
+            if (EPI == RD_EPI_RES) {
+              OutT r[kEach];
+              *reinterpret_cast<uint4*>(r) = *reinterpret_cast<const uint4*>((const OutT*)a.R + (int64_t)(t0 + row) * a.ldr + o0 + part);
+#pragma unroll
+              for (int e = 0; e < kEach; ++e) x[e] += rd::Num<OutT>::to_f(r[e]);
+            }
+            OutT out[kEach];
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) out[e] = rd::Num<OutT>::from_f(x[e]);
+            *reinterpret_cast<uint4*>((OutT*)a.C + (int64_t)(t0 + row) * a.ldc + o0 + part) = *reinterpret_cast<const uint4*>(out);
+          }
+        } else {
+          for (int row = 0; row < 32 && t0 + row < M; ++row) {
+            if (o0 + lane >= wide) continue;
+            float x = scr[row * 32 + (((lane >> 2) ^ (row & 7)) << 2) + (lane & 3)];
+            if (EPI == RD_EPI_RES) x += rd::Num<OutT>::to_f(((const OutT*)a.R)[(int64_t)(t0 + row) * a.ldr + o0 + lane]);
+            ((OutT*)a.C)[(int64_t)(t0 + row) * a.ldc + o0 + lane] = rd::Num<OutT>::from_f(x);
+          }
+        }
+      }
+      rd_umma::fence_before();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(&acc_empty[acc])) : "memory");
+    }
   }
+  if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 520 + site);
+  __syncwarp();
+  rd_umma::fence_before();
+  __syncthreads();
+  if (*stop)
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land
+  cluster_sync();  // the peer signals and reads no more
+  if (warp == 1) {
+    rd_umma::fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kMostWidth) : "memory");
+  }
+}
+
+// Lets a kernel have its dynamic shared memory on the current device; once for each.
+template <auto Kernel>
+bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) {
+    rd_set_last_cuda_error((int)err);
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+  }();
+  return n;
+}
+
+template <typename OutT, int EPI>
+int launch_few(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
+  constexpr auto kernel = int8_few_kernel<OutT, EPI>;
+  RD_REQUIRE(allow_smem<kernel>(kFewSmem), RD_ERR_LAUNCH);
+  FewShape sh;
+  sh.tokens = (a.m_max + 15) / 16 * 16;
+  // the fewest weight rows, a multiple of 16, with which all slabs run at the same time: one on each SM, or else two
+  const int sms = sm_count();
+  sh.slab = ((a.N + sms - 1) / sms + 15) / 16 * 16;
+  if (sh.slab > 128) sh.slab = ((a.N + 2 * sms - 1) / (2 * sms) + 15) / 16 * 16;
+  if (sh.slab > 128) sh.slab = 128;
+  // loads of 16 KB or so
+  const int block = (sh.slab + sh.tokens) * kBlock;
+  sh.blocks = block >= 12 * 1024 ? 1 : block >= 6 * 1024 ? 2 : 4;
+  sh.stages = kFewRing / (sh.blocks * block);
+  if (sh.stages > kFewStagesMost) sh.stages = kFewStagesMost;
+  sh.tmem_cols = 32;
+  while (sh.tmem_cols < sh.tokens) sh.tmem_cols *= 2;
+  sh.early = early;
+  CUtensorMap ma, mw;
+  RD_REQUIRE(rd_umma::make_byte_map(&ma, a.A, a.m_max, a.K, a.lda, sh.tokens) && rd_umma::make_byte_map(&mw, a.W, a.N, a.K, a.ldw, sh.slab), RD_ERR_ARG);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)((a.N + sh.slab - 1) / sh.slab)), dim3(kFewThreads), kFewSmem, s, 1, ma, mw, a, sh, status);
+  RD_CHECK_CHAINED(err);
+  return RD_OK;
+}
+
+template <typename OutT, int EPI>
+int launch_many(const Int8Args& a, int32_t* status, cudaStream_t s) {
+  constexpr auto kernel = int8_many_kernel<OutT, EPI>;
+  RD_REQUIRE(allow_smem<kernel>(ManySmem::kBytes), RD_ERR_LAUNCH);
+  // Features of a tile: the width with which the rounds of tiles take least, a tile of w features counting w + 64.
+  const int64_t pairs = sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
+  int width = kMostWidth;
+  int64_t best = INT64_MAX;
+  for (int w = kMostWidth; w >= 64; w /= 2) {
+    const int64_t tiles = t_tiles * ((a.N + w - 1) / w), cost = (tiles + pairs - 1) / pairs * (w + 64);
+    if (cost < best) best = cost, width = w;
+  }
+  ManyMaps maps;
+  RD_REQUIRE(rd_umma::make_byte_map(&maps.a, a.A, a.m_max, a.K, a.lda, 128) && rd_umma::make_byte_map(&maps.w, a.W, a.N, a.K, a.ldw, width / 2), RD_ERR_ARG);
+  const int64_t tiles = t_tiles * ((a.N + width - 1) / width);
+  RD_REQUIRE(tiles <= 0x7fffffff, RD_ERR_SIZE);
+  const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
+  cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kManyThreads), ManySmem::kBytes, s, 2, maps, a, width, status);
+  RD_CHECK_CHAINED(err);
+  return RD_OK;
 }
 
 int check_rows(int dtype, const void* x, int64_t ldx, const int8_t* codes, int64_t ld_codes, const float* scales, int m_max, int K) {
@@ -140,25 +624,29 @@ int check_product(int out_dtype, const Int8Args& a, int epilogue) {
 
 int quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max, const int32_t* m_dev, int K, cudaStream_t s) {
   cudaError_t err;
-  if (dtype == RD_BF16)
-    err = rd::launch_chained(quant_rows_kernel<__nv_bfloat16>, dim3(m_max), dim3(kQuantThreads), 0, s, 1, (const __nv_bfloat16*)x, ldx, codes, ld_codes, scales,
-                             m_max, m_dev, K);
-  else
-    err = rd::launch_chained(quant_rows_kernel<float>, dim3(m_max), dim3(kQuantThreads), 0, s, 1, (const float*)x, ldx, codes, ld_codes, scales, m_max, m_dev, K);
+  auto run = [&](auto kern, auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    err = rd::launch_chained(kern, dim3(m_max), dim3(kQuantThreads), 0, s, 1, (const T*)x, ldx, codes, ld_codes, scales, m_max, m_dev, K);
+  };
+  const bool vec = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (ldx * (dtype == RD_BF16 ? 2 : 4)) % 16 == 0;
+  if (dtype == RD_BF16) vec ? run(quant_rows_kernel<__nv_bfloat16, true>, (__nv_bfloat16*)nullptr) : run(quant_rows_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)nullptr);
+  else vec ? run(quant_rows_kernel<float, true>, (float*)nullptr) : run(quant_rows_kernel<float, false>, (float*)nullptr);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
 
-int product(int out_dtype, const Int8Args& a, int epilogue, cudaStream_t s) {
-  const dim3 grid((a.N + BN - 1) / BN, (a.m_max + BM - 1) / BM);
-  cudaError_t err;
-  auto run = [&](auto kern) { err = rd::launch_chained(kern, grid, dim3(256), 0, s, 1, a); };
-  const bool f32 = out_dtype == RD_F32;
-  if (epilogue == RD_EPI_NONE) f32 ? run(gemm_int8_kernel<float, RD_EPI_NONE>) : run(gemm_int8_kernel<__nv_bfloat16, RD_EPI_NONE>);
-  else if (epilogue == RD_EPI_RES) f32 ? run(gemm_int8_kernel<float, RD_EPI_RES>) : run(gemm_int8_kernel<__nv_bfloat16, RD_EPI_RES>);
-  else f32 ? run(gemm_int8_kernel<float, RD_EPI_SWIGLU>) : run(gemm_int8_kernel<__nv_bfloat16, RD_EPI_SWIGLU>);
-  RD_CHECK_CHAINED(err);
-  return RD_OK;
+template <typename OutT, int EPI>
+int product_of(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
+  return a.m_max <= kFewTokens ? launch_few<OutT, EPI>(a, early, status, s) : launch_many<OutT, EPI>(a, status, s);
+}
+template <typename OutT>
+int product_as(const Int8Args& a, int epilogue, bool early, int32_t* status, cudaStream_t s) {
+  if (epilogue == RD_EPI_NONE) return product_of<OutT, RD_EPI_NONE>(a, early, status, s);
+  if (epilogue == RD_EPI_RES) return product_of<OutT, RD_EPI_RES>(a, early, status, s);
+  return product_of<OutT, RD_EPI_SWIGLU>(a, early, status, s);
+}
+int product(int out_dtype, const Int8Args& a, int epilogue, bool early, int32_t* status, cudaStream_t s) {
+  return out_dtype == RD_F32 ? product_as<float>(a, epilogue, early, status, s) : product_as<__nv_bfloat16>(a, epilogue, early, status, s);
 }
 
 }  // namespace
@@ -173,22 +661,20 @@ extern "C" int rd_quant_rows(int dtype, const void* x, int64_t ldx, int8_t* code
 extern "C" int rd_gemm_int8(int out_dtype, const int8_t* A, int64_t lda, const float* a_scales, const int8_t* W, int64_t ldw, const float* w_scales,
                             void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev, int N, int K, int epilogue,
                             int32_t* status, void* stream) {
-  (void)status;
   const Int8Args a{A, lda, a_scales, W, ldw, w_scales, C, ldc, R, ldr, m_max, m_dev, N, K};
   const int rc = check_product(out_dtype, a, epilogue);
   if (rc != RD_OK || m_max == 0) return rc;
-  return product(out_dtype, a, epilogue, (cudaStream_t)stream);
+  return product(out_dtype, a, epilogue, false, status, (cudaStream_t)stream);
 }
 
 extern "C" int rd_linear_int8(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, const int8_t* W, int64_t ldw,
                               const float* w_scales, int out_dtype, void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev,
                               int N, int K, int epilogue, int32_t* status, void* stream) {
-  (void)status;
   int rc = check_rows(dtype, x, ldx, codes, ld_codes, scales, m_max, K);
   if (rc != RD_OK) return rc;
   const Int8Args a{codes, ld_codes, scales, W, ldw, w_scales, C, ldc, R, ldr, m_max, m_dev, N, (K + 15) / 16 * 16};
   rc = check_product(out_dtype, a, epilogue);
   if (rc != RD_OK || m_max == 0) return rc;
   rc = quant_rows(dtype, x, ldx, codes, ld_codes, scales, m_max, m_dev, K, (cudaStream_t)stream);
-  return rc != RD_OK ? rc : product(out_dtype, a, epilogue, (cudaStream_t)stream);
+  return rc != RD_OK ? rc : product(out_dtype, a, epilogue, true, status, (cudaStream_t)stream);
 }
