@@ -7,8 +7,11 @@
 // the operands in shared memory or TMEM: writing the unpacked codes there costs more than these products, 8 columns wide.)
 //   S^T = K Q^T   A: 16 keys x 16 features of codes, B: 8 query rows, scaled by a power of two to fp16 (bf16's 8 bits fit) and, where the codes
 //                 are 16 times too large, by 1/16.  score = scale_k (S - zero_k sum q).
-//   O^T += V^T W  A: 16 features x 16 keys of codes minus their zeros (exact in fp16), B: W = p scale_v / r 2^14 in fp16, where r is the
-//                 largest value scale so far: weights keep fp16's 11 bits down to 2^-28 of the largest.
+//   O^T += V^T W  A: 16 features x 16 keys of codes, B: W = p scale_v / r 2^14 in fp16, where r is the largest value scale so far: weights
+//                 keep fp16's 11 bits down to 2^-28 of the largest.  What the zeros come to, sum W zero, is one number for a row of
+//                 queries and is taken off its features every eight tiles: until then O's fp32 holds at most some 2000 codes too much.
+//                 Codes of 4 bits are all taken four bits up here: the tensor core cuts a sum some 24 bits below what its factors' exponents allow for,
+//                 and with factors of code * 2^-24 that was 2^-19 of the largest value, unmoved that is 2^-23.
 // The accumulators' layouts fit: a lane holds the same query columns in S^T and in O^T, so the running maximum and sum need no
 // exchange but the maximum's over the 8 lanes of a column, and only where some lane's exceeds it; the weights become a B operand by
 // movmatrix.
@@ -43,6 +46,11 @@ struct Shape {
     const uint32_t b = k * kRowBytes + at;
     return b ^ ((b >> 3) & 0x70);
   }
+  // the place of a byte of sub-tile u from its tile's first byte (a multiple of 1024) and its place in sub-tile 0
+  static __device__ __forceinline__ uint32_t in_sub(uint32_t tile, uint32_t at, int u) {
+    const uint32_t b = tile + at + u * 16 * kRowBytes;
+    return kRowBytes == 32 && (u & 1) ? b ^ 64 : b;  // 512 bytes on, the swizzle's third bit is another
+  }
   // first feature of word w of a lane with t = lane % 4
   static __device__ __forceinline__ int feature(int t, int w) {
     if constexpr (kWords == 8) return (w >> 2) * 64 + t * 16 + (w & 3) * 4;
@@ -64,6 +72,15 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t y;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
   return y;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t x;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ void lds64(uint32_t at, uint32_t* x) { asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at) : "memory"); }
+__device__ __forceinline__ void lds128(uint32_t at, uint32_t* x) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t y;
@@ -192,6 +209,13 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   if (blockIdx.x == 0 && threadIdx.x == 0 && header != nullptr) *header = chunk;
   const int group = a.nh / a.nkv;
   const int64_t plane_rows = (int64_t)a.B * a.nkv * a.max_len;
+  // where a lane reads: key codes of rows g and g + 8 of a product, value codes of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9, parameters of the former
+  const uint32_t codes_u32 = rd_umma::smem_u32(codes), params_u32 = rd_umma::smem_u32(params);
+  uint32_t k_at[2], v_at[4], p_at[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) k_at[x] = S::place(S::key(g + 8 * x), t * (S::kWords == 2 ? 8 : 16)), p_at[x] = 4 * S::key(g + 8 * x);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) v_at[x] = S::place(S::key(2 * t + (x & 1) + 8 * (x >> 1)), g * (S::kRowBytes / 8));
   uint32_t used = 0;  // tiles that this warp has waited for so far: stage and phase
   bool ok = true;
   for (int item = blockIdx.x; ok; item += gridDim.x) {
@@ -221,7 +245,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     // the queries: row n * 8 + g is head (row % group) of new token row / group; a lane holds its share of the features
     const int rows = r.n_new * group;
     uint32_t q[NT][S::kSteps][2];
-    float q_sum[NT][2], unit[NT][2];  // of the columns 2 t, 2 t + 1 of a block of rows: sum q, and what a score is to be multiplied with
+    float q_sum[NT][2], unit[NT][2];  // of the columns 2 t, 2 t + 1 of a block of rows: 2^-24 sum q, and what a score is to be multiplied with
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = n * 8 + g;
@@ -279,46 +303,53 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       const float back = a.scale * 1.44269504f * 16777216.f * i1 * i2;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        q_sum[n][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + c));
+        q_sum[n][c] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + c)) * 0x1p-24f;
         unit[n][c] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + c));
       }
     }
 
-    float o[NT][kMT][4], m[NT][2], l[NT][2], ref = 0.f, inv_ref = 0.f;
+    float o[NT][kMT][4], m[NT][2], l[NT][2], z[NT][2], ref = 0.f, inv_ref = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < kMT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+      l[n][0] = l[n][1] = z[n][0] = z[n][1] = 0.f;
     }
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
-      const uint32_t stage = (used + i) % kFewStages;
-      if (!__all_sync(0xffffffffu, rd_umma::mbar_wait(&full[stage], ((used + i) / kFewStages) & 1))) {
-        ok = false;
-        break;
+    // O holds sums of codes; their zeros' part, the same for all features of a row, is taken off here
+    auto centre = [&]() {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f[c] = z[n][c];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) f[c] += __shfl_xor_sync(0xffffffffu, f[c], x);
+          f[c] *= BITS == 4 ? 0x1p-20f : 0x1p-24f;
+          z[n][c] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kMT; ++k) {
+          o[n][k][0] -= f[0], o[n][k][1] -= f[1], o[n][k][2] -= f[0], o[n][k][3] -= f[1];
+        }
       }
-      const uint8_t* kt = codes + stage * 2 * kTileBytes;
-      const uint8_t* vt = kt + kTileBytes;
-      const uint32_t *kp = params + stage * 128, *vp = kp + 64;
-      const int j0 = (from + warp + i * kFewWarps) * kKeys - r.first;  // key of the tile's first slot
-      const bool whole = j0 >= 0 && j0 + kKeys <= r.base;              // every row sees every key
-      float s[NT][kSub][4], sv[kSub][2];
-      bool more = false;
+    };
+    // One tile; kt: its codes in shared memory, pt: its parameters.  WHOLE: every row sees every key.
+    auto tile = [&](auto whole, uint32_t kt, uint32_t pt, int j0) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      float s[NT][kSub][4], sv[kSub][2], zv[kSub][2], most = 0.f, mx[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
-        const int key[2] = {u * 16 + S::key(g), u * 16 + S::key(g + 8)};
         uint32_t w[2][S::kWords];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if constexpr (S::kWords == 2) {
-            *reinterpret_cast<uint2*>(w[x]) = *reinterpret_cast<const uint2*>(kt + S::place(key[x], t * 8));
-          } else {
-#pragma unroll
-            for (int y = 0; y < S::kWords / 4; ++y)
-              *reinterpret_cast<uint4*>(w[x] + 4 * y) = *reinterpret_cast<const uint4*>(kt + S::place(key[x], t * 16 + y * 64));
-          }
+          const uint32_t at = S::in_sub(kt, k_at[x], u);
+          if constexpr (S::kWords == 2) lds64(at, w[x]);
+          else lds128(at, w[x]);
+          if constexpr (S::kWords == 8) lds128(at ^ 64, w[x] + 4);
         }
         float acc[NT][4];
 #pragma unroll
@@ -335,25 +366,24 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
           } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-              mma_f16(acc[n], w[0][y] & 0x00ff00ffu, w[1][y] & 0x00ff00ffu, (w[0][y] >> 8) & 0x00ff00ffu, (w[1][y] >> 8) & 0x00ff00ffu, q[n][y][0], q[n][y][1]);
+              mma_f16(acc[n], w[0][y] & 0x00ff00ffu, w[1][y] & 0x00ff00ffu, __byte_perm(w[0][y], 0, 0x4341), __byte_perm(w[1][y], 0, 0x4341), q[n][y][0], q[n][y][1]);
           }
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t p = kp[key[x]];
-          const float sk = param_scale(p), zk = (float)param_zero(p) * 0x1p-24f;
-          sv[u][x] = param_scale(vp[key[x]]);
+          const uint32_t at = pt + p_at[x] + u * 64;
+          const uint32_t pk = lds32(at), pv = lds32(at + 256);
+          const float sk = param_scale(pk), zk = code_as_float(param_zero(pk));
+          sv[u][x] = param_scale(pv);
+          zv[u][x] = code_as_float(param_zero(pv));
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) s[n][u][2 * x + c] = fmaf(-zk, q_sum[n][c], acc[n][2 * x + c]) * sk;
-        }
-        if (!whole) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int j = j0 + key[x];
+          if constexpr (!WHOLE) {
+            const int j = j0 + u * 16 + S::key(g + 8 * x);
             const bool there = j >= 0 && j < r.end;
-            if (!there) sv[u][x] = 0.f;
+            if (!there) sv[u][x] = zv[u][x] = 0.f;  // whatever lies there
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -362,22 +392,20 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
                 if (!(there && row < rows && (j < r.base || sees(a, r, row / group, j)))) s[n][u][2 * x + c] = -INFINITY;
               }
           }
-        }
+          most = fmaxf(most, sv[u][x]);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          more |= sv[u][x] > ref;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) more |= s[n][u][2 * x] > m[n][0] || s[n][u][2 * x + 1] > m[n][1];
+          for (int n = 0; n < NT; ++n) mx[n][0] = fmaxf(mx[n][0], s[n][u][2 * x]), mx[n][1] = fmaxf(mx[n][1], s[n][u][2 * x + 1]);
         }
       }
+      bool more = most > ref;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) more |= mx[n][0] > m[n][0] || mx[n][1] > m[n][1];
       if (__any_sync(0xffffffffu, more)) {
         // a larger maximum or a larger value scale: what has been summed so far is brought to it
-        float top = ref, mx[NT][2];
+        float top = fmaxf(most, ref);
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) top = fmaxf(top, fmaxf(sv[u][0], sv[u][1]));
-#pragma unroll
-        for (int o2 = 4; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
-        const float back = ref * __frcp_rn(fmaxf(top, 0x1p-100f));
+        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float back = ref / fmaxf(top, 0x1p-100f);
         ref = top;
         inv_ref = 16384.f / fmaxf(ref, 0x1p-100f);
 #pragma unroll
@@ -385,15 +413,14 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
           float f[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            mx[n][c] = m[n][c];
+            float x = fmaxf(mx[n][c], m[n][c]);
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) mx[n][c] = fmaxf(mx[n][c], fmaxf(s[n][u][c], s[n][u][2 + c]));
-#pragma unroll
-            for (int o2 = 4; o2 < 32; o2 <<= 1) mx[n][c] = fmaxf(mx[n][c], __shfl_xor_sync(0xffffffffu, mx[n][c], o2));
-            f[c] = m[n][c] == -INFINITY ? 0.f : ex2((m[n][c] - mx[n][c]) * unit[n][c]);
-            m[n][c] = mx[n][c];
+            for (int y = 4; y < 32; y <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+            f[c] = m[n][c] == -INFINITY ? 0.f : ex2((m[n][c] - x) * unit[n][c]);
+            m[n][c] = x;
             l[n][c] *= f[c];
             f[c] *= back;
+            z[n][c] *= f[c];
           }
 #pragma unroll
           for (int k = 0; k < kMT; ++k) o[n][k][0] *= f[0], o[n][k][1] *= f[1], o[n][k][2] *= f[0], o[n][k][3] *= f[1];
@@ -406,7 +433,15 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
         for (int c = 0; c < 2; ++c) off[n][c] = m[n][c] == -INFINITY ? 0.f : -m[n][c] * unit[n][c];
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
-        uint32_t b[NT][2];
+        constexpr int kVWords = S::kRowBytes / 32;  // words of a key that a lane holds: features g * HD / 8 ..
+        uint32_t w[4][kVWords], b[NT][2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = S::in_sub(kt + kTileBytes, v_at[x], u);
+          if constexpr (kVWords == 1) w[x][0] = lds32(at);
+          else if constexpr (kVWords == 2) lds64(at, w[x]);
+          else lds128(at, w[x]);
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float f = sv[u][x] * inv_ref;
@@ -416,30 +451,14 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
             l[n][0] += p0;
             l[n][1] += p1;
             float w0 = p0 * f, w1 = p1 * f;
-            if (!whole) w0 = p0 == 0.f ? 0.f : w0, w1 = p1 == 0.f ? 0.f : w1;  // a hidden value counts for nothing, NaN or not
-            b[n][x] = transpose8x8(pack_f16(w0, w1));
+            if constexpr (!WHOLE) w0 = p0 == 0.f ? 0.f : w0, w1 = p1 == 0.f ? 0.f : w1;  // a hidden value counts for nothing, NaN or not
+            const uint32_t h = pack_f16(w0, w1);
+            z[n][0] = fmaf(__low2float(*reinterpret_cast<const __half2*>(&h)), zv[u][x], z[n][0]);  // the weights as the products have them
+            z[n][1] = fmaf(__high2float(*reinterpret_cast<const __half2*>(&h)), zv[u][x], z[n][1]);
+            b[n][x] = transpose8x8(h);
           }
         }
-        // values of the keys whose weights this lane's B registers hold: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        uint32_t z[2], z16[2];
-        constexpr int kVWords = S::kRowBytes / 32;  // words of a key that a lane holds: features g * HD / 8 ..
-        uint32_t w[4][kVWords];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = u * 16 + S::key(2 * t + (x & 1) + 8 * (x >> 1));
-          uint32_t zero = param_zero(vp[key]);
-          if (!whole) {
-            const int j = j0 + key;
-            if (j < 0 || j >= r.end) zero = 0;  // whatever lies there
-          }
-          if (x & 1) z[x >> 1] |= zero << 16;
-          else z[x >> 1] = zero;
-          const uint8_t* src = vt + S::place(key, g * (S::kRowBytes / 8));
-          if constexpr (kVWords == 1) w[x][0] = *reinterpret_cast<const uint32_t*>(src);
-          else if constexpr (kVWords == 2) *reinterpret_cast<uint2*>(w[x]) = *reinterpret_cast<const uint2*>(src);
-          else *reinterpret_cast<uint4*>(w[x]) = *reinterpret_cast<const uint4*>(src);
-        }
-        z16[0] = z[0] << 4, z16[1] = z[1] << 4;
+        // the values of the keys whose weights this lane's B registers hold: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
         for (int y = 0; y < kVWords; ++y) {
 #pragma unroll
@@ -447,29 +466,40 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
             // two bytes of each of two keys: four features of 4 bits, or two of 8
             const uint32_t c0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), c1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
             if constexpr (BITS == 4) {
-              const uint32_t d0 = c0 >> 8, d1 = c1 >> 8;
-              const uint32_t e0 = sub_f16x2(c0 & 0x000f000fu, z[0]), e1 = sub_f16x2(c0 & 0x00f000f0u, z16[0]);
-              const uint32_t e2 = sub_f16x2(c1 & 0x000f000fu, z[1]), e3 = sub_f16x2(c1 & 0x00f000f0u, z16[1]);
-              const uint32_t f0 = sub_f16x2(d0 & 0x000f000fu, z[0]), f1 = sub_f16x2(d0 & 0x00f000f0u, z16[0]);
-              const uint32_t f2 = sub_f16x2(d1 & 0x000f000fu, z[1]), f3 = sub_f16x2(d1 & 0x00f000f0u, z16[1]);
+              const uint32_t e0 = c0 << 4, e1 = c1 << 4, f0 = c0 >> 4, f1 = c1 >> 4, h0 = c0 >> 8, h1 = c1 >> 8;
+              constexpr uint32_t kMask = 0x00f000f0u;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma_f16(o[n][4 * y + 2 * half], e0, e1, e2, e3, b[n][0], b[n][1]);
-                mma_f16(o[n][4 * y + 2 * half + 1], f0, f1, f2, f3, b[n][0], b[n][1]);
+                mma_f16(o[n][4 * y + 2 * half], e0 & kMask, c0 & kMask, e1 & kMask, c1 & kMask, b[n][0], b[n][1]);
+                mma_f16(o[n][4 * y + 2 * half + 1], f0 & kMask, h0 & kMask, f1 & kMask, h1 & kMask, b[n][0], b[n][1]);
               }
             } else {
-              const uint32_t e0 = sub_f16x2(c0 & 0x00ff00ffu, z[0]), e1 = sub_f16x2((c0 >> 8) & 0x00ff00ffu, z[0]);
-              const uint32_t e2 = sub_f16x2(c1 & 0x00ff00ffu, z[1]), e3 = sub_f16x2((c1 >> 8) & 0x00ff00ffu, z[1]);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * y + half], e0, e1, e2, e3, b[n][0], b[n][1]);
+              for (int n = 0; n < NT; ++n)
+                mma_f16(o[n][2 * y + half], c0 & 0x00ff00ffu, __byte_perm(c0, 0, 0x4341), c1 & 0x00ff00ffu, __byte_perm(c1, 0, 0x4341), b[n][0], b[n][1]);
             }
           }
         }
       }
+    };
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const uint32_t stage = (used + i) % kFewStages;
+      if (!__all_sync(0xffffffffu, rd_umma::mbar_wait(&full[stage], ((used + i) / kFewStages) & 1))) {
+        ok = false;
+        break;
+      }
+      const int j0 = (from + warp + i * kFewWarps) * kKeys - r.first;  // key of the tile's first slot
+      const uint32_t kt = codes_u32 + stage * 2 * kTileBytes, pt = params_u32 + stage * 512;
+      if (j0 >= 0 && j0 + kKeys <= r.base) tile(std::true_type(), kt, pt, j0);
+      else tile(std::false_type(), kt, pt, j0);
       __syncwarp();  // every lane has read its part of the stage
       if (i + kFewStages < mine && rd::elect_one()) load(i + kFewStages);
       __syncwarp();
+      // often enough that the sums of codes stay near those of the values that they stand for
+      if ((i & 7) == 7) centre();
     }
+    centre();
     used += mine;
     if (!ok) *gave_up = 1;
 
@@ -489,12 +519,12 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 #pragma unroll
         for (int o2 = 4; o2 < 32; o2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
         const int row = n * 8 + 2 * t + c;
-        // 2^24 / 2^14: the codes' factor and the weights'
+        constexpr float kBack = BITS == 4 ? 64.f : 1024.f;  // the codes' 2^20 or 2^24 over the weights' 2^14
         float* dst = so + (warp * kRows + row) * (HD + 2);
 #pragma unroll
         for (int k = 0; k < kMT; ++k) {
-          dst[g * (HD / 8) + 2 * k] = o[n][k][c] * 1024.f * ref;
-          dst[g * (HD / 8) + 2 * k + 1] = o[n][k][2 + c] * (BITS == 4 ? 64.f : 1024.f) * ref;
+          dst[g * (HD / 8) + 2 * k] = o[n][k][c] * kBack * ref;
+          dst[g * (HD / 8) + 2 * k + 1] = o[n][k][2 + c] * kBack * ref;
         }
         if (g == 0) {
           ss[(warp * kRows + row) * 2] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * unit[n][c];
@@ -535,17 +565,18 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   }
 }
 
-// Sums the chunks of the chains that have several.  A warp for each query row of each chain.
+// Sums the chunks of the chains that have several.  A CTA for each query row of each chain, its warps a share of the chunks each: a trip to
+// memory for every eight chunks.
 template <int HD>
 __global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a, const float* partial, const int* header, int keys, int item_rows) {
+  __shared__ float vs[8][HD], sums[8][2];
   rd::pdl_launch_dependents();
   rd::pdl_wait();
-  const int b = blockIdx.y, lane = threadIdx.x & 31, group = a.nh / a.nkv;
-  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5);  // (key/value head, row)
-  const int head = unit / item_rows, row = unit - head * item_rows;
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.nh / a.nkv;
+  const int head = blockIdx.x / item_rows, row = blockIdx.x - head * item_rows;
   const int chunk = *reinterpret_cast<const volatile int*>(header);
   const Row r = row_of(a, b);
-  if (head >= a.nkv || row >= r.n_new * group) return;
+  if (row >= r.n_new * group) return;
   const int n = (rounds_of(a, b, keys) + chunk - 1) / chunk;
   if (n <= 1) return;
   int before = 0;
@@ -553,20 +584,34 @@ __global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a
   before = rd::warp_sum_i(before) * a.nkv;
   const int64_t step = few_item_floats(HD, item_rows) * a.nkv;
   const float* p = partial + (before + head) * few_item_floats(HD, item_rows) + row * (HD + 2);
-  float top = -INFINITY;
-  for (int c = lane; c < n; c += 32) top = fmaxf(top, p[c * step + HD]);
-  top = rd::warp_max(top);
-  float sum = 0.f, v[HD / 32] = {};
+  float top = -INFINITY, sum = 0.f, v[HD / 32] = {};
 #pragma unroll 4
-  for (int c = 0; c < n; ++c) {
+  for (int c = warp; c < n; c += 8) {
     const float* x = p + c * step;
-    const float mw = x[HD];
-    const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
-    sum += f * x[HD + 1];
+    const float mc = x[HD], lc = x[HD + 1];
+    float y[HD / 32];
 #pragma unroll
-    for (int k = 0; k < HD / 32; ++k) v[k] += mw == -INFINITY ? 0.f : f * x[k * 32 + lane];
+    for (int k = 0; k < HD / 32; ++k) y[k] = x[k * 32 + lane];
+    const float t = fmaxf(top, mc);
+    const float f = top == -INFINITY ? 0.f : ex2(top - t), fc = mc == -INFINITY ? 0.f : ex2(mc - t);
+    top = t;
+    sum = sum * f + lc * fc;
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) v[k] = v[k] * f + (mc == -INFINITY ? 0.f : y[k] * fc);
   }
-  __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((int64_t)(r.start + row / group) * a.nh + head * group + row % group) * HD;
 #pragma unroll
-  for (int k = 0; k < HD / 32; ++k) dst[k * 32 + lane] = __float2bfloat16_rn(sum == 0.f ? 0.f : v[k] / sum);
+  for (int k = 0; k < HD / 32; ++k) vs[warp][k * 32 + lane] = v[k];
+  if (lane == 0) sums[warp][0] = top, sums[warp][1] = sum;
+  __syncthreads();
+  if (threadIdx.x >= HD) return;
+  float all = -INFINITY, total = 0.f, out = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) all = fmaxf(all, sums[w][0]);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float f = sums[w][0] == -INFINITY ? 0.f : ex2(sums[w][0] - all);
+    total += sums[w][1] * f;
+    out += f == 0.f ? 0.f : vs[w][threadIdx.x] * f;
+  }
+  ((__nv_bfloat16*)a.out)[((int64_t)(r.start + row / group) * a.nh + head * group + row % group) * HD + threadIdx.x] = __float2bfloat16_rn(total == 0.f ? 0.f : out / total);
 }

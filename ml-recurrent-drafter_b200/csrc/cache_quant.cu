@@ -13,64 +13,61 @@ namespace {
 using namespace rd_quant;
 
 constexpr int kThreads = 256;
-constexpr int kVec = 8;  // features of a lane
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
+// VEC consecutive values from a 16-byte boundary
+template <int VEC, typename T>
+__device__ __forceinline__ void load_values(const T* p, float* x) {
   if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int v = 0; v < VEC; v += 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + v);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[v + 2 * i] = __uint_as_float(w[i] << 16);
+        x[v + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
   } else {
-    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+#pragma unroll
+    for (int v = 0; v < VEC; v += 4) *reinterpret_cast<float4*>(x + v) = *reinterpret_cast<const float4*>(p + v);
   }
 }
 
-// One row by `lanes` lanes (a power of two), 8 features each; lanes past hd hold zeros, which change no range.
-template <int BITS>
+// One row by `lanes` lanes (a power of two), VEC features each; lanes past hd hold zeros, which change no range.
+template <int BITS, int VEC>
 __device__ __forceinline__ void quantise_row(const float* x, int lanes, bool mine, bool first, uint8_t* codes, uint32_t* param) {
-  constexpr float kQ = (float)((1 << BITS) - 1);
+  constexpr int kQ = (1 << BITS) - 1;
   float low = 0.f, high = 0.f;
-  bool odd = false;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    low = fminf(low, x[i]);
-    high = fmaxf(high, x[i]);
-    odd |= !(fabsf(x[i]) <= 3.402823466e38f);
-  }
-  if (odd) high = INFINITY;
+  for (int i = 0; i < VEC; ++i) low = min_nan(low, x[i]), high = max_nan(high, x[i]);
   for (int o = lanes >> 1; o > 0; o >>= 1) {
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
   }
   const float range = high - low;
-  __nv_bfloat16 s = __float2bfloat16_rn(range / kQ);
-  const bool fine = range <= 3.402823466e38f;
+  const bool fine = range <= 3.402823466e38f;  // not so for NaN either
+  const __nv_bfloat16 s = __float2bfloat16_rn(range / (float)kQ);
   const float scale = __bfloat162float(s);
   const bool some = fine && scale > 0.f;
-  const float zero = some ? fminf(rintf(-low / scale), kQ) : 0.f;
-  uint32_t c[kVec];
+  const Divider by(some ? scale : 1.f);
+  const int zero = some ? min((int)(by.rint_bits(-low) - kRintBias), kQ) : 0;
+  uint32_t w[VEC * BITS / 32];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) c[i] = some ? (uint32_t)fminf(fmaxf(rintf(x[i] / scale) + zero, 0.f), kQ) : 0u;
-  if (mine) {
-    if constexpr (BITS == 4) {
-      uint32_t w = 0;
+  for (int i = 0; i < VEC * BITS / 32; ++i) w[i] = 0;
+  if (some) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) w |= c[i] << (4 * i);
-      *reinterpret_cast<uint32_t*>(codes) = w;
-    } else {
-      uint2 w = make_uint2(0u, 0u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w.x |= c[i] << (8 * i), w.y |= c[4 + i] << (8 * i);
-      *reinterpret_cast<uint2*>(codes) = w;
+    for (int i = 0; i < VEC; ++i) {
+      const uint32_t c = (uint32_t)__vimin_s32_relu((int)(by.rint_bits(x[i]) - kRintBias) + zero, kQ);
+      w[i * BITS / 32] |= c << (i * BITS % 32);
     }
   }
-  if (first) *param = (uint32_t)(fine ? __bfloat16_as_ushort(s) : (unsigned short)kNanScale) | ((uint32_t)zero << 16);
+  if (mine) {
+    if constexpr (VEC * BITS == 32) *reinterpret_cast<uint32_t*>(codes) = w[0];
+    else if constexpr (VEC * BITS == 64) *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (first) *param = (fine ? (uint32_t)__bfloat16_as_ushort(s) : kNanScale) | ((uint32_t)zero << 16);
 }
 
 struct Planes {
@@ -78,97 +75,93 @@ struct Planes {
   uint32_t *k_params, *v_params;
 };
 
-// A unit is one head of one token, its key and its value.  Bound by memory: hd values read and hd * BITS / 8 + 4 bytes written for
-// each of the two.
-template <typename T, int BITS>
+// A unit is one head of one token, its key and its value, by hd / VEC lanes (rounded up to a power of two).
+template <typename T, int BITS, int VEC>
 __global__ void __launch_bounds__(kThreads) cache_quant_append_kernel(const T* k, const T* v, int64_t tok_stride, int64_t head_stride, Planes to,
                                                                       const int32_t* tok_row, const int32_t* tok_slot, int m_max,
                                                                       const int32_t* m_dev, int B, int nkv, int hd, int max_len, int lanes) {
   rd::pdl_launch_dependents();
   rd::pdl_wait();
-  const int64_t units = (int64_t)rd::live_rows(m_dev, m_max) * nkv;
-  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
-  const int part = threadIdx.x & (lanes - 1), d = part * kVec;
+  const uint32_t units = (uint32_t)rd::live_rows(m_dev, m_max) * (uint32_t)nkv;
+  const uint32_t unit = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
+  const int part = threadIdx.x & (lanes - 1), d = part * VEC;
   bool live = unit < units;
-  const int64_t t = live ? unit / nkv : 0;
-  const int head = (int)(unit - t * nkv);
+  const uint32_t t = live ? unit / (uint32_t)nkv : 0;
+  const int head = live ? (int)(unit - t * nkv) : 0;
+  const bool mine = live && d < hd;
+  float xk[VEC], xv[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) xk[i] = xv[i] = 0.f;
+  if (mine) {
+    const int64_t from = (int64_t)t * tok_stride + head * head_stride + d;
+    load_values<VEC>(k + from, xk);
+    load_values<VEC>(v + from, xv);
+  }
   int row = 0, slot = 0;
   if (live) {
     row = tok_row[t];
     slot = tok_slot[t];
     live = row >= 0 && row < B && slot >= 0 && slot < max_len;
   }
-  const bool mine = live && d < hd;
-  float xk[kVec] = {}, xv[kVec] = {};
-  if (mine) {
-    const int64_t from = t * tok_stride + head * head_stride + d;
-    load8(k + from, xk);
-    load8(v + from, xv);
-  }
   const int64_t at = ((int64_t)row * nkv + head) * max_len + slot;  // row of the planes
   const int64_t byte = at * (hd * BITS / 8) + d * BITS / 8;
-  quantise_row<BITS>(xk, lanes, mine, live && part == 0, to.k_codes + byte, to.k_params + at);
-  quantise_row<BITS>(xv, lanes, mine, live && part == 0, to.v_codes + byte, to.v_params + at);
+  quantise_row<BITS, VEC>(xk, lanes, mine && live, live && part == 0, to.k_codes + byte, to.k_params + at);
+  quantise_row<BITS, VEC>(xv, lanes, mine && live, live && part == 0, to.v_codes + byte, to.v_params + at);
 }
 
-// Eight codes as the values that they stand for.
-template <int BITS>
-__device__ __forceinline__ void values8(const uint8_t* codes, uint32_t param, float* x) {
-  const float scale = param_scale(param), zero = (float)param_zero(param);
-  if constexpr (BITS == 4) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = scale * (code_as_float((w >> (4 * i)) & 15u) - zero);
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(codes);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = scale * (code_as_float((w.x >> (8 * i)) & 255u) - zero);
-      x[4 + i] = scale * (code_as_float((w.y >> (8 * i)) & 255u) - zero);
-    }
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x) {
-  if constexpr (sizeof(T) == 2) {
-    __nv_bfloat162 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-  } else {
-    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
-    *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
-  }
-}
+constexpr int kReadRows = 8;  // rows of a thread, all asked for before the first is written
 
-constexpr int kReadRows = 4;  // rows of a thread
-
-// grid: x = blocks of rows, y = heads of all batch rows, keys first, then values
+// grid: x = blocks of rows, y = heads of all batch rows, keys first, then values.  A lane has 16 bytes of the output.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads) cache_quant_read_kernel(Planes from, const int32_t* begin, const int32_t* length, int nkv, int hd,
-                                                                    int max_len, T* k_out, T* v_out, int out_len, int chains) {
+                                                                    int max_len, T* k_out, T* v_out, int out_len, int chains, int lanes) {
+  constexpr int VEC = 16 / (int)sizeof(T);
   rd::pdl_launch_dependents();
   rd::pdl_wait();
+  const int rows = kThreads / lanes, part = threadIdx.x & (lanes - 1), d = part * VEC;
+  const int row_bytes = hd * BITS / 8;
   for (int64_t y = blockIdx.y; y < 2 * (int64_t)chains; y += gridDim.y) {
     const bool value = y >= chains;
     const int64_t chain = value ? y - chains : y;
-    const int b = (int)(chain / nkv);
+    const int b = (int)((uint32_t)chain / (uint32_t)nkv);
     const int first = begin[b];
     // rows outside the cache or the output do not exist
-    const int n = min(min(length[b], out_len), max_len - max(first, 0));
-    const uint8_t* codes = value ? from.v_codes : from.k_codes;
-    const uint32_t* params = value ? from.v_params : from.k_params;
-    T* out = (value ? v_out : k_out) + chain * out_len * hd;
-    const int vecs = hd / kVec;
-    const int64_t work = (int64_t)n * vecs, step = (int64_t)gridDim.x * kThreads;
-    if (first < 0) continue;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < work; i += step) {
-      const int64_t j = i / vecs;
-      const int d = (int)(i - j * vecs) * kVec;
-      const int64_t at = chain * max_len + first + j;
-      float x[kVec];
-      values8<BITS>(codes + at * (hd * BITS / 8) + d * BITS / 8, params[at], x);
-      store8(out + j * hd + d, x);
+    const int n = first < 0 ? 0 : min(min(length[b], out_len), max_len - first);
+    const int j0 = blockIdx.x * rows * kReadRows + threadIdx.x / lanes;
+    if (d >= hd) continue;
+    const uint8_t* codes = (value ? from.v_codes : from.k_codes) + (chain * max_len + first) * row_bytes + d * BITS / 8;
+    const uint32_t* params = (value ? from.v_params : from.k_params) + chain * max_len + first;
+    T* out = (value ? v_out : k_out) + chain * out_len * hd + d;
+    uint32_t w[kReadRows][2], p[kReadRows];
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+      const int j = j0 + i * rows;
+      if (j >= n) continue;
+      const uint8_t* c = codes + (int64_t)j * row_bytes;
+      if constexpr (VEC * BITS == 16) w[i][0] = *reinterpret_cast<const uint16_t*>(c);
+      else w[i][0] = *reinterpret_cast<const uint32_t*>(c);
+      if constexpr (VEC * BITS == 64) w[i][1] = *reinterpret_cast<const uint32_t*>(c + 4);
+      p[i] = params[j];
+    }
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+      const int j = j0 + i * rows;
+      if (j >= n) continue;
+      const float scale = param_scale(p[i]), zero = 8388608.f + (float)param_zero(p[i]);
+      float x[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint32_t c = (w[i][e * BITS / 32] >> (e * BITS % 32)) & ((1u << BITS) - 1);
+        x[e] = scale * (__uint_as_float(0x4b000000u | c) - zero);  // both sums exact
+      }
+      if constexpr (sizeof(T) == 2) {
+        __nv_bfloat162 h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4*>(out + (int64_t)j * hd) = *reinterpret_cast<const uint4*>(h);
+      } else {
+        *reinterpret_cast<float4*>(out + (int64_t)j * hd) = *reinterpret_cast<const float4*>(x);
+      }
     }
   }
 }
@@ -213,10 +206,11 @@ extern "C" int rd_cache_quant_append(int dtype, int bits, const void* k, const v
   const int esz = dtype == RD_BF16 ? 2 : 4;
   RD_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (tok_stride * esz) % 16 == 0 && (head_stride * esz) % 16 == 0, RD_ERR_ALIGN);
   RD_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params) & 15) == 0, RD_ERR_ALIGN);
+  const int vec = hd % 16 == 0 ? 16 : 8;
   int lanes = 1;
-  while (lanes * kVec < hd) lanes *= 2;
-  const int64_t blocks = ((int64_t)m_max * nkv * lanes + kThreads - 1) / kThreads;
-  RD_REQUIRE(blocks <= 0x7fffffff, RD_ERR_SIZE);
+  while (lanes * vec < hd) lanes *= 2;
+  RD_REQUIRE((int64_t)m_max * nkv <= 0x7fffffff - kThreads, RD_ERR_SIZE);
+  const int64_t blocks = ((int64_t)m_max * nkv + kThreads / lanes - 1) / (kThreads / lanes);
   const Planes to{k_codes, v_codes, (uint32_t*)k_params, (uint32_t*)v_params};
   cudaError_t err;
   auto run = [&](auto kern, auto* zero) {
@@ -224,8 +218,13 @@ extern "C" int rd_cache_quant_append(int dtype, int bits, const void* k, const v
     err = rd::launch_chained(kern, dim3((unsigned)blocks), dim3(kThreads), 0, (cudaStream_t)stream, 1, (const T*)k, (const T*)v, tok_stride, head_stride, to,
                              tok_row, tok_slot, m_max, m_dev, B, nkv, hd, max_len, lanes);
   };
-  if (dtype == RD_BF16) bits == 4 ? run(cache_quant_append_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr) : run(cache_quant_append_kernel<__nv_bfloat16, 8>, (__nv_bfloat16*)nullptr);
-  else bits == 4 ? run(cache_quant_append_kernel<float, 4>, (float*)nullptr) : run(cache_quant_append_kernel<float, 8>, (float*)nullptr);
+  auto pick = [&](auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    if (vec == 16) bits == 4 ? run(cache_quant_append_kernel<T, 4, 16>, zero) : run(cache_quant_append_kernel<T, 8, 16>, zero);
+    else bits == 4 ? run(cache_quant_append_kernel<T, 4, 8>, zero) : run(cache_quant_append_kernel<T, 8, 8>, zero);
+  };
+  if (dtype == RD_BF16) pick((__nv_bfloat16*)nullptr);
+  else pick((float*)nullptr);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
@@ -243,15 +242,17 @@ extern "C" int rd_cache_quant_read(int dtype, int bits, const uint8_t* k_codes, 
              RD_ERR_ALIGN);
   const int64_t chains = (int64_t)B * nkv;
   RD_REQUIRE(chains <= 0x3fffffff, RD_ERR_SIZE);
-  const int64_t vecs = (int64_t)out_len * (hd / kVec);
-  const unsigned gx = (unsigned)((vecs + kThreads * kReadRows - 1) / (kThreads * kReadRows));
+  int lanes = 1;
+  while (lanes * (dtype == RD_BF16 ? 8 : 4) < hd) lanes *= 2;
+  const int rows = kThreads / lanes * kReadRows;
+  const unsigned gx = (unsigned)(((int64_t)out_len + rows - 1) / rows);
   const unsigned gy = (unsigned)(2 * chains < 65535 ? 2 * chains : 65535);
   const Planes from{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params};
   cudaError_t err;
   auto run = [&](auto kern, auto* zero) {
     using T = std::remove_pointer_t<decltype(zero)>;
     err = rd::launch_chained(kern, dim3(gx, gy), dim3(kThreads), 0, (cudaStream_t)stream, 1, from, begin, length, nkv, hd, max_len, (T*)k_out, (T*)v_out, out_len,
-                             (int)chains);
+                             (int)chains, lanes);
   };
   if (dtype == RD_BF16) bits == 4 ? run(cache_quant_read_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr) : run(cache_quant_read_kernel<__nv_bfloat16, 8>, (__nv_bfloat16*)nullptr);
   else bits == 4 ? run(cache_quant_read_kernel<float, 4>, (float*)nullptr) : run(cache_quant_read_kernel<float, 8>, (float*)nullptr);

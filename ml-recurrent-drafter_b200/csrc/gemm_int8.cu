@@ -4,18 +4,18 @@
 #include <atomic>
 #include <type_traits>
 
+#include "quant.cuh"
 #include "umma.cuh"
 
 namespace {
 
-constexpr int kQuantThreads = 256;
 
-// One block a row, 8 values of a thread at a time; rows of up to kQuantHeld * 2048 values stay in registers between the maximum and the
-// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows.  VEC: rows on 16-byte boundaries, K a multiple of 8.
-constexpr int kQuantHeld = 6;
+// One block a row, 8 values of a thread at a time; rows of up to kQuantHeld * 8 * THREADS values stay in registers between the maximum and the
+// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows: these have blocks of 1024 threads.  VEC: rows on
+// 16-byte boundaries, K a multiple of 8.
 
-__device__ __forceinline__ uint32_t int8_code(float x, float scale) {
-  return (uint32_t)(int)fminf(fmaxf(rintf(x / scale), -127.f), 127.f) & 0xffu;
+__device__ __forceinline__ uint32_t int8_code(float x, const rd_quant::Divider& by) {
+  return (uint32_t)min(max((int)(by.rint_bits(x) - rd_quant::kRintBias), -127), 127) & 0xffu;
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_row8(const T* row, int i, int K, float* x) {
@@ -33,26 +33,23 @@ __device__ __forceinline__ void load_row8(const T* row, int i, int K, float* x) 
   }
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max,
+template <typename T, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max,
                                                                    const int32_t* m_dev, int K) {
-  __shared__ float red[kQuantThreads / 32];
+  constexpr int kQuantHeld = THREADS == 1024 ? 2 : 6;
+  __shared__ float red[THREADS / 32];
   rd::pdl_wait();
   rd::pdl_launch_dependents();  // after the wait: a product that follows may read what was complete before this kernel began
   const int t = blockIdx.x;
   if (t >= rd::live_rows(m_dev, m_max)) return;
   const T* row = x + (int64_t)t * ldx;
   int8_t* to = codes + (int64_t)t * ld_codes;
-  constexpr int kStep = kQuantThreads * 8;
+  constexpr int kStep = THREADS * 8;
   const int first = threadIdx.x * 8;
   float held[kQuantHeld][8], top = 0.f;
-  bool odd = false;
   auto look = [&](const float* v) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      odd |= !(fabsf(v[e]) <= 3.402823466e38f);
-      top = fmaxf(top, fabsf(v[e]));
-    }
+    for (int e = 0; e < 8; ++e) top = rd_quant::max_nan(top, fabsf(v[e]));
   };
 #pragma unroll
   for (int j = 0; j < kQuantHeld; ++j)
@@ -65,22 +62,23 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, i
     load_row8<T, VEC>(row, i, K, v);
     look(v);
   }
-  if (odd) top = INFINITY;
-  top = rd::warp_max(top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = rd_quant::max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
   top = red[0];
 #pragma unroll
-  for (int i = 1; i < kQuantThreads / 32; ++i) top = fmaxf(top, red[i]);
-  const bool fine = top <= 3.402823466e38f;
+  for (int i = 1; i < THREADS / 32; ++i) top = rd_quant::max_nan(top, red[i]);
+  const bool fine = top <= 3.402823466e38f;  // not so for NaN either
   const float scale = __bfloat162float(__float2bfloat16_rn(top / 127.f));
   const bool some = fine && scale > 0.f;
+  const rd_quant::Divider by(some ? scale : 1.f);
   if (threadIdx.x == 0) scales[t] = fine ? scale : __int_as_float(0x7fffffff);
   auto put = [&](int i, const float* v) {
     uint2 w = make_uint2(0u, 0u);
     if (some && v != nullptr) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w.x |= int8_code(v[e], scale) << (8 * e), w.y |= int8_code(v[4 + e], scale) << (8 * e);
+      for (int e = 0; e < 4; ++e) w.x |= int8_code(v[e], by) << (8 * e), w.y |= int8_code(v[4 + e], by) << (8 * e);
     }
     *reinterpret_cast<uint2*>(to + i) = w;
   };
@@ -162,10 +160,10 @@ __device__ __forceinline__ float gated(float gate, float up) {
 // ride the products' M, the tokens their N.  In a chain that begins with the row quantiser the first ring of weights is asked
 // for before the codes of the tokens are there (`early`: the quantiser starts its successors only when all before it is complete).
 constexpr int kFewTokens = 128;
-constexpr int kFewRing = 94 * 1024, kFewStagesMost = 16, kFewThreads = 192;
-constexpr int kFewSmem = 1024 + kFewRing + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512;
+constexpr int kFewRing = 200 * 1024, kFewHalfRing = 94 * 1024, kFewStagesMost = 16, kFewThreads = 192;  // one CTA on an SM, two
+constexpr int few_smem(int ring) { return 1024 + ring + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512; }
 struct FewShape {
-  int slab, tokens, blocks, stages, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
+  int slab, tokens, blocks, stages, ring, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
 };
 
 template <typename OutT, int EPI>
@@ -173,7 +171,7 @@ __global__ void __launch_bounds__(kFewThreads)
     int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Int8Args a, const FewShape sh, int32_t* status) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFewRing + 16 * 1024);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + sh.ring + 16 * 1024);
   uint64_t* empty = full + kFewStagesMost;
   uint64_t* acc_full = empty + kFewStagesMost;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
@@ -262,6 +260,8 @@ __global__ void __launch_bounds__(kFewThreads)
       int v[32];
       tmem_ld32i(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
       const int n = min(32, M - c);
+      // a load inside the loop of stores would wait for each of them
+      const float sa = lane < n ? a.a_scales[c + lane] : 0.f;
       const OutT* res = (const OutT*)a.R + (int64_t)c * a.ldr + col;
       OutT* out = (OutT*)a.C + (int64_t)c * a.ldc + col;
       float r[32];
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kFewThreads)
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         if (i >= n) break;
-        float y = (float)v[i] * (a.a_scales[c + i] * sw);
+        float y = (float)v[i] * (__shfl_sync(0xffffffffu, sa, i) * sw);
         if (EPI == RD_EPI_SWIGLU) {
           const float up = __shfl_xor_sync(0xffffffffu, y, 1);
           if (mine && !(lane & 1)) out[i * a.ldc] = rd::Num<OutT>::from_f(gated<OutT>(y, up));
@@ -552,7 +552,7 @@ int sm_count() {
 template <typename OutT, int EPI>
 int launch_few(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
   constexpr auto kernel = int8_few_kernel<OutT, EPI>;
-  RD_REQUIRE(allow_smem<kernel>(kFewSmem), RD_ERR_LAUNCH);
+  RD_REQUIRE(allow_smem<kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
   FewShape sh;
   sh.tokens = (a.m_max + 15) / 16 * 16;
   // the fewest weight rows, a multiple of 16, with which all slabs run at the same time: one on each SM, or else two
@@ -560,17 +560,19 @@ int launch_few(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
   sh.slab = ((a.N + sms - 1) / sms + 15) / 16 * 16;
   if (sh.slab > 128) sh.slab = ((a.N + 2 * sms - 1) / (2 * sms) + 15) / 16 * 16;
   if (sh.slab > 128) sh.slab = 128;
-  // loads of 16 KB or so
+  const int slabs = (a.N + sh.slab - 1) / sh.slab;
+  sh.ring = slabs <= sms ? kFewRing : kFewHalfRing;
+  // four blocks of K a stage, 512 consecutive bytes of each row, where at least four such stages fit
   const int block = (sh.slab + sh.tokens) * kBlock;
-  sh.blocks = block >= 12 * 1024 ? 1 : block >= 6 * 1024 ? 2 : 4;
-  sh.stages = kFewRing / (sh.blocks * block);
+  sh.blocks = 16 * block <= sh.ring ? 4 : 8 * block <= sh.ring ? 2 : 1;
+  sh.stages = sh.ring / (sh.blocks * block);
   if (sh.stages > kFewStagesMost) sh.stages = kFewStagesMost;
   sh.tmem_cols = 32;
   while (sh.tmem_cols < sh.tokens) sh.tmem_cols *= 2;
   sh.early = early;
   CUtensorMap ma, mw;
   RD_REQUIRE(rd_umma::make_byte_map(&ma, a.A, a.m_max, a.K, a.lda, sh.tokens) && rd_umma::make_byte_map(&mw, a.W, a.N, a.K, a.ldw, sh.slab), RD_ERR_ARG);
-  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)((a.N + sh.slab - 1) / sh.slab)), dim3(kFewThreads), kFewSmem, s, 1, ma, mw, a, sh, status);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)slabs), dim3(kFewThreads), few_smem(sh.ring), s, 1, ma, mw, a, sh, status);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
@@ -624,13 +626,19 @@ int check_product(int out_dtype, const Int8Args& a, int epilogue) {
 
 int quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max, const int32_t* m_dev, int K, cudaStream_t s) {
   cudaError_t err;
-  auto run = [&](auto kern, auto* zero) {
-    using T = std::remove_pointer_t<decltype(zero)>;
-    err = rd::launch_chained(kern, dim3(m_max), dim3(kQuantThreads), 0, s, 1, (const T*)x, ldx, codes, ld_codes, scales, m_max, m_dev, K);
-  };
   const bool vec = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (ldx * (dtype == RD_BF16 ? 2 : 4)) % 16 == 0;
-  if (dtype == RD_BF16) vec ? run(quant_rows_kernel<__nv_bfloat16, true>, (__nv_bfloat16*)nullptr) : run(quant_rows_kernel<__nv_bfloat16, false>, (__nv_bfloat16*)nullptr);
-  else vec ? run(quant_rows_kernel<float, true>, (float*)nullptr) : run(quant_rows_kernel<float, false>, (float*)nullptr);
+  const bool wide = m_max <= sm_count() && K > 2048;  // a block an SM: the row's latency is the kernel's
+  auto run = [&](auto kern, int threads, auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    err = rd::launch_chained(kern, dim3(m_max), dim3(threads), 0, s, 1, (const T*)x, ldx, codes, ld_codes, scales, m_max, m_dev, K);
+  };
+  auto pick = [&](auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    if (wide) vec ? run(quant_rows_kernel<T, true, 1024>, 1024, zero) : run(quant_rows_kernel<T, false, 1024>, 1024, zero);
+    else vec ? run(quant_rows_kernel<T, true, 256>, 256, zero) : run(quant_rows_kernel<T, false, 256>, 256, zero);
+  };
+  if (dtype == RD_BF16) pick((__nv_bfloat16*)nullptr);
+  else pick((float*)nullptr);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }

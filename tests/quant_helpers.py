@@ -79,7 +79,12 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
     Weights in fp16 have a smallest step besides, which counts where a feature's large weights all meet values of 0.  A weight is p s / r
     2^8 (2^14 in the kernel for few rows), s the value's scale, r a power of two (the scale) that is no more than the largest scale R of the keys;
     the largest p is at least 1 and the sum l that the result is divided by too.  Half of fp16's smallest step is 2^-25, so a key adds at
-    most 2^-25 2^-8 r (code - zero) / l <= 2^-33 R (2^bits - 1)."""
+    most 2^-25 2^-8 r (code - zero) / l <= 2^-33 R (2^bits - 1).
+
+    The kernel for few rows sums W code and W zero apart, in fp32, and takes one from the other, which shows where values cancel or are 0.  A
+    product of 16 keys adds to a sum of at most (2^bits - 1) R times the weights' share; a tensor core's addition may cut 2^-23 of that, the sum
+    of W zero, an addition for each of a lane's keys, too, and so may the difference.  A warp, one of eight, has n / 128 such products, two
+    more at the ends: (n / 128 + 2) 2^-22 (2^bits - 1) R in all."""
     l = cache.layers[layer]
     B, heads, cap, _ = l.k_codes.shape
     hd = cache.head_dim
@@ -112,7 +117,7 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
                 weight = weight_step + exp_step + 2 * err + seen.size * 2.0 ** -23
                 bound[s + i, h] = weight * (p @ np.abs(v[b, g, seen])) + weight * np.abs(out[s + i, h])
                 if weight_step > 2.0 ** -12:
-                    bound[s + i, h] += seen.size * 2.0 ** -33 * vs[b, g, seen].max() * top
+                    bound[s + i, h] += (seen.size * 2.0 ** -33 + (seen.size / 128 + 2) * 2.0 ** -22) * vs[b, g, seen].max() * top
     return out.reshape(m, -1), bound.reshape(m, -1)
 
 
