@@ -635,21 +635,39 @@ RD_API int rd_decode_advance(const int64_t* next_tok, int64_t* token_buf, int64_
  * zero = rint(-low / scale), code = rint(x / scale) + zero, both cut to 0 .. Q; a code stands for scale * (code - zero).  A scale
  * of 0 (a row of zeros, or of values too small) makes all codes 0; NaN, infinities, or a difference past fp32's largest number make
  * the scale NaN, and with it all that the row stands for.  Divisions round correctly, ties go to even: the codes are those of exact arithmetic.
+ * Arguments come in host structs, read before the call returns; the sizes of these are rd_quant_desc_bytes(0 .. 3) for append, read,
+ * attention and linear, for bindings that restate them.
  * k_codes / v_codes [B, nkv, max_len, hd * bits / 8] bytes, one code each or two (feature 2 i in the low half); k_params / v_params
  * [B, nkv, max_len] 32-bit words, the scale's bf16 pattern in the lower half, zero in the upper.  All four 16-byte aligned. */
 
+RD_API int rd_quant_desc_bytes(int which);
 /* Quantises the keys and values of new tokens as they are written: head g of token t at k + t*tok_stride + g*head_stride (strides in
  * elements; k, v and strides 16-byte aligned), to slot tok_slot[t] of row tok_row[t].  Tokens whose row or slot lies outside the cache are
  * left out; two tokens of a call must not have the same place. */
-RD_API int rd_cache_quant_append(int dtype, int bits, const void* k, const void* v, int64_t tok_stride, int64_t head_stride, uint8_t* k_codes,
-                          void* k_params, uint8_t* v_codes, void* v_params, const int32_t* tok_row, const int32_t* tok_slot, int m_max,
-                          const int32_t* m_dev, int B, int nkv, int hd, int max_len, void* stream);
+typedef struct rd_cache_quant_append_desc {
+  const void *k, *v;
+  int64_t tok_stride, head_stride;
+  uint8_t* k_codes;
+  void* k_params;
+  uint8_t* v_codes;
+  void* v_params;
+  const int32_t *tok_row, *tok_slot, *m_dev;
+  int32_t dtype, bits, m_max, B, nkv, hd, max_len;
+} rd_cache_quant_append_desc;
+RD_API int rd_cache_quant_append(const rd_cache_quant_append_desc* desc, void* stream);
 
 /* Reads back: slots begin[b] .. begin[b] + length[b] - 1 of row b to rows 0 .. of k_out / v_out [B, nkv, out_len, hd] in `dtype`, rounded
  * once.  At most out_len rows, none past the cache; what lies behind a row's last is left as it was.  A row with begin < 0 is left out. */
-RD_API int rd_cache_quant_read(int dtype, int bits, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes, const void* v_params,
-                        const int32_t* begin, const int32_t* length, int B, int nkv, int hd, int max_len, void* k_out, void* v_out,
-                        int out_len, void* stream);
+typedef struct rd_cache_quant_read_desc {
+  const uint8_t* k_codes;
+  const void* k_params;
+  const uint8_t* v_codes;
+  const void* v_params;
+  const int32_t *begin, *length;
+  void *k_out, *v_out;
+  int32_t dtype, bits, B, nkv, hd, max_len, out_len;
+} rd_cache_quant_read_desc;
+RD_API int rd_cache_quant_read(const rd_cache_quant_read_desc* desc, void* stream);
 
 /* rd_cache_commit for `planes` consecutive planes of codes [planes, B, nkv, max_len, hd * bits / 8] and their parameters at once. */
 RD_API int rd_cache_quant_commit(int bits, uint8_t* codes, void* params, int planes, int B, int nkv, int max_len, int hd,
@@ -662,10 +680,23 @@ RD_API int rd_cache_quant_commit(int bits, uint8_t* codes, void* params, int pla
  * max_kv bound the new tokens of a row and its keys.  workspace: rd_attention_quant_workspace_bytes() of device memory, 16-byte aligned
  * (NULL if that is 0); calls that may run at the same time need one each. */
 RD_API int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m_max, int B, int nh, int nkv, int hd, int max_new, int max_kv);
-RD_API int rd_attention_quant(int dtype, int bits, const void* q, int64_t ldq, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,
-                       const void* v_params, void* out, const int32_t* row_start, const int32_t* kv_begin, const int32_t* base_len, int m_max,
-                       int B, int nh, int nkv, int hd, int max_len, int max_new, int max_kv, int mode, const uint32_t* tree_mask,
-                       int mask_words, float scale, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+typedef struct rd_attention_quant_desc {
+  const void* q;
+  int64_t ldq;
+  const uint8_t* k_codes;
+  const void* k_params;
+  const uint8_t* v_codes;
+  const void* v_params;
+  void* out;
+  const int32_t *row_start, *kv_begin, *base_len;
+  const uint32_t* tree_mask;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int32_t dtype, bits, m_max, B, nh, nkv, hd, max_len, max_new, max_kv, mode, mask_words;
+  float scale;
+} rd_attention_quant_desc;
+RD_API int rd_attention_quant(const rd_attention_quant_desc* desc, void* stream);
 
 /* Rows as 8-bit integers: scale = bf16(max |x| / 127) held in fp32, code = rint(x / scale) cut to -127 .. 127 (ties to even, exact as
  * above); a row of zeros has scale 0, one with NaN or infinities scale NaN and codes 0.  Columns K .. ld_codes - 1 are set to 0.
@@ -680,9 +711,24 @@ RD_API int rd_gemm_int8(int out_dtype, const int8_t* A, int64_t lda, const float
                  int32_t* status, void* stream);
 /* rd_quant_rows of x [m, K] into codes / scales (the caller's, kept until the product has run), then rd_gemm_int8 of these with K rounded up
  * to a multiple of 16 (columns of W past K are zeros). */
-RD_API int rd_linear_int8(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, const int8_t* W, int64_t ldw,
-                   const float* w_scales, int out_dtype, void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev,
-                   int N, int K, int epilogue, int32_t* status, void* stream);
+typedef struct rd_linear_int8_desc {
+  const void* x;
+  int64_t ldx;
+  int8_t* codes;
+  int64_t ld_codes;
+  float* scales;
+  const int8_t* W;
+  int64_t ldw;
+  const float* w_scales;
+  void* C;
+  int64_t ldc;
+  const void* R;
+  int64_t ldr;
+  const int32_t* m_dev;
+  int32_t* status;
+  int32_t dtype, out_dtype, m_max, N, K, epilogue;
+} rd_linear_int8_desc;
+RD_API int rd_linear_int8(const rd_linear_int8_desc* desc, void* stream);
 
 #ifdef __cplusplus
 }

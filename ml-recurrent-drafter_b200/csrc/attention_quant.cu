@@ -252,10 +252,10 @@ extern "C" int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m
   return 0;
 }
 
-extern "C" int rd_attention_quant(int dtype, int bits, const void* q, int64_t ldq, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes,
-                                  const void* v_params, void* out, const int32_t* row_start, const int32_t* kv_begin, const int32_t* base_len, int m_max,
-                                  int B, int nh, int nkv, int hd, int max_len, int max_new, int max_kv, int mode, const uint32_t* tree_mask,
-                                  int mask_words, float scale, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+extern "C" int rd_attention_quant(const rd_attention_quant_desc* desc, void* stream) {
+  RD_REQUIRE(desc, RD_ERR_ARG);
+  const auto [q, ldq, k_codes, k_params, v_codes, v_params, out, row_start, kv_begin, base_len, tree_mask, workspace, workspace_bytes, status, dtype, bits, m_max,
+              B, nh, nkv, hd, max_len, max_new, max_kv, mode, mask_words, scale] = *desc;
   RD_REQUIRE(dtype == RD_F32 || dtype == RD_BF16, RD_ERR_DTYPE);
   RD_REQUIRE(bits == 4 || bits == 8, RD_ERR_UNSUPPORTED);
   RD_REQUIRE(mode == RD_ATTN_CAUSAL || mode == RD_ATTN_TREE, RD_ERR_UNSUPPORTED);

@@ -193,10 +193,9 @@ int check_layout(int bits, int B, int nkv, int hd, int max_len) {
 
 }  // namespace
 
-extern "C" int rd_cache_quant_append(int dtype, int bits, const void* k, const void* v, int64_t tok_stride, int64_t head_stride,
-                                     uint8_t* k_codes, void* k_params, uint8_t* v_codes, void* v_params, const int32_t* tok_row,
-                                     const int32_t* tok_slot, int m_max, const int32_t* m_dev, int B, int nkv, int hd, int max_len,
-                                     void* stream) {
+extern "C" int rd_cache_quant_append(const rd_cache_quant_append_desc* desc, void* stream) {
+  RD_REQUIRE(desc, RD_ERR_ARG);
+  const auto [k, v, tok_stride, head_stride, k_codes, k_params, v_codes, v_params, tok_row, tok_slot, m_dev, dtype, bits, m_max, B, nkv, hd, max_len] = *desc;
   RD_REQUIRE(dtype == RD_F32 || dtype == RD_BF16, RD_ERR_DTYPE);
   int rc = check_layout(bits, B, nkv, hd, max_len);
   if (rc != RD_OK) return rc;
@@ -229,9 +228,9 @@ extern "C" int rd_cache_quant_append(int dtype, int bits, const void* k, const v
   return RD_OK;
 }
 
-extern "C" int rd_cache_quant_read(int dtype, int bits, const uint8_t* k_codes, const void* k_params, const uint8_t* v_codes, const void* v_params,
-                                   const int32_t* begin, const int32_t* length, int B, int nkv, int hd, int max_len, void* k_out, void* v_out,
-                                   int out_len, void* stream) {
+extern "C" int rd_cache_quant_read(const rd_cache_quant_read_desc* desc, void* stream) {
+  RD_REQUIRE(desc, RD_ERR_ARG);
+  const auto [k_codes, k_params, v_codes, v_params, begin, length, k_out, v_out, dtype, bits, B, nkv, hd, max_len, out_len] = *desc;
   RD_REQUIRE(dtype == RD_F32 || dtype == RD_BF16, RD_ERR_DTYPE);
   int rc = check_layout(bits, B, nkv, hd, max_len);
   if (rc != RD_OK) return rc;

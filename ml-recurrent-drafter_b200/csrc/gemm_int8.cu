@@ -150,20 +150,41 @@ __device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int* v) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
 }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// all threads of the cluster's CTAs, each warp where it stands
+__device__ __forceinline__ void cluster_sync_part() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the same place of shared memory in another CTA of the cluster
+__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(rd_umma::smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void ld_cluster(uint32_t at, int* x) {
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
 template <typename OutT>
 __device__ __forceinline__ float gated(float gate, float up) {
   return (sizeof(OutT) == 2 ? rd::silu_f(gate) : rd::silu_exact(gate)) * up;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Few tokens (up to kFewTokens): bound by the weight's bytes.  A CTA owns `slab` rows of the weight, all of K and all tokens; the weight rows
-// ride the products' M, the tokens their N.  In a chain that begins with the row quantiser the first ring of weights is asked
-// for before the codes of the tokens are there (`early`: the quantiser starts its successors only when all before it is complete).
-constexpr int kFewTokens = 128;
+// Few tokens (up to kFewTokens): bound by the weight's bytes, and with more tokens by theirs, which every CTA reads from L2.  A CTA owns `slab` rows
+// of the weight, a share of K and all tokens; the weight rows ride the products' M, the tokens their N.  The CTAs of a slab are a
+// cluster: their sums, integers, meet in shared memory, and each finishes a part of the tokens.  In a chain that begins with the
+// row quantiser the first ring of weights is asked for before the codes of the tokens are there (`early`: the quantiser starts its
+// successors only when all before it is complete).
+constexpr int kFewTokens = 256, kMostShares = 8;
 constexpr int kFewRing = 200 * 1024, kFewHalfRing = 94 * 1024, kFewStagesMost = 16, kFewThreads = 192;  // one CTA on an SM, two
 constexpr int few_smem(int ring) { return 1024 + ring + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512; }
 struct FewShape {
-  int slab, tokens, blocks, stages, ring, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
+  int slab, shares, tokens, blocks, stages, ring, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
 };
 
 template <typename OutT, int EPI>
@@ -177,9 +198,10 @@ __global__ void __launch_bounds__(kFewThreads)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.x * sh.slab;
+  const int share = blockIdx.x % sh.shares, row0 = blockIdx.x / sh.shares * sh.slab;
   const int w_bytes = sh.slab * kBlock, a_bytes = sh.tokens * kBlock, stage_bytes = sh.blocks * (w_bytes + a_bytes);
-  const int k_blocks = (a.K + kBlock - 1) / kBlock, steps = (k_blocks + sh.blocks - 1) / sh.blocks;
+  const int all_blocks = (a.K + kBlock - 1) / kBlock, block0 = share * all_blocks / sh.shares, k_blocks = (share + 1) * all_blocks / sh.shares - block0;
+  const int steps = (k_blocks + sh.blocks - 1) / sh.blocks;
   rd::pdl_launch_dependents();
   if (warp == 0 && rd::elect_one()) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -207,7 +229,7 @@ __global__ void __launch_bounds__(kFewThreads)
         uint8_t* to = smem + s * stage_bytes + (weights ? 0 : sh.blocks * w_bytes);
         rd_umma::mbar_expect_tx(&full[s], n * (weights ? w_bytes : a_bytes));
         for (int i = 0; i < n; ++i)
-          rd_umma::tma_load_2d(to + i * (weights ? w_bytes : a_bytes), weights ? &map_w : &map_a, &full[s], (step * sh.blocks + i) * kBlock, weights ? row0 : 0);
+          rd_umma::tma_load_2d(to + i * (weights ? w_bytes : a_bytes), weights ? &map_w : &map_a, &full[s], (block0 + step * sh.blocks + i) * kBlock, weights ? row0 : 0);
       };
       const int ahead = min(steps, sh.stages);
       if (!sh.early) rd::pdl_wait();
@@ -248,40 +270,80 @@ __global__ void __launch_bounds__(kFewThreads)
   } else {
     rd::pdl_wait();
     const int M = rd::live_rows(a.m_dev, a.m_max), quarter = warp & 3;
-    const int f = row0 + quarter * 32 + lane;
-    // the lane's feature; rows of the product past the slab are the next slab's
-    const bool mine = quarter * 32 + lane < sh.slab && f < a.N;
-    const float sw = mine ? a.w_scales[f] : 0.f;
-    const int64_t col = EPI == RD_EPI_SWIGLU ? f >> 1 : f;
+    const int row = quarter * 32 + lane;
     ok = warp_wait(acc_full, 0, stop);
     if (!ok) site = 3;
     rd_umma::fence_after();
-    for (int c = 0; ok && quarter * 32 < sh.slab && c < M; c += 32) {
+    // Sums go to shared memory, [token][128 features], where the ring was; then a warp takes a token at a time, a lane four features.  Short
+    // loops: code that an SM has not run since the last kernel costs a trip to L2 for every stretch of it (an epilogue unrolled over
+    // 32 tokens took 4 us for one).
+    int* sums = reinterpret_cast<int*>(smem);
+    for (int c = 0; ok && row - lane < sh.slab && c < M; c += 32) {
       int v[32];
       tmem_ld32i(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
-      const int n = min(32, M - c);
-      // a load inside the loop of stores would wait for each of them
-      const float sa = lane < n ? a.a_scales[c + lane] : 0.f;
-      const OutT* res = (const OutT*)a.R + (int64_t)c * a.ldr + col;
-      OutT* out = (OutT*)a.C + (int64_t)c * a.ldc + col;
-      float r[32];
-      if (EPI == RD_EPI_RES) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = mine && i < n ? rd::Num<OutT>::to_f(res[i * a.ldr]) : 0.f;
-      }
+      for (int i = 0; i < 32; ++i) sums[(c + i) * 128 + row] = v[i];
+    }
+    if (sh.shares > 1) cluster_sync_part();
+    else asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int each = (M + sh.shares - 1) / sh.shares, t1 = ok ? min(M, (share + 1) * each) : 0;
+    const int f = row0 + lane * 4;
+    const bool mine = lane * 4 < sh.slab && f < a.N;  // rows of the product past the slab are the next slab's
+    constexpr bool kGated = EPI == RD_EPI_SWIGLU;
+    constexpr int kOut = kGated ? 2 : 4;
+    const int col = kGated ? f / 2 : f, wide = kGated ? a.N / 2 : a.N;
+    const bool vec = col + kOut <= wide && ((uintptr_t)a.C % (kOut * sizeof(OutT))) == 0 && a.ldc % kOut == 0 &&
+                     (EPI != RD_EPI_RES || (((uintptr_t)a.R % (kOut * sizeof(OutT))) == 0 && a.ldr % kOut == 0));
+    float sw[4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i >= n) break;
-        float y = (float)v[i] * (__shfl_sync(0xffffffffu, sa, i) * sw);
-        if (EPI == RD_EPI_SWIGLU) {
-          const float up = __shfl_xor_sync(0xffffffffu, y, 1);
-          if (mine && !(lane & 1)) out[i * a.ldc] = rd::Num<OutT>::from_f(gated<OutT>(y, up));
+    for (int e = 0; e < 4; ++e) sw[e] = mine && f + e < a.N ? a.w_scales[f + e] : 0.f;
+    using Vec = std::conditional_t<kOut * sizeof(OutT) == 16, uint4, std::conditional_t<kOut * sizeof(OutT) == 8, uint2, uint32_t>>;
+#pragma unroll 2
+    for (int t = share * each + quarter; t < t1; t += 4) {
+      const float sa = a.a_scales[t];
+      OutT r[kOut];
+      if (EPI == RD_EPI_RES && mine) {
+        const OutT* from = (const OutT*)a.R + (int64_t)t * a.ldr + col;
+        if (vec) {
+          *reinterpret_cast<Vec*>(r) = *reinterpret_cast<const Vec*>(from);
         } else {
-          if (EPI == RD_EPI_RES) y += r[i];
-          if (mine) out[i * a.ldc] = rd::Num<OutT>::from_f(y);
+#pragma unroll
+          for (int e = 0; e < kOut; ++e) r[e] = col + e < wide ? from[e] : rd::Num<OutT>::from_f(0.f);
         }
       }
+      int v[4] = {};
+      for (int s = 0; s < sh.shares; ++s) {
+        int x[4];
+        ld_cluster(of_rank(sums + t * 128 + lane * 4, sh.shares > 1 ? s : (int)cluster_rank()), x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += x[e];
+      }
+      if (!mine) continue;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (float)v[e] * (sa * sw[e]);
+      OutT out[kOut];
+      if constexpr (kGated) {
+        out[0] = rd::Num<OutT>::from_f(gated<OutT>(y[0], y[1]));
+        out[1] = rd::Num<OutT>::from_f(gated<OutT>(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = rd::Num<OutT>::from_f(EPI == RD_EPI_RES ? y[e] + rd::Num<OutT>::to_f(r[e]) : y[e]);
+      }
+      OutT* to = (OutT*)a.C + (int64_t)t * a.ldc + col;
+      if (vec) {
+        *reinterpret_cast<Vec*>(to) = *reinterpret_cast<const Vec*>(out);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kOut; ++e)
+          if (col + e < wide) to[e] = out[e];
+      }
     }
+  }
+  __syncwarp();
+  if (sh.shares > 1) {
+    if (warp < 2) cluster_sync_part();  // the epilogue warps have met the others' above
+    cluster_sync_part();                // no CTA leaves while its sums are read
   }
   if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 510 + site);
   __syncwarp();
@@ -311,20 +373,6 @@ struct ManySmem {
 struct ManyMaps {
   CUtensorMap a, w;
 };
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_leader(void* p) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(rd_umma::smem_u32(p)));
-  return r;
-}
 __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(rd_umma::smem_u32(dst)),
@@ -376,7 +424,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   }
   rd_umma::fence_before();
   __syncthreads();
-  cluster_sync();
+  cluster_sync_part();
   rd_umma::fence_after();
   const uint32_t tmem = *tmem_slot;
   rd::pdl_wait();
@@ -397,7 +445,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             ok = false, site = 1;
             break;
           }
-          const uint32_t bar = in_leader(&full[stage]);
+          const uint32_t bar = of_rank(&full[stage], 0);
           if (rank == 0) rd_umma::mbar_expect_tx(&full[stage], 2 * (L::kTokens + width / 2 * kBlock));
           load_pair(sA + stage * L::kTokens, &maps.a, bar, kb * kBlock, t0);
           load_pair(sW + stage * L::kFeatures, &maps.w, bar, kb * kBlock, f0);
@@ -509,7 +557,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
       rd_umma::fence_before();
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(&acc_empty[acc])) : "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(of_rank(&acc_empty[acc], 0)) : "memory");
     }
   }
   if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 520 + site);
@@ -518,7 +566,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncthreads();
   if (*stop)
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land
-  cluster_sync();  // the peer signals and reads no more
+  cluster_sync_part();  // the peer signals and reads no more
   if (warp == 1) {
     rd_umma::fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kMostWidth) : "memory");
@@ -549,19 +597,80 @@ int sm_count() {
   return n;
 }
 
-template <typename OutT, int EPI>
-int launch_few(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
-  constexpr auto kernel = int8_few_kernel<OutT, EPI>;
-  RD_REQUIRE(allow_smem<kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
-  FewShape sh;
+// How many CTAs of a kernel run at the same time in clusters of `shares`; asked once for each size of cluster and of shared memory.
+template <auto Kernel>
+int64_t resident_ctas(int shares, int threads, int smem, bool half) {
+  static std::atomic<int> known[kMostShares + 1][2] = {};
+  std::atomic<int>& here = known[shares][half];
+  int n = here.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (shares == 1) {
+      n = sm_count() * (half ? 2 : 1);
+    } else {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(shares);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = shares;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, Kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        clusters = 0;
+      }
+      n = clusters > 0 ? clusters * shares : 1;
+    }
+    here.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// What a call costs with either kernel: rows of 128 bytes that an SM brings in, and for few tokens those that the sums come to in shared memory.
+struct ManyShape {
+  int width;
+  int64_t cost, tiles;
+};
+ManyShape many_shape(const Int8Args& a) {
+  // features of a tile: the width with which the rounds of tiles take least, a tile of w features counting w + 64
+  const int64_t pairs = sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
+  ManyShape sh{kMostWidth, 0, 0};
+  int64_t best = INT64_MAX;
+  for (int w = kMostWidth; w >= 64; w /= 2) {
+    const int64_t tiles = t_tiles * ((a.N + w - 1) / w), rounds = (tiles + pairs - 1) / pairs;
+    if (rounds * (w + 64) < best) best = rounds * (w + 64), sh = ManyShape{w, rounds * (128 + w / 2) * ((a.K + kBlock - 1) / kBlock), tiles};
+  }
+  return sh;
+}
+// cost INT64_MAX: not for this call
+template <auto kernel>
+int64_t few_shape(const Int8Args& a, FewShape& sh) {
   sh.tokens = (a.m_max + 15) / 16 * 16;
-  // the fewest weight rows, a multiple of 16, with which all slabs run at the same time: one on each SM, or else two
-  const int sms = sm_count();
-  sh.slab = ((a.N + sms - 1) / sms + 15) / 16 * 16;
-  if (sh.slab > 128) sh.slab = ((a.N + 2 * sms - 1) / (2 * sms) + 15) / 16 * 16;
-  if (sh.slab > 128) sh.slab = 128;
-  const int slabs = (a.N + sh.slab - 1) / sh.slab;
-  sh.ring = slabs <= sms ? kFewRing : kFewHalfRing;
+  if (sh.tokens > kFewTokens) return INT64_MAX;
+  // Weight rows of a CTA and shares of K: those with which an SM has the fewest bytes to bring in, all CTAs at the same time, one on an SM or two.
+  // Fewer shares where that is the same.
+  const int sms = sm_count(), k_blocks = (a.K + kBlock - 1) / kBlock;
+  int64_t best = INT64_MAX;
+  for (int shares = 1; shares <= kMostShares && shares <= k_blocks; ++shares)
+    for (int half = 0; half < 2; ++half) {
+      const int ring = half ? kFewHalfRing : kFewRing;
+      if (sh.tokens * 512 > ring) continue;  // the sums
+      const int64_t most = resident_ctas<kernel>(shares, kFewThreads, few_smem(ring), half);
+      for (int slab = 128; slab >= 16; slab -= 16) {
+        const int64_t ctas = (int64_t)((a.N + slab - 1) / slab) * shares;
+        if (ctas > most) break;
+        const int64_t cost = (ctas + sms - 1) / sms * ((slab + sh.tokens) * ((k_blocks + shares - 1) / shares) + 8 * sh.tokens);
+        if (cost < best) best = cost, sh.slab = slab, sh.shares = shares, sh.ring = ring;
+      }
+    }
+  if (best == INT64_MAX) {  // more slabs than run at the same time
+    if (sh.tokens > 128) return best;
+    sh.slab = 128, sh.shares = 1, sh.ring = kFewHalfRing;
+    best = ((a.N + 127) / 128 + sms - 1) / sms * ((128 + sh.tokens) * (int64_t)k_blocks + 8 * sh.tokens);
+  }
   // four blocks of K a stage, 512 consecutive bytes of each row, where at least four such stages fit
   const int block = (sh.slab + sh.tokens) * kBlock;
   sh.blocks = 16 * block <= sh.ring ? 4 : 8 * block <= sh.ring ? 2 : 1;
@@ -569,32 +678,31 @@ int launch_few(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
   if (sh.stages > kFewStagesMost) sh.stages = kFewStagesMost;
   sh.tmem_cols = 32;
   while (sh.tmem_cols < sh.tokens) sh.tmem_cols *= 2;
-  sh.early = early;
+  sh.early = 0;
+  return best;
+}
+
+template <typename OutT, int EPI>
+int launch_few(const Int8Args& a, const FewShape& sh, int32_t* status, cudaStream_t s) {
+  constexpr auto kernel = int8_few_kernel<OutT, EPI>;
+  const int slabs = (a.N + sh.slab - 1) / sh.slab;
   CUtensorMap ma, mw;
   RD_REQUIRE(rd_umma::make_byte_map(&ma, a.A, a.m_max, a.K, a.lda, sh.tokens) && rd_umma::make_byte_map(&mw, a.W, a.N, a.K, a.ldw, sh.slab), RD_ERR_ARG);
-  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)slabs), dim3(kFewThreads), few_smem(sh.ring), s, 1, ma, mw, a, sh, status);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)(slabs * sh.shares)), dim3(kFewThreads), few_smem(sh.ring), s, sh.shares, ma, mw, a, sh, status);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
 
 template <typename OutT, int EPI>
-int launch_many(const Int8Args& a, int32_t* status, cudaStream_t s) {
+int launch_many(const Int8Args& a, const ManyShape& sh, int32_t* status, cudaStream_t s) {
   constexpr auto kernel = int8_many_kernel<OutT, EPI>;
   RD_REQUIRE(allow_smem<kernel>(ManySmem::kBytes), RD_ERR_LAUNCH);
-  // Features of a tile: the width with which the rounds of tiles take least, a tile of w features counting w + 64.
-  const int64_t pairs = sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
-  int width = kMostWidth;
-  int64_t best = INT64_MAX;
-  for (int w = kMostWidth; w >= 64; w /= 2) {
-    const int64_t tiles = t_tiles * ((a.N + w - 1) / w), cost = (tiles + pairs - 1) / pairs * (w + 64);
-    if (cost < best) best = cost, width = w;
-  }
   ManyMaps maps;
-  RD_REQUIRE(rd_umma::make_byte_map(&maps.a, a.A, a.m_max, a.K, a.lda, 128) && rd_umma::make_byte_map(&maps.w, a.W, a.N, a.K, a.ldw, width / 2), RD_ERR_ARG);
-  const int64_t tiles = t_tiles * ((a.N + width - 1) / width);
-  RD_REQUIRE(tiles <= 0x7fffffff, RD_ERR_SIZE);
-  const unsigned grid = 2 * (unsigned)(tiles < pairs ? tiles : pairs);
-  cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kManyThreads), ManySmem::kBytes, s, 2, maps, a, width, status);
+  RD_REQUIRE(rd_umma::make_byte_map(&maps.a, a.A, a.m_max, a.K, a.lda, 128) && rd_umma::make_byte_map(&maps.w, a.W, a.N, a.K, a.ldw, sh.width / 2), RD_ERR_ARG);
+  RD_REQUIRE(sh.tiles <= 0x7fffffff, RD_ERR_SIZE);
+  const int64_t pairs = sm_count() / 2;
+  const unsigned grid = 2 * (unsigned)(sh.tiles < pairs ? sh.tiles : pairs);
+  cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kManyThreads), ManySmem::kBytes, s, 2, maps, a, sh.width, status);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
@@ -645,7 +753,15 @@ int quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_
 
 template <typename OutT, int EPI>
 int product_of(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
-  return a.m_max <= kFewTokens ? launch_few<OutT, EPI>(a, early, status, s) : launch_many<OutT, EPI>(a, status, s);
+  // The kernel for few tokens where its SMs bring in less (one B200, row quantiser included, us, few against many: 11008 x 4096, 256
+  // tokens 30 : 35; 4096 x 12288, 110 tokens 23 : 28, 256 tokens 33 : 28; 4096 x 22016, 200 tokens 55 : 36; 2048 x 4096, 200 tokens 12.6 : 9.2).
+  FewShape few;
+  const ManyShape many = many_shape(a);
+  constexpr auto few_kernel = int8_few_kernel<OutT, EPI>;
+  RD_REQUIRE(allow_smem<few_kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
+  if (few_shape<few_kernel>(a, few) > many.cost) return launch_many<OutT, EPI>(a, many, status, s);
+  few.early = early;
+  return launch_few<OutT, EPI>(a, few, status, s);
 }
 template <typename OutT>
 int product_as(const Int8Args& a, int epilogue, bool early, int32_t* status, cudaStream_t s) {
@@ -675,14 +791,13 @@ extern "C" int rd_gemm_int8(int out_dtype, const int8_t* A, int64_t lda, const f
   return product(out_dtype, a, epilogue, false, status, (cudaStream_t)stream);
 }
 
-extern "C" int rd_linear_int8(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, const int8_t* W, int64_t ldw,
-                              const float* w_scales, int out_dtype, void* C, int64_t ldc, const void* R, int64_t ldr, int m_max, const int32_t* m_dev,
-                              int N, int K, int epilogue, int32_t* status, void* stream) {
-  int rc = check_rows(dtype, x, ldx, codes, ld_codes, scales, m_max, K);
+extern "C" int rd_linear_int8(const rd_linear_int8_desc* d, void* stream) {
+  RD_REQUIRE(d, RD_ERR_ARG);
+  int rc = check_rows(d->dtype, d->x, d->ldx, d->codes, d->ld_codes, d->scales, d->m_max, d->K);
   if (rc != RD_OK) return rc;
-  const Int8Args a{codes, ld_codes, scales, W, ldw, w_scales, C, ldc, R, ldr, m_max, m_dev, N, (K + 15) / 16 * 16};
-  rc = check_product(out_dtype, a, epilogue);
-  if (rc != RD_OK || m_max == 0) return rc;
-  rc = quant_rows(dtype, x, ldx, codes, ld_codes, scales, m_max, m_dev, K, (cudaStream_t)stream);
-  return rc != RD_OK ? rc : product(out_dtype, a, epilogue, true, status, (cudaStream_t)stream);
+  const Int8Args a{d->codes, d->ld_codes, d->scales, d->W, d->ldw, d->w_scales, d->C, d->ldc, d->R, d->ldr, d->m_max, d->m_dev, d->N, (d->K + 15) / 16 * 16};
+  rc = check_product(d->out_dtype, a, d->epilogue);
+  if (rc != RD_OK || d->m_max == 0) return rc;
+  rc = quant_rows(d->dtype, d->x, d->ldx, d->codes, d->ld_codes, d->scales, d->m_max, d->m_dev, d->K, (cudaStream_t)stream);
+  return rc != RD_OK ? rc : product(d->out_dtype, a, d->epilogue, true, d->status, (cudaStream_t)stream);
 }

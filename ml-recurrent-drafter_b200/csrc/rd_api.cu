@@ -34,3 +34,8 @@ extern "C" const char* rd_strerror(int code) {
     default: return "unknown error code";
   }
 }
+
+extern "C" int rd_quant_desc_bytes(int which) {
+  const size_t sizes[4] = {sizeof(rd_cache_quant_append_desc), sizeof(rd_cache_quant_read_desc), sizeof(rd_attention_quant_desc), sizeof(rd_linear_int8_desc)};
+  return which >= 0 && which < 4 ? (int)sizes[which] : RD_ERR_ARG;
+}

@@ -6,6 +6,7 @@ operators raise.  Build it with `python ml-recurrent-drafter_b200/build.py`.
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -106,14 +107,15 @@ SIGNATURES = {
     "rd_mlstm_scan": (_I, [_I, _P, _L, _P, _L, _P, _P, _F, _P, _F, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P]),
     "rd_cache_commit": (_I, [_I, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P]),
     "rd_decode_advance": (_I, [_P, _P, _L, _P, _P, _P, _P, _P, _I, _I, _P]),
-    "rd_cache_quant_append": (_I, [_I, _I, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
-    "rd_cache_quant_read": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P]),
+    "rd_quant_desc_bytes": (_I, [_I]),
+    "rd_cache_quant_append": (_I, [_P, _P]),
+    "rd_cache_quant_read": (_I, [_P, _P]),
     "rd_cache_quant_commit": (_I, [_I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P]),
     "rd_attention_quant_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
-    "rd_attention_quant": (_I, [_I, _I, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _L, _P, _P]),
+    "rd_attention_quant": (_I, [_P, _P]),
     "rd_quant_rows": (_I, [_I, _P, _L, _P, _L, _P, _I, _P, _I, _P]),
     "rd_gemm_int8": (_I, [_I, _P, _L, _P, _P, _L, _P, _P, _L, _P, _L, _I, _P, _I, _I, _I, _P, _P]),
-    "rd_linear_int8": (_I, [_I, _P, _L, _P, _L, _P, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _I, _P, _P]),
+    "rd_linear_int8": (_I, [_P, _P]),
     "rd_cache_unpack_static": (_I, [_I, _P, _I, _I, _I, _I, _I, _I, _P, _I, _P]),
 }
 
@@ -131,6 +133,13 @@ class AttentionDesc(ctypes.Structure):
     ] + [(n, ctypes.c_int32) for n in ("mask_words", "dtype", "B", "nh", "nkv", "dim", "tail_dim", "vdim", "max_new", "max_kv", "mode",
                                        "mask_kind", "window", "keep_first")] + [("scale", _F)]
 
+
+# The structs of include/redrafter_b200.h that the calls of a cache in codes and of 8-bit linear layers take, packed field by field in their
+# order (pointers, 0 for none, and int64 first, then int32 and float): the conversion of 27 separate arguments costs 7 us, this one.
+CACHE_APPEND = struct.Struct("@11q7i4x")  # k, v, tok_stride, head_stride, k_codes, k_params, v_codes, v_params, tok_row, tok_slot, m_dev | dtype ..
+CACHE_READ = struct.Struct("@8q7i4x")  # k_codes, k_params, v_codes, v_params, begin, length, k_out, v_out | dtype ..
+ATTENTION_QUANT = struct.Struct("@14q12if4x")  # q, ldq, planes, out, row_start, kv_begin, base_len, tree_mask, workspace, its bytes, status | dtype ..
+LINEAR_INT8 = struct.Struct("@14q6i")  # x, ldx, codes, ld_codes, scales, W, ldw, w_scales, C, ldc, R, ldr, m_dev, status | dtype ..
 
 _lib = None
 

@@ -6,9 +6,8 @@ it and only grows: row b occupies slots [kv_begin[b], kv_begin[b] + kv_len[b]). 
 are device int32 vectors owned by the decode loop; the View/Cache surface below keeps the
 reference's scalar `length` semantics for callers that use the cache the reference's way.
 """
-import math
 from dataclasses import dataclass
-from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -136,6 +135,11 @@ class QuantizedCache:
         self._codes = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, head_dim * bits // 8, dtype=torch.uint8, device=device)
         self._params = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, 2, dtype=torch.int16, device=device)
         self.layers = [LayerCodes(c[0], p[0], c[1], p[1]) for c, p in zip(self._codes, self._params)]
+        # what every call needs of them
+        self._planes = [tuple(t.data_ptr() for t in l) for l in self.layers]
+        self._shape = (batch_size, n_heads, capacity, head_dim)
+        self._device: int = self._codes.get_device()
+        self._workspace_bytes: Dict[Tuple, int] = {}
 
     @property
     def storage(self) -> "QuantizedCache":
@@ -149,57 +153,64 @@ class QuantizedCache:
         n_layers, _, _, heads, _, row = self._codes.shape
         return 2 * n_layers * heads * (row + 4)
 
-    def _here(self, **tensors) -> None:
-        """The tensors lie on the cache's device, which is the current one: kernels are launched on its current stream."""
-        dev = self._codes.device
-        if not self._codes.is_cuda:
+    def _on_device(self) -> int:
+        """The cache's device, which has to be the current one: kernels are launched on its current stream."""
+        if self._device < 0:
             raise _lib.RedrafterError("operator called with a CPU tensor: this library has no CPU path")
-        if dev.index != torch._C._cuda_getDevice():
-            raise _lib.RedrafterError(f"the cache lies on {dev}, which is not the current device")
-        for name, t in tensors.items():
-            if t is not None and t.device != dev:
-                raise _lib.RedrafterError(f"{name} lies on {t.device}, the cache on {dev}")
+        if self._device != torch._C._cuda_getDevice():
+            raise _lib.RedrafterError(f"the cache lies on cuda:{self._device}, which is not the current device")
+        return self._device
 
-    @staticmethod
-    def _indices(**tensors) -> None:
-        for name, (t, n) in tensors.items():
-            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
-                raise _lib.RedrafterError(f"{name} is a contiguous int32 vector of {n} elements")
+    def _elsewhere(self, **tensors) -> None:
+        for name, t in tensors.items():
+            if t is not None and t.get_device() != self._device:
+                raise _lib.RedrafterError(f"{name} lies on {t.device}, the cache on cuda:{self._device}")
+
+    def _index(self, name: str, t: torch.Tensor, n: int) -> int:
+        """The address of a vector of indices."""
+        if t.dtype is not torch.int32 or t.numel() < n or t.dim() != 1 or not t.is_contiguous():
+            raise _lib.RedrafterError(f"{name} is a contiguous int32 vector of {n} elements")
+        if t.get_device() != self._device:
+            self._elsewhere(**{name: t})
+        return t.data_ptr()
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, tok_row: torch.Tensor, tok_slot: torch.Tensor,
                m_dev: Optional[torch.Tensor] = None) -> None:
         """Writes the keys and values [tokens, heads, head_dim] of new tokens (bf16 or fp32; any strides of tokens and heads, the same in
         both) to slots tok_slot of batch rows tok_row.  Two tokens must not have the same place."""
-        l = self.layers[layer]
-        B, heads, capacity, _ = l.k_codes.shape
-        m = k.shape[0]
-        if k.shape != (m, heads, self.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
-            raise _lib.RedrafterError(f"keys {tuple(k.shape)} and values {tuple(v.shape)}: [tokens, {heads}, {self.head_dim}] of one type is wanted")
+        B, heads, capacity, hd = self._shape
+        dims = k.shape
+        if len(dims) != 3 or dims[1] != heads or dims[2] != hd or v.shape != dims or k.dtype is not v.dtype:
+            raise _lib.RedrafterError(f"keys {tuple(k.shape)} and values {tuple(v.shape)}: [tokens, {heads}, {hd}] of one type is wanted")
+        m = dims[0]
         # the stride of a dimension of size 1 says nothing
-        strides = [tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)) for t in (k, v)]
-        if strides[0] != strides[1] or (self.head_dim > 1 and strides[0][2] != 1):
+        s, u = k.stride(), v.stride()
+        tok, head = (s[0] if m > 1 else 0), (s[1] if heads > 1 else 0)
+        if s[2] != 1 or u[2] != 1 or (m > 1 and u[0] != tok) or (heads > 1 and u[1] != head):
             raise _lib.RedrafterError("keys and values need the same strides, and their features one after another")
-        self._here(k=k, v=v, tok_row=tok_row, tok_slot=tok_slot, m_dev=m_dev)
-        self._indices(tok_row=(tok_row, m), tok_slot=(tok_slot, m))
-        _lib.call("rd_cache_quant_append", _lib.dtype_code(k.dtype), self.bits, _lib.ptr(k), _lib.ptr(v), strides[0][0], strides[0][1],
-                  _lib.ptr(l.k_codes), _lib.ptr(l.k_params), _lib.ptr(l.v_codes), _lib.ptr(l.v_params), _lib.ptr(tok_row), _lib.ptr(tok_slot), m,
-                  _lib.ptr(m_dev), B, heads, self.head_dim, capacity, _lib.stream())
+        dev = self._on_device()
+        if k.get_device() != dev or v.get_device() != dev or (m_dev is not None and m_dev.get_device() != dev):
+            self._elsewhere(k=k, v=v, m_dev=m_dev)
+        rows, slots = self._index("tok_row", tok_row, m), self._index("tok_slot", tok_slot, m)
+        _lib.call("rd_cache_quant_append", _lib.CACHE_APPEND.pack(
+            k.data_ptr(), v.data_ptr(), tok, head, *self._planes[layer], rows, slots, 0 if m_dev is None else m_dev.data_ptr(),
+            _lib.dtype_code(k.dtype), self.bits, m, B, heads, hd, capacity), _lib.stream())
 
     def read(self, layer: int, begin: torch.Tensor, length: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
         """Slots begin[b] .. begin[b] + length[b] - 1 of every row b as plain keys and values: rows 0 .. of k_out and v_out [batch, heads,
         rows, head_dim] (bf16 or fp32, contiguous).  What lies behind a row's last is left as it was."""
-        l = self.layers[layer]
-        B, heads, capacity, _ = l.k_codes.shape
-        rows = k_out.shape[2] if k_out.dim() == 4 else -1
-        if k_out.shape != (B, heads, rows, self.head_dim) or v_out.shape != k_out.shape or k_out.dtype != v_out.dtype:
-            raise _lib.RedrafterError(f"outputs {tuple(k_out.shape)} and {tuple(v_out.shape)}: [{B}, {heads}, rows, {self.head_dim}] of one type is wanted")
+        B, heads, capacity, hd = self._shape
+        dims = k_out.shape
+        if len(dims) != 4 or dims[0] != B or dims[1] != heads or dims[3] != hd or v_out.shape != dims or k_out.dtype is not v_out.dtype:
+            raise _lib.RedrafterError(f"outputs {tuple(k_out.shape)} and {tuple(v_out.shape)}: [{B}, {heads}, rows, {hd}] of one type is wanted")
         if not (k_out.is_contiguous() and v_out.is_contiguous()):
             raise _lib.RedrafterError("the outputs are contiguous")
-        self._here(begin=begin, length=length, k_out=k_out, v_out=v_out)
-        self._indices(begin=(begin, B), length=(length, B))
-        _lib.call("rd_cache_quant_read", _lib.dtype_code(k_out.dtype), self.bits, _lib.ptr(l.k_codes), _lib.ptr(l.k_params), _lib.ptr(l.v_codes),
-                  _lib.ptr(l.v_params), _lib.ptr(begin), _lib.ptr(length), B, heads, self.head_dim, capacity, _lib.ptr(k_out), _lib.ptr(v_out), rows,
-                  _lib.stream())
+        dev = self._on_device()
+        if k_out.get_device() != dev or v_out.get_device() != dev:
+            self._elsewhere(k_out=k_out, v_out=v_out)
+        first, count = self._index("begin", begin, B), self._index("length", length, B)
+        _lib.call("rd_cache_quant_read", _lib.CACHE_READ.pack(*self._planes[layer], first, count, k_out.data_ptr(), v_out.data_ptr(),
+                                                              _lib.dtype_code(k_out.dtype), self.bits, B, heads, hd, capacity, dims[2]), _lib.stream())
 
     def attend(self, layer: int, q: torch.Tensor, out: torch.Tensor, row_start: torch.Tensor, kv_begin: torch.Tensor, base_len: torch.Tensor,
                max_new: int, max_kv: int, mode: int = _lib.ATTN_CAUSAL, tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -207,34 +218,46 @@ class QuantizedCache:
         """Attention of new tokens, whose keys and values have been appended.  q [tokens, query heads * head_dim] (bf16 or fp32; rows any
         stride apart), out the same, contiguous; row b of the batch has tokens row_start[b] .. row_start[b + 1] - 1, its keys are slots
         kv_begin[b] .. + base_len[b] (all visible) and its new tokens' own, visible causally or through tree_mask [tokens, words] (ATTN_TREE).
-        max_new, max_kv: upper bounds of a row's new tokens and keys.  scale: of the scores, 1 / sqrt(head_dim) unless given."""
-        l = self.layers[layer]
-        B, heads, capacity, _ = l.k_codes.shape
-        m, width = q.shape
-        if width % (heads * self.head_dim) or out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-            raise _lib.RedrafterError(f"queries {tuple(q.shape)}, output {tuple(out.shape)}: [tokens, a multiple of {heads} heads * {self.head_dim}] of one type is wanted")
-        if width > 1 and q.stride(1) != 1:
+        max_new, max_kv: upper bounds of a row's new tokens and keys; what exceeds them is left out.  scale: of the scores, 1 / sqrt(head_dim) unless
+        given."""
+        B, heads, capacity, hd = self._shape
+        dims = q.shape
+        if len(dims) != 2 or dims[1] == 0 or dims[1] % (heads * hd) or out.shape != dims or out.dtype is not q.dtype or not out.is_contiguous():
+            raise _lib.RedrafterError(f"queries {tuple(q.shape)}, output {tuple(out.shape)}: [tokens, a multiple of {heads} heads * {hd}] of one type is wanted")
+        m, width = dims
+        ldq, step = q.stride()
+        if step != 1:
             raise _lib.RedrafterError("the features of a query lie one after another")
-        self._here(q=q, out=out, row_start=row_start, kv_begin=kv_begin, base_len=base_len, tree_mask=tree_mask, status=status)
-        self._indices(row_start=(row_start, B + 1), kv_begin=(kv_begin, B), base_len=(base_len, B))
-        words = 0
+        dev = self._on_device()
+        if q.get_device() != dev or out.get_device() != dev or (status is not None and status.get_device() != dev):
+            self._elsewhere(q=q, out=out, status=status)
+        starts, begins, bases = self._index("row_start", row_start, B + 1), self._index("kv_begin", kv_begin, B), self._index("base_len", base_len, B)
+        words = mask = 0
         if mode == _lib.ATTN_TREE:
-            if tree_mask is None or tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] < m or not tree_mask.is_contiguous():
+            if tree_mask is None or tree_mask.dtype is not torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] < m or not tree_mask.is_contiguous():
                 raise _lib.RedrafterError("tree_mask is a contiguous int32 matrix with a row for each token")
-            words = tree_mask.shape[1]
-        code = _lib.dtype_code(q.dtype)
-        nh = width // self.head_dim
-        need = _lib.load().rd_attention_quant_workspace_bytes(code, self.bits, m, B, nh, heads, self.head_dim, max_new, max_kv)
+            self._elsewhere(tree_mask=tree_mask)
+            words, mask = tree_mask.shape[1], tree_mask.data_ptr()
+        code, nh = _lib.dtype_code(q.dtype), width // hd
+        sizes = (code, m, nh, max_new, max_kv)
+        need = self._workspace_bytes.get(sizes)
+        if need is None:
+            need = _lib.load().rd_attention_quant_workspace_bytes(code, self.bits, m, B, nh, heads, hd, max_new, max_kv)
+            if len(self._workspace_bytes) >= 256:
+                self._workspace_bytes.clear()
+            self._workspace_bytes[sizes] = need
+        # a new one for each call: calls on other streams and captured graphs each have their own
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        _lib.call("rd_attention_quant", code, self.bits, _lib.ptr(q), q.stride(0) if m > 1 else width, _lib.ptr(l.k_codes), _lib.ptr(l.k_params),
-                  _lib.ptr(l.v_codes), _lib.ptr(l.v_params), _lib.ptr(out), _lib.ptr(row_start), _lib.ptr(kv_begin), _lib.ptr(base_len), m, B, nh, heads,
-                  self.head_dim, capacity, max_new, max_kv, mode, _lib.ptr(tree_mask) if words else None, words,
-                  1.0 / math.sqrt(self.head_dim) if scale is None else scale, _lib.ptr(workspace), max(need, 0), _lib.ptr(status), _lib.stream())
+        _lib.call("rd_attention_quant", _lib.ATTENTION_QUANT.pack(
+            q.data_ptr(), ldq if m > 1 else width, *self._planes[layer], out.data_ptr(), starts, begins, bases, mask,
+            0 if workspace is None else workspace.data_ptr(), max(need, 0), 0 if status is None else status.data_ptr(),
+            code, self.bits, m, B, nh, heads, hd, capacity, max_new, max_kv, mode, words, hd ** -0.5 if scale is None else scale), _lib.stream())
 
     def commit_draft(self, fp, n_accepted: torch.Tensor, seq_in_beam: torch.Tensor, beam_shape, kv_begin: torch.Tensor) -> None:
         """Moves the accepted tokens of a packed draft behind the rows' prefixes, in all layers."""
         n_layers, _, B, heads, capacity, _ = self._codes.shape
-        self._here()
+        self._on_device()
+        self._elsewhere(kv_begin=kv_begin, n_accepted=n_accepted, seq_in_beam=seq_in_beam)
         _lib.call("rd_cache_quant_commit", self.bits, _lib.ptr(self._codes), _lib.ptr(self._params), 2 * n_layers, B, heads, capacity, self.head_dim,
                   _lib.ptr(kv_begin), _lib.ptr(fp.base_len), _lib.ptr(fp.unpacker), beam_shape.width, beam_shape.length, _lib.ptr(n_accepted),
                   _lib.ptr(seq_in_beam), _lib.stream())

@@ -272,6 +272,8 @@ class Int8Linear:
 
     def _hold(self, codes: torch.Tensor, scales: torch.Tensor, k: int) -> None:
         self.codes, self.scales, self.in_features, self.out_features = codes, scales, k, codes.shape[0]
+        # what every call needs of them
+        self._k16, self._codes_ptr, self._scales_ptr, self._device = codes.shape[1], codes.data_ptr(), scales.data_ptr(), codes.get_device()
 
     def drop_plans(self) -> None:
         """Nothing is kept between calls."""
@@ -280,27 +282,36 @@ class Int8Linear:
                  m_dev: Optional[torch.Tensor] = None, m_max: Optional[int] = None, status: Optional[torch.Tensor] = None) -> None:
         """c = epilogue(a W^T); a [rows, in] bf16 or fp32, c [rows, out] (out / 2 with EPI_SWIGLU) bf16 or fp32, residual as c (EPI_RES; it
         may be c).  Rows may lie any stride apart."""
-        m = a.shape[0] if m_max is None else m_max
+        rows, width = a.shape
+        m = rows if m_max is None else m_max
         wide = self.out_features // 2 if epilogue == _lib.EPI_SWIGLU else self.out_features
-        if a.dim() != 2 or a.shape[0] < m or a.shape[1] != self.in_features or c.dim() != 2 or c.shape[0] < m or c.shape[1] != wide:
+        crows, cwidth = c.shape
+        if rows < m or width != self.in_features or crows < m or cwidth != wide:
             raise _lib.RedrafterError(f"input {tuple(a.shape)}, output {tuple(c.shape)}: [rows, {self.in_features}] and [rows, {wide}] are wanted")
-        for t in (a, c) + ((residual,) if residual is not None else ()):
-            if t.device != self.codes.device or (t.shape[1] > 1 and t.stride(1) != 1):
+        (lda, astep), (ldc, cstep) = a.stride(), c.stride()
+        dev = self._device
+        if (astep != 1 and width > 1) or (cstep != 1 and wide > 1) or a.get_device() != dev or c.get_device() != dev:
+            raise _lib.RedrafterError("rows of consecutive features on the weight's device are wanted")
+        res, ldr = 0, 0
+        if residual is not None:
+            if residual.dim() != 2 or residual.shape[0] < m or residual.shape[1] != wide or residual.dtype is not c.dtype:
+                raise _lib.RedrafterError("the residual has the output's shape and type")
+            ldr, step = residual.stride()
+            if (step != 1 and wide > 1) or residual.get_device() != dev:
                 raise _lib.RedrafterError("rows of consecutive features on the weight's device are wanted")
-        if residual is not None and (residual.dim() != 2 or residual.shape[0] < m or residual.shape[1] != wide or residual.dtype != c.dtype):
-            raise _lib.RedrafterError("the residual has the output's shape and type")
-        if self.codes.is_cuda and self.codes.device.index != torch._C._cuda_getDevice():
-            raise _lib.RedrafterError(f"the weight lies on {self.codes.device}, which is not the current device")
-        k16 = self.codes.shape[1]
-        codes = torch.empty(m, k16, dtype=torch.int8, device=a.device)
-        scales = torch.empty(m, dtype=torch.float32, device=a.device)
-
-        def ld(t: torch.Tensor) -> int:
-            return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-        _lib.call("rd_linear_int8", _lib.dtype_code(a.dtype), _lib.ptr(a), ld(a), _lib.ptr(codes), k16, _lib.ptr(scales), _lib.ptr(self.codes), k16,
-                  _lib.ptr(self.scales), _lib.dtype_code(c.dtype), _lib.ptr(c), ld(c), _lib.ptr(residual), 0 if residual is None else ld(residual), m,
-                  _lib.ptr(m_dev), self.out_features, self.in_features, epilogue, _lib.ptr(status), _lib.stream())
+            res, ldr = residual.data_ptr(), ldr if residual.shape[0] > 1 else wide
+        if dev < 0:
+            raise _lib.RedrafterError("operator called with a CPU tensor: this library has no CPU path")
+        if dev != torch._C._cuda_getDevice() or (m_dev is not None and m_dev.get_device() != dev) or (status is not None and status.get_device() != dev):
+            raise _lib.RedrafterError(f"the weight lies on cuda:{dev}, which is not the current device or not that of m_dev and status")
+        k16 = self._k16
+        # codes of the rows, then (on a 16-byte boundary) their scales; a new one for each call, as calls may run at the same time
+        scratch = torch.empty(m * (k16 + 4), dtype=torch.int8, device=a.device)
+        codes = scratch.data_ptr()
+        _lib.call("rd_linear_int8", _lib.LINEAR_INT8.pack(
+            a.data_ptr(), lda if rows > 1 else width, codes, k16, codes + m * k16, self._codes_ptr, k16, self._scales_ptr, c.data_ptr(),
+            ldc if crows > 1 else wide, res, ldr, 0 if m_dev is None else m_dev.data_ptr(), 0 if status is None else status.data_ptr(),
+            _lib.dtype_code(a.dtype), _lib.dtype_code(c.dtype), m, self.out_features, self.in_features, epilogue), _lib.stream())
 
 
 def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, m_dev: Optional[torch.Tensor] = None) -> None:

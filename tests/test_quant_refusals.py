@@ -10,16 +10,22 @@ from recurrent_drafting import _lib
 P = 1 << 20  # an aligned address; nothing reads it
 
 
+def order(a, names):
+    """The fields of a struct, None as the null pointer."""
+    assert sorted(names.split()) == sorted(a)
+    return [0 if a[n] is None else a[n] for n in names.split()]
+
+
 def append(**kw):
     a = dict(dtype=1, bits=4, k=P, v=P, ts=64, hs=64, kc=P, kp=P, vc=P, vp=P, row=P, slot=P, m=2, m_dev=None, B=1, nkv=2, hd=64, max_len=16)
     a.update(kw)
-    return _lib.load().rd_cache_quant_append(*a.values(), None)
+    return _lib.load().rd_cache_quant_append(_lib.CACHE_APPEND.pack(*order(a, "k v ts hs kc kp vc vp row slot m_dev dtype bits m B nkv hd max_len")), None)
 
 
 def read(**kw):
     a = dict(dtype=1, bits=4, kc=P, kp=P, vc=P, vp=P, begin=P, length=P, B=1, nkv=2, hd=64, max_len=16, ko=P, vo=P, out_len=4)
     a.update(kw)
-    return _lib.load().rd_cache_quant_read(*a.values(), None)
+    return _lib.load().rd_cache_quant_read(_lib.CACHE_READ.pack(*order(a, "kc kp vc vp begin length ko vo dtype bits B nkv hd max_len out_len")), None)
 
 
 def commit(**kw):
@@ -32,7 +38,8 @@ def attend(**kw):
     a = dict(dtype=1, bits=4, q=P, ldq=128, kc=P, kp=P, vc=P, vp=P, out=P, rs=P, kb=P, bl=P, m=2, B=1, nh=2, nkv=2, hd=64, max_len=16, max_new=1, max_kv=16,
              mode=0, mask=None, words=0, scale=0.125, ws=None, ws_bytes=0, status=None)
     a.update(kw)
-    return _lib.load().rd_attention_quant(*a.values(), None)
+    return _lib.load().rd_attention_quant(_lib.ATTENTION_QUANT.pack(*order(
+        a, "q ldq kc kp vc vp out rs kb bl mask ws ws_bytes status dtype bits m B nh nkv hd max_len max_new max_kv mode words scale")), None)
 
 
 def rows(**kw):
@@ -45,6 +52,12 @@ def product(**kw):
     a = dict(out=1, A=P, lda=64, sa=P, W=P, ldw=64, sw=P, C=P, ldc=8, R=None, ldr=0, m=2, m_dev=None, N=8, K=64, epi=0, status=None)
     a.update(kw)
     return _lib.load().rd_gemm_int8(*a.values(), None)
+
+
+def linear(**kw):
+    a = dict(x=P, ldx=64, codes=P, ld=64, scales=P, W=P, ldw=64, sw=P, C=P, ldc=8, R=None, ldr=0, m_dev=None, status=None, dtype=1, out=1, m=2, N=8, K=64, epi=0)
+    a.update(kw)
+    return _lib.load().rd_linear_int8(_lib.LINEAR_INT8.pack(*order(a, "x ldx codes ld scales W ldw sw C ldc R ldr m_dev status dtype out m N K epi")), None)
 
 
 ARG, DTYPE, SIZE, ALIGN, UNSUPPORTED = -1, -2, -3, -5, -6
@@ -64,6 +77,8 @@ ARG, DTYPE, SIZE, ALIGN, UNSUPPORTED = -1, -2, -3, -5, -6
     (rows, dict(dtype=2), DTYPE), (rows, dict(K=0), ARG), (rows, dict(ld=48), ARG), (rows, dict(x=None), ARG), (rows, dict(codes=P + 8), ALIGN), (rows, dict(ld=72), ALIGN),
     (product, dict(out=2), DTYPE), (product, dict(epi=1), UNSUPPORTED), (product, dict(K=40), SIZE), (product, dict(K=131088, lda=131088, ldw=131088), SIZE),
     (product, dict(epi=5, N=7), SIZE), (product, dict(A=None), ARG), (product, dict(epi=4), ARG), (product, dict(lda=48), ARG), (product, dict(ldc=7), ARG),
+    (linear, dict(dtype=7), DTYPE), (linear, dict(out=7), DTYPE), (linear, dict(epi=2), UNSUPPORTED), (linear, dict(K=65), ARG), (linear, dict(K=60, ld=48), ARG),
+    (linear, dict(x=None), ARG), (linear, dict(W=None), ARG), (linear, dict(codes=P + 8), ALIGN), (linear, dict(ldw=72), ALIGN), (linear, dict(epi=5, N=9), SIZE),
     (product, dict(A=P + 8), ALIGN), (product, dict(ldw=72), ALIGN), (product, dict(C=P + 1), ALIGN),
 ])
 def test_refused(call, kw, want):
@@ -71,7 +86,7 @@ def test_refused(call, kw, want):
 
 
 @pytest.mark.parametrize("call, kw", [(append, dict(m=0)), (append, dict(B=0)), (read, dict(out_len=0)), (read, dict(B=0)), (attend, dict(m=0)), (attend, dict(B=0)),
-                                      (attend, dict(max_new=0)), (rows, dict(m=0)), (product, dict(m=0))])
+                                      (attend, dict(max_new=0)), (rows, dict(m=0)), (product, dict(m=0)), (linear, dict(m=0))])
 def test_nothing_to_do(call, kw):
     assert call(**kw) == 0
 
@@ -119,6 +134,14 @@ def test_int8_linear_refuses_on_the_host():
         Int8Linear.from_codes(torch.zeros(4, 16), torch.ones(4))
     with pytest.raises(rd._lib.RedrafterError, match="codes"):
         rd.modeling_common.quantize_rows(torch.zeros(2, 20), torch.zeros(2, 20, dtype=torch.int8), torch.zeros(2))
+
+
+def test_structs_agree_with_the_header():
+    sizes = [x.size for x in (_lib.CACHE_APPEND, _lib.CACHE_READ, _lib.ATTENTION_QUANT, _lib.LINEAR_INT8)]
+    assert [_lib.load().rd_quant_desc_bytes(i) for i in range(4)] == sizes
+    assert _lib.load().rd_quant_desc_bytes(4) < 0
+    for call in ("rd_cache_quant_append", "rd_cache_quant_read", "rd_attention_quant", "rd_linear_int8"):
+        assert getattr(_lib.load(), call)(None, None) == ARG
 
 
 def test_workspace_sizes_are_host_calls():
