@@ -209,35 +209,43 @@ int launch_few(const Args& a, const FewPlan& p, void* workspace, int32_t* status
 // The many-rows kernel serves the other 16-bit calls of such heads.
 struct ManyPlan {
   bool here;
+  int tiles;    // of 128 query rows to a CTA
   int n_split;
 };
 ManyPlan many_plan(int dtype, int B, int nh, int nkv, int hd, int max_new, int max_kv) {
-  ManyPlan p{dtype == RD_BF16 && (hd == 64 || hd == 128) && (int64_t)max_new * (nh / nkv) > kFewRows, 1};
+  const int64_t rows = (int64_t)max_new * (nh / nkv), chains = (int64_t)B * nkv;
+  ManyPlan p{dtype == RD_BF16 && (hd == 64 || hd == 128) && rows > kFewRows, 1, 1};
   if (!p.here) return p;
-  // Shares of the keys where the query tiles leave CTAs idle: enough to fill two to an SM, each of at least four tiles.
-  const int64_t chains = (int64_t)B * nkv * (((int64_t)max_new * (nh / nkv) + kManyRows - 1) / kManyRows), slots = 2 * sm_count();
-  if (2 * chains >= slots) return p;
-  const int64_t by_fill = slots / chains, by_length = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys / 4;
+  // two tiles to a CTA where these CTAs, one on an SM, still fill the SMs
+  if (chains * ((rows + 2 * kManyRows - 1) / (2 * kManyRows)) >= sm_count() && rows > kManyRows) p.tiles = 2;
+  // Shares of the keys where the query tiles leave CTAs idle: enough to fill two to an SM, each of at least four tiles of keys.
+  const int64_t ctas = chains * ((rows + p.tiles * kManyRows - 1) / (p.tiles * kManyRows)), slots = 2 * sm_count() / p.tiles;
+  if (2 * ctas >= slots) return p;
+  const int64_t by_fill = slots / ctas, by_length = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys / 4;
   int64_t n = by_fill < by_length ? by_fill : by_length;
   n = n < kManyMaxSplit ? n : kManyMaxSplit;
   p.n_split = n > 1 ? (int)n : 1;
   return p;
 }
 
-template <int HD, int BITS>
+template <int HD, int BITS, int QT>
 int launch_many(const Args& a, const ManyPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
-  constexpr auto kernel = attention_quant_many_kernel<HD, BITS>;
-  RD_REQUIRE(allow_smem<kernel>(ManySmem<HD>::kBytes), RD_ERR_LAUNCH);
-  const int64_t tiles = ((int64_t)a.max_new * (a.nh / a.nkv) + kManyRows - 1) / kManyRows * p.n_split;
+  constexpr auto kernel = attention_quant_many_kernel<HD, BITS, QT>;
+  using L = Many<HD, QT>;
+  RD_REQUIRE(allow_smem<kernel>(L::kBytes), RD_ERR_LAUNCH);
+  const int64_t tiles = ((int64_t)a.max_new * (a.nh / a.nkv) + QT * kManyRows - 1) / (QT * kManyRows) * p.n_split;
   RD_REQUIRE(tiles <= 0x7fffffff, RD_ERR_SIZE);
-  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)tiles, a.nkv, a.B), dim3(kManyThreads), ManySmem<HD>::kBytes, s, 1, a, (float*)workspace, p.n_split,
-                                       status);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)tiles, a.nkv, a.B), dim3(L::kThreads), L::kBytes, s, 1, a, (float*)workspace, p.n_split, status);
   RD_CHECK_CHAINED(err);
   if (p.n_split == 1) return RD_OK;
   err = rd::launch_chained(attention_quant_merge_shares_kernel<HD>, dim3((unsigned)(((int64_t)a.max_new * a.nh + 7) / 8), a.B), dim3(256), 0, s, 1, a,
                            (const float*)workspace, p.n_split);
   RD_CHECK_CHAINED(err);
   return RD_OK;
+}
+template <int HD, int BITS>
+int launch_many(const Args& a, const ManyPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
+  return p.tiles == 2 ? launch_many<HD, BITS, 2>(a, p, workspace, status, s) : launch_many<HD, BITS, 1>(a, p, workspace, status, s);
 }
 
 }  // namespace

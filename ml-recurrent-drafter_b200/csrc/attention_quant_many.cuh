@@ -1,32 +1,61 @@
 // Attention over a cache in codes for many query rows to a key/value head (packed drafts, prompts), on the 5th-generation tensor cores:
 // included by attention_quant.cu.
 //
-// One CTA serves 128 query rows of one (batch row, key/value head): row R is head R % group of new token R / group, so that the codes of a
-// tile are unpacked once for all heads of a group.
-//   warps 0-3  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), S times
-//              its keys' scales, running maximum (moved only when exceeded by 2^6) and sum, weights W = p scale_v / r 2^8 as fp16 to TMEM;
-//   warps 4-7  unpacking: codes minus their zeros as fp16 (exact: 1024 + code is one masking instruction, minus 1024 + zero) into
-//              swizzled shared-memory tiles of 64 keys, two stages each for K and V; scales of keys and values beside them.  r, a power
-//              of two, is the largest value scale of the tiles so far;
-//   warp 8     issues S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
+// One CTA serves QT tiles of 128 query rows of one (batch row, key/value head): row R is head R % group of new token R / group, so that the codes of
+// a tile of keys are unpacked once for all of them.
+//   4 QT warps  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), S times
+//               its keys' scales, running maximum (moved only when exceeded by 2^6) and sum, weights W = p scale_v / r 2^8 as fp16 to TMEM;
+//   4 warps     unpacking: codes minus their zeros as fp16 (exact: 1024 + code is one masking instruction, minus 1024 + zero) into
+//               swizzled shared-memory tiles of 64 keys, two stages each for K and V; scales of keys and values beside them.  r, a power
+//               of two, is the largest value scale of the tiles so far;
+//   1 warp      issues S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
+// S has two buffers, W of a tile takes the place of its S: QK of the next tile runs under the softmax of this one.  A tile is read from TMEM once, 32
+// scores at a time, and weighted by the maximum so far; only where that turns out too low is it done again.
 // Features lie in the order in which the masks deliver them (within 8 of 4 bits: 0 4 1 5 2 6 3 7, within 4 of 8 bits: 0 2 1 3); the queries
-// take the same order, the output undoes it.  Two CTAs on an SM overlap each other's waits.
+// take the same order, the output undoes it.  QT = 1: two CTAs on an SM overlap each other's waits; QT = 2: one, which unpacks half as often.
 // With n_split > 1 a CTA walks its share of the tiles and leaves its sums for attention_quant_merge_shares_kernel.
 //
 // Every wait is bounded; on give-up the kernel records a code in *status, frees its TMEM and returns.
 
-constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 288;
+constexpr int kManyRows = 128, kManyKeys = 64;
 constexpr int kManyMaxSplit = 16;
-constexpr float kManySlack = 6.f;      // log2 units that a tile's maximum may exceed the running one
-constexpr uint32_t kColS = 0, kColP = 64, kColO = 128;  // TMEM: S 64 fp32 columns, W two buffers of 32, O HD
+constexpr float kManySlack = 6.f;  // log2 units that a tile's maximum may exceed the running one
 
-template <int HD>
-struct ManySmem {
-  static constexpr int kQ = kManyRows * HD * 2, kTile = kManyKeys * HD * 2;
-  static constexpr int kVectors = 4 * kManyKeys * 4 * 2 + 4 * 4;  // scales of keys and values of four tiles, and r of each
-  static constexpr int kBytes = 1024 + kQ + 4 * kTile + kVectors + kManyRows * 4 + 32 * 8;
-  static constexpr uint32_t kTmemCols = 256;
+template <int HD, int QT>
+struct Many {
+  static constexpr int kThreads = (4 * QT + 5) * 32;
+  static constexpr int kQ = kManyRows * HD * 2, kTile = kManyKeys * HD * 2;  // bytes
+  static constexpr int kVectors = 4 * kManyKeys * 4 * 2 + 4 * 4;             // scales of keys and values of four tiles, and r of each
+  static constexpr int kBytes = 1024 + QT * kQ + 4 * kTile + kVectors + QT * kManyRows * 4 + 32 * 8;
+  // TMEM of a tile of rows: two buffers of 64 columns for S, then W; O
+  static constexpr uint32_t kColS = 0, kColO = 128, kCols = 128 + HD;
+  static constexpr uint32_t kTmem = QT * kCols <= 256 ? 256 : 512;
 };
+
+using F2 = unsigned long long;  // two fp32 numbers
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ void unpack2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+// two pairs, the same for all lanes of a warp
+__device__ __forceinline__ void lds_pairs(uint32_t at, F2& a, F2& b) { asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(at) : "memory"); }
 
 __device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
   if (rd_umma::mbar_try(bar, parity)) return true;
@@ -48,6 +77,22 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// complete only after a wait::st
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 // fp16 operands, fp32 accumulator, M = 128
@@ -77,24 +122,29 @@ __device__ __forceinline__ constexpr int order8(int k) {
   return BITS == 4 ? (k < 4 ? 2 * k : 2 * (k - 4) + 1) : (k & 4) + ((k & 1) * 2 + ((k >> 1) & 1));
 }
 
-template <int HD, int BITS>
-__global__ void __launch_bounds__(kManyThreads, 2)
+template <int HD, int BITS, int QT>
+__global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     attention_quant_many_kernel(const Args a, float* partial, int n_split, int32_t* status) {
-  using Sm = ManySmem<HD>;
+  using L = Many<HD, QT>;
+  constexpr int kUnpack = 4 * QT, kIssue = kUnpack + 4;  // first warps of these roles
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;
-  uint8_t* sK = smem + Sm::kQ;
-  uint8_t* sV = sK + 2 * Sm::kTile;
-  float* k_scale = reinterpret_cast<float*>(sV + 2 * Sm::kTile);  // [4][64]
-  float* v_scale = k_scale + 4 * kManyKeys;                       // [4][64], over r, times 2^8
-  float* refs = v_scale + 4 * kManyKeys;                          // [4]
-  float* units = refs + 4;                                        // [128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(units + kManyRows);
-  uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *s_full = bars + 5, *o_full = bars + 7, *p_full = bars + 9, *s_empty = bars + 11;
-  uint64_t* scales_full = bars + 12;  // [4]: the scales of a tile are there; a tile's place is written again only when the softmax is done with it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  uint8_t* sK = smem + QT * L::kQ;
+  uint8_t* sV = sK + 2 * L::kTile;
+  float* k_scale = reinterpret_cast<float*>(sV + 2 * L::kTile);  // [4][64]
+  float* v_scale = k_scale + 4 * kManyKeys;                      // [4][64], over r, times 2^8
+  float* refs = v_scale + 4 * kManyKeys;                         // [4]
+  float* units = refs + 4;                                       // [QT][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(units + QT * kManyRows);
+  uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7;
+  uint64_t* scales_full = bars + 9;       // [4]: the scales of a tile are there; its place is written again only when the softmax is done with it
+  uint64_t* s_full = bars + 13;           // [QT][2]
+  uint64_t* p_full = s_full + 2 * QT;     // [QT][2]
+  uint64_t* o_full = p_full + 2 * QT;     // [QT][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2 * QT);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(13 + 6 * 2 + 1 <= 32, "barriers");
 
   const int group = a.nh / a.nkv;
   // in causal calls later tiles see more keys: they start first
@@ -102,33 +152,37 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   const int linear = (int)(blockIdx.x + gridDim.x * blockIdx.y);
   const int bx = late_first ? (int)gridDim.x - 1 - linear / (int)gridDim.y : (int)blockIdx.x;
   const int hk = late_first ? linear % (int)gridDim.y : (int)blockIdx.y;
-  const int b = blockIdx.z, split = bx % n_split, q0 = bx / n_split * kManyRows;
+  const int b = blockIdx.z, split = bx % n_split, q0 = bx / n_split * (QT * kManyRows);
   rd::pdl_launch_dependents();
   rd::pdl_wait();
   const Row r = row_of(a, b);
   const int rows = r.n_new * group;
   if (q0 >= rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first_token = q0 / group, last_token = (min(q0 + kManyRows, rows) - 1) / group;
+  const int n_q = QT == 1 ? 1 : min(QT, (rows - q0 + kManyRows - 1) / kManyRows);  // tiles of rows that there are
+  const int first_token = q0 / group, last_token = (min(q0 + QT * kManyRows, rows) - 1) / group;
   const int kv_end = a.mode == RD_ATTN_CAUSAL ? min(r.end, r.base + last_token + 1) : r.end;
   const int all_tiles = (max(kv_end, 0) + kManyKeys - 1) / kManyKeys;
   const int per_split = (all_tiles + n_split - 1) / n_split;
   const int t_begin = split * per_split, n_tiles = max(0, min(per_split, all_tiles - t_begin));
   if (threadIdx.x == 0) {
-    rd_umma::mbar_init(q_full, 4);
+    rd_umma::mbar_init(q_full, 4 * n_q);
     for (int s = 0; s < 2; ++s) {
       rd_umma::mbar_init(&k_full[s], 4);
       rd_umma::mbar_init(&v_full[s], 4);
-      rd_umma::mbar_init(&s_full[s], 1);
-      rd_umma::mbar_init(&o_full[s], 1);
-      rd_umma::mbar_init(&p_full[s], 4);
+      rd_umma::mbar_init(&k_empty[s], 1);
+      rd_umma::mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 4; ++s) rd_umma::mbar_init(&scales_full[s], 4);
-    rd_umma::mbar_init(s_empty, 4);
+    for (int s = 0; s < 2 * QT; ++s) {
+      rd_umma::mbar_init(&s_full[s], 1);
+      rd_umma::mbar_init(&p_full[s], 4);
+      rd_umma::mbar_init(&o_full[s], 1);
+    }
     *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) rd_umma::tmem_alloc(tmem_slot, Sm::kTmemCols);
+  if (warp == kIssue) rd_umma::tmem_alloc(tmem_slot, L::kTmem);
   rd_umma::fence_before();
   __syncthreads();
   rd_umma::fence_after();
@@ -136,11 +190,11 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   bool ok = true;
   int site = 0;
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= kUnpack && warp < kIssue) {
     // ---------------- unpacking ----------------
     constexpr int kBytes = HD * BITS / 16;  // a thread's half of a key: 16, 32 or 64 bytes
     constexpr int kLoads = kBytes / 16, kChunks = HD / 16, kWordsOf8 = BITS / 4;
-    const int tid = threadIdx.x - 128, key = tid & 63, half = tid >> 6;
+    const int tid = threadIdx.x - kUnpack * 32, key = tid & 63, half = tid >> 6;
     const int64_t plane = ((int64_t)b * a.nkv + hk) * a.max_len + r.first;
     uint4 kc[kLoads], vc[kLoads];
     uint32_t kp = 0, vp = 0, vq = 0;
@@ -176,15 +230,16 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       request_v(0);
     }
     for (int t = 0; t < n_tiles; ++t) {
-      if (t >= 2 && !warp_wait_or(&s_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
+      if (t >= 2 && !warp_wait_or(&k_empty[t & 1], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 1;
         break;
       }
-      store(sK + (t & 1) * Sm::kTile, kc, kp);
+      store(sK + (t & 1) * L::kTile, kc, kp);
       // scales are never negative; NaN counts as none
       const float v0 = param_scale(vp), v1 = param_scale(vq);
       const uint32_t bits = max(v0 == v0 ? __float_as_uint(v0) : 0u, v1 == v1 ? __float_as_uint(v1) : 0u);
       top = max(max(top, 27u << 23), __reduce_max_sync(0xffffffffu, bits) & 0x7f800000u);
+      // QK of tile t - 2 is done: it was issued when the softmax was through with tile t - 4, whose place this is
       if (half == 0) {
         k_scale[(t & 3) * kManyKeys + key] = param_scale(kp);
         v_scale[(t & 3) * kManyKeys + key] = v0 * __uint_as_float((262u << 23) - top);  // 2^8 / r
@@ -198,27 +253,31 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         mbar_arrive(&scales_full[t & 3]);
         mbar_arrive(&k_full[t & 1]);
       }
-      if (t >= 2 && !warp_wait_or(&o_full[t & 1], ((t - 2) >> 1) & 1, stop)) {
+      if (t >= 2 && !warp_wait_or(&v_empty[t & 1], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 2;
         break;
       }
-      store(sV + (t & 1) * Sm::kTile, vc, vz);
+      store(sV + (t & 1) * L::kTile, vc, vz);
       if (t + 1 < n_tiles) request_v(t + 1);
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[t & 1]);
     }
-  } else if (warp == 8) {
+  } else if (warp == kIssue) {
     // ---------------- products ----------------
     if (rd::elect_one()) {
       const uint32_t idesc_qk = idesc_fp16(kManyKeys, false), idesc_pv = idesc_fp16(HD, true);
       auto issue_qk = [&](int t) {
-        const uint32_t k = rd_umma::smem_u32(sK + (t & 1) * Sm::kTile), q = rd_umma::smem_u32(sQ);
+        const uint32_t k = rd_umma::smem_u32(sK + (t & 1) * L::kTile);
+        for (int x = 0; x < n_q; ++x) {
+          const uint32_t q = rd_umma::smem_u32(sQ + x * L::kQ);
 #pragma unroll
-        for (int kd = 0; kd < HD / 16; ++kd)
-          rd_umma::mma_ss(tmem + kColS, rd_umma::desc_k_major(q + (kd >> 2) * (kManyRows * 128) + (kd & 3) * 32),
-                          rd_umma::desc_k_major(k + (kd >> 2) * (kManyKeys * 128) + (kd & 3) * 32), idesc_qk, kd != 0);
-        rd_umma::commit(&s_full[t & 1]);
+          for (int kd = 0; kd < HD / 16; ++kd)
+            rd_umma::mma_ss(tmem + x * L::kCols + L::kColS + (t & 1) * 64, rd_umma::desc_k_major(q + (kd >> 2) * (kManyRows * 128) + (kd & 3) * 32),
+                            rd_umma::desc_k_major(k + (kd >> 2) * (kManyKeys * 128) + (kd & 3) * 32), idesc_qk, kd != 0);
+          rd_umma::commit(&s_full[2 * x + (t & 1)]);
+        }
+        rd_umma::commit(&k_empty[t & 1]);
       };
       ok = mbar_wait_or(q_full, 0, stop);
       if (ok && n_tiles > 0) {
@@ -230,31 +289,38 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       }
       for (int t = 0; ok && t < n_tiles; ++t) {
         if (t + 1 < n_tiles) {
-          ok = mbar_wait_or(&k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, stop) && mbar_wait_or(s_empty, t & 1, stop);
+          // its buffer held W of tile t - 1, whose product has been issued before: products run in that order
+          ok = mbar_wait_or(&k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, stop);
           if (!ok) break;
           rd_umma::fence_after();
           issue_qk(t + 1);
         }
-        ok = mbar_wait_or(&p_full[t & 1], (t >> 1) & 1, stop) && mbar_wait_or(&v_full[t & 1], (t >> 1) & 1, stop);
-        if (!ok) break;
-        rd_umma::fence_after();
-        const uint32_t v = rd_umma::smem_u32(sV + (t & 1) * Sm::kTile);
+        for (int x = 0; ok && x < n_q; ++x) {
+          ok = mbar_wait_or(&p_full[2 * x + (t & 1)], (t >> 1) & 1, stop) && (x > 0 || mbar_wait_or(&v_full[t & 1], (t >> 1) & 1, stop));
+          if (!ok) break;
+          rd_umma::fence_after();
+          const uint32_t v = rd_umma::smem_u32(sV + (t & 1) * L::kTile);
 #pragma unroll
-        for (int ks = 0; ks < kManyKeys / 16; ++ks)
-          mma_ts(tmem + kColO, tmem + kColP + (t & 1) * 32 + ks * 8, rd_umma::desc_mn_major(v + ks * 2048, kManyKeys * 128), idesc_pv, (t | ks) != 0);
-        rd_umma::commit(&o_full[t & 1]);
+          for (int ks = 0; ks < kManyKeys / 16; ++ks)
+            mma_ts(tmem + x * L::kCols + L::kColO, tmem + x * L::kCols + L::kColS + (t & 1) * 64 + ks * 8, rd_umma::desc_mn_major(v + ks * 2048, kManyKeys * 128),
+                   idesc_pv, (t | ks) != 0);
+          rd_umma::commit(&o_full[2 * x + (t & 1)]);
+        }
+        if (ok) rd_umma::commit(&v_empty[t & 1]);
       }
       if (!ok) site = 3;
     }
     __syncwarp();
-  } else {
+  } else if (warp < 4 * n_q) {
+    const int tile = warp >> 2, quarter = warp & 3;
+    uint8_t* myQ = sQ + tile * L::kQ;
     // ---------------- queries: eight lanes a row ----------------
     {
       const int part = lane & 7;
       constexpr int kPart = HD / 8;  // features of a lane: 8 or 16
 #pragma unroll 2
       for (int i = 0; i < 8; ++i) {
-        const int row = warp * 32 + i * 4 + (lane >> 3), R = q0 + row;
+        const int row = quarter * 32 + i * 4 + (lane >> 3), R = q0 + tile * kManyRows + row;
         const bool live = R < rows;
         const __nv_bfloat16* src =
             (const __nv_bfloat16*)a.q + (int64_t)(r.start + (live ? R / group : 0)) * a.ldq + (hk * group + (live ? R % group : 0)) * HD + part * kPart;
@@ -281,26 +347,75 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 #pragma unroll
           for (int k = 0; k < 8; ++k) y[order8<BITS>(k)] = x[8 * c + k] * f1 * f2;
           const int chunk = part * (kPart / 8) + c;
-          *reinterpret_cast<uint4*>(sQ + (chunk >> 3) * (kManyRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(myQ + (chunk >> 3) * (kManyRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
               make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7]));
         }
         if (part == 0)
-          units[row] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
+          units[tile * kManyRows + row] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
       }
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
     // ---------------- softmax: a thread a row ----------------
-    const int row = warp * 32 + lane, R = q0 + row;
+    const int row = quarter * 32 + lane, R = q0 + tile * kManyRows + row;
     const bool live = R < rows;
     const int token = live ? R / group : 0;
-    const float unit = units[row];  // its own warp's
-    const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+    const float unit = units[tile * kManyRows + row];  // its own warp's
+    const uint32_t taddr = tmem + tile * L::kCols + ((uint32_t)(quarter * 32) << 16);
     const int all_see = a.mode == RD_ATTN_CAUSAL ? min(kv_end, r.base + first_token + 1) : min(kv_end, r.base);
     float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
+    // One tile's weights (packed, 32 words) at the maximum m; returns their sum and the tile's largest score.
+    auto weigh = [&](auto whole, int t, uint64_t vis, float m, uint32_t* w, float& mx) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const uint32_t ks = rd_umma::smem_u32(k_scale + (t & 3) * kManyKeys), vs = rd_umma::smem_u32(v_scale + (t & 3) * kManyKeys);
+      const float off = m == -INFINITY ? 0.f : -m;
+      const F2 unit2 = pack2(unit, unit), off2 = pack2(off, off);
+      F2 sum = 0;
+      float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float s[32];
+        rd_umma::tmem_ld32(taddr + L::kColS + (t & 1) * 64 + 32 * hf, s);
+        const uint32_t v = (uint32_t)(vis >> (32 * hf));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          F2 k[2], f[2];
+          lds_pairs(ks + 128 * hf + 16 * i, k[0], k[1]);
+          lds_pairs(vs + 128 * hf + 16 * i, f[0], f[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int n = 4 * i + 2 * e;
+            F2 x = mul2(pack2(s[n], s[n + 1]), k[e]);
+            float x0, x1;
+            unpack2(x, x0, x1);
+            if (!WHOLE) {
+              if (!((v >> n) & 1)) x0 = -INFINITY;
+              if (!((v >> (n + 1)) & 1)) x1 = -INFINITY;
+              x = pack2(x0, x1);
+            }
+            part[2 * e] = fmaxf(part[2 * e], x0);
+            part[2 * e + 1] = fmaxf(part[2 * e + 1], x1);
+            unpack2(fma2(x, unit2, off2), x0, x1);
+            x0 = ex2(x0), x1 = ex2(x1);
+            const F2 p = pack2(x0, x1);
+            sum = add2(sum, p);
+            unpack2(mul2(p, f[e]), x0, x1);
+            if (!WHOLE) {  // a hidden value counts for nothing, NaN or not
+              if (!((v >> n) & 1)) x0 = 0.f;
+              if (!((v >> (n + 1)) & 1)) x1 = 0.f;
+            }
+            w[16 * hf + 2 * i + e] = pack_f16(x0, x1);
+          }
+        }
+      }
+      mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      float s0, s1;
+      unpack2(sum, s0, s1);
+      return s0 + s1;
+    };
     for (int t = 0; t < n_tiles; ++t) {
-      if (!warp_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !warp_wait_or(&s_full[t & 1], (t >> 1) & 1, stop)) {
+      if (!warp_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !warp_wait_or(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
         ok = false, site = 4;
         break;
       }
@@ -325,108 +440,51 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         if (n_in < 64) vis &= (1ull << max(n_in, 0)) - 1ull;
         if (!live) vis = 0;
       }
-      const float4* ks = reinterpret_cast<const float4*>(k_scale + (t & 3) * kManyKeys);
-      const float4* vs = reinterpret_cast<const float4*>(v_scale + (t & 3) * kManyKeys);
       const float ref_t = refs[t & 3];
-      float mx = -INFINITY;
-      // S is read twice, a half at a time: 64 scores and their weights at once would not fit the registers of two CTAs
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float s[32];
-        rd_umma::tmem_ld32(taddr + kColS + 32 * hf, s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 f = ks[8 * hf + i];
-          s[4 * i] *= f.x, s[4 * i + 1] *= f.y, s[4 * i + 2] *= f.z, s[4 * i + 3] *= f.w;
+      float keep = ref_t != ref && t > 0 ? ref / ref_t : 1.f;  // what O is to be multiplied with
+      ref = ref_t;
+      uint32_t w[32];
+      float sum;
+      for (;;) {
+        float mx;
+        sum = whole ? weigh(std::true_type(), t, vis, m_run, w, mx) : weigh(std::false_type(), t, vis, m_run, w, mx);
+        const float mx2 = mx * unit;
+        const bool moved = mx2 > m_run + kManySlack;  // also for the first visible key
+        if (!__any_sync(0xffffffffu, moved)) break;
+        // again, at the tile's own maximum: not a second time
+        if (moved) {
+          const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - mx2);
+          l_run *= alpha;
+          if (m_run != -INFINITY) keep *= alpha;
+          m_run = mx2;
         }
-        if (!whole) {
-          const uint32_t v = (uint32_t)(vis >> (32 * hf));
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((v >> i) & 1)) s[i] = -INFINITY;
-        }
-        float part[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], s[i]);
-        mx = fmaxf(mx, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
       }
-      const float mx2 = mx * unit;
-      const bool moved = mx2 > m_run + kManySlack;  // also for the first visible key
-      const float m_new = moved ? mx2 : m_run;
-      const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - m_new);
-      float keep = moved && m_run != -INFINITY ? alpha : 1.f;
-      l_run *= moved ? alpha : 1.f;
-      m_run = m_new;
-      if (ref_t != ref) {
-        if (t > 0) keep *= ref / ref_t;
-        ref = ref_t;
-      }
+      l_run += sum;
       if (__any_sync(0xffffffffu, t > 0 && keep != 1.f)) {
         // O has to be quiet while it is brought to the new maximum or r
-        if (!warp_wait_or(&o_full[(t - 1) & 1], ((t - 1) >> 1) & 1, stop)) {
+        if (!warp_wait_or(&o_full[2 * tile + ((t - 1) & 1)], ((t - 1) >> 1) & 1, stop)) {
           ok = false, site = 5;
           break;
         }
         rd_umma::fence_after();
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          float x[32];
-          rd_umma::tmem_ld32(taddr + kColO + c * 32, x);
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t x[16];
+          tmem_ld16(taddr + L::kColO + c * 16, x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] *= keep;
-          rd_umma::tmem_st32(taddr + kColO + c * 32, x);
+          for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * keep);
+          tmem_st16(taddr + L::kColO + c * 16, x);
         }
       }
-      const float off = m_run == -INFINITY ? 0.f : -m_run;
-      float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float s[32];
-        rd_umma::tmem_ld32(taddr + kColS + 32 * hf, s);
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 f = ks[8 * hf + i];
-          s[4 * i] *= f.x, s[4 * i + 1] *= f.y, s[4 * i + 2] *= f.z, s[4 * i + 3] *= f.w;
-        }
-        const uint32_t v = (uint32_t)(vis >> (32 * hf));
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          s[i] = ex2(fmaf(s[i], unit, off));
-          if (!whole && !((v >> i) & 1)) s[i] = 0.f;
-          if (i & 1) sum1 += s[i];
-          else sum0 += s[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 f = vs[8 * hf + i];
-          float y[4] = {s[4 * i] * f.x, s[4 * i + 1] * f.y, s[4 * i + 2] * f.z, s[4 * i + 3] * f.w};
-          if (!whole) {  // a hidden value counts for nothing, NaN or not
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!((v >> (4 * i + e)) & 1)) y[e] = 0.f;
-          }
-          w[2 * i] = pack_f16(y[0], y[1]);
-          w[2 * i + 1] = pack_f16(y[2], y[3]);
-        }
-        asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
-                taddr + kColP + (t & 1) * 32 + 16 * hf),
-            "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11]),
-            "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-            : "memory");
-      }
+      tmem_st16(taddr + L::kColS + (t & 1) * 64, w);
+      tmem_st16(taddr + L::kColS + (t & 1) * 64 + 16, w + 16);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      l_run += sum0 + sum1;
       rd_umma::fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(s_empty);
-        mbar_arrive(&p_full[t & 1]);
-      }
+      if (lane == 0) mbar_arrive(&p_full[2 * tile + (t & 1)]);
     }
     if (ok && n_tiles > 0) {
-      ok = warp_wait_or(&o_full[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, stop);
+      ok = warp_wait_or(&o_full[2 * tile + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, stop);
       if (!ok) site = 6;
     }
     if (ok) {
@@ -438,7 +496,7 @@ __global__ void __launch_bounds__(kManyThreads, 2)
       for (int c = 0; c < HD / 32; ++c) {
         float x[32], y[32];
         if (n_tiles > 0) {
-          rd_umma::tmem_ld32(taddr + kColO + c * 32, x);
+          rd_umma::tmem_ld32(taddr + L::kColO + c * 32, x);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = 0.f;
@@ -466,9 +524,9 @@ __global__ void __launch_bounds__(kManyThreads, 2)
   if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 420 + site);
   rd_umma::fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kIssue) {
     rd_umma::fence_after();
-    rd_umma::tmem_dealloc(tmem, Sm::kTmemCols);
+    rd_umma::tmem_dealloc(tmem, L::kTmem);
   }
 }
 
