@@ -3,14 +3,18 @@
 //
 // One CTA serves QT tiles of 128 query rows of one (batch row, key/value head): row R is head R % group of new token R / group, so that the codes of
 // a tile of keys are unpacked once for all of them.
-//   4 QT warps  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), S times
-//               its keys' scales, running maximum (moved only when exceeded by 2^6) and sum, weights W = p scale_v / r 2^8 as fp16 to TMEM;
-//   4 warps     unpacking: codes minus their zeros as fp16 (exact: 1024 + code is one masking instruction, minus 1024 + zero) into
-//               swizzled shared-memory tiles of 64 keys, two stages each for K and V; scales of keys and values beside them.  r, a power
-//               of two, is the largest value scale of the tiles so far;
+//   4 QT warps  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), running
+//               maximum and sum, weights W = 2^7 p as fp16 to TMEM;
+//   4 warps     unpacking: codes minus their zeros (exact: 1024 + code is one masking instruction, minus 1024 + zero) times their scales
+//               over a power of two, fp16, into swizzled shared-memory tiles of 64 keys, two stages each for K and V.  For keys that power
+//               is of the tile and goes into the scores' unit; for values it is r, that of the largest scale so far;
 //   1 warp      issues S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
-// S has two buffers, W of a tile takes the place of its S: QK of the next tile runs under the softmax of this one.  A tile is read from TMEM once, 32
-// scores at a time, and weighted by the maximum so far; only where that turns out too low is it done again.
+// Keys, values and weights are thus rounded to fp16's 11 bits, each by at most 2^-12 of itself, an eighth of what a bf16 cache costs.  With the
+// scales left to the softmax instead (codes alone are exact) its 64 x 128 scores cost four instructions for two where they now take
+// two and a half, which bounded the kernel: a tile of 256 rows 2560 cycles.
+// S has two buffers, W of a tile takes the place of its S: QK of the next tile runs under the softmax of this one.  A tile is read from TMEM once,
+// 32 scores at a time, and weighted by the maximum so far; only where the sum of the weights turns out too large the tile's maximum is
+// looked for and the tile weighted again.
 // Features lie in the order in which the masks deliver them (within 8 of 4 bits: 0 4 1 5 2 6 3 7, within 4 of 8 bits: 0 2 1 3); the queries
 // take the same order, the output undoes it.  QT = 1: two CTAs on an SM overlap each other's waits; QT = 2: one, which unpacks half as often.
 // With n_split > 1 a CTA walks its share of the tiles and leaves its sums for attention_quant_merge_shares_kernel.
@@ -19,19 +23,25 @@
 
 constexpr int kManyRows = 128, kManyKeys = 64;
 constexpr int kManyMaxSplit = 16;
-constexpr float kManySlack = 6.f;  // log2 units that a tile's maximum may exceed the running one
+constexpr float kWeightBits = 7.f;        // weights are 2^7 p
+constexpr float kMostWeights = 32768.f;   // of a tile of a row: none is more, and fp16 holds it
 
 template <int HD, int QT>
 struct Many {
   static constexpr int kThreads = (4 * QT + 5) * 32;
   static constexpr int kQ = kManyRows * HD * 2, kTile = kManyKeys * HD * 2;  // bytes
-  static constexpr int kVectors = 4 * kManyKeys * 4 * 2 + 4 * 4;             // scales of keys and values of four tiles, and r of each
+  static constexpr int kVectors = 4 * 4 * 4;                                // of four tiles: r, the keys' power of two, which values are NaN
   static constexpr int kBytes = 1024 + QT * kQ + 4 * kTile + kVectors + QT * kManyRows * 4 + 32 * 8;
   // TMEM of a tile of rows: two buffers of 64 columns for S, then W; O
   static constexpr uint32_t kColS = 0, kColO = 128, kCols = 128 + HD;
   static constexpr uint32_t kTmem = QT * kCols <= 256 ? 256 : 512;
 };
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
 using F2 = unsigned long long;  // two fp32 numbers
 __device__ __forceinline__ F2 pack2(float a, float b) {
   F2 y;
@@ -39,11 +49,6 @@ __device__ __forceinline__ F2 pack2(float a, float b) {
   return y;
 }
 __device__ __forceinline__ void unpack2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-  return y;
-}
 __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   F2 y;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
@@ -54,9 +59,6 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
   return y;
 }
-// two pairs, the same for all lanes of a warp
-__device__ __forceinline__ void lds_pairs(uint32_t at, F2& a, F2& b) { asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(at) : "memory"); }
-
 __device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
   if (rd_umma::mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
@@ -99,9 +101,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ uint32_t idesc_fp16(int n, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// Eight codes (4 bits: one word; 8 bits: two) minus zero as fp16; z2: 1024 + zero in both halves.
+// Eight codes (4 bits: one word; 8 bits: two) minus zero, times a scale, as fp16; z2: 1024 + zero in both halves.
 template <int BITS>
-__device__ __forceinline__ uint4 unpack8(const uint32_t* w, uint32_t z2) {
+__device__ __forceinline__ uint4 unpack8(const uint32_t* w, uint32_t z2, uint32_t s2) {
   uint4 u;
   if constexpr (BITS == 4) {
     u.x = sub_f16x2((w[0] & 0x000f000fu) | 0x64006400u, z2);
@@ -114,6 +116,7 @@ __device__ __forceinline__ uint4 unpack8(const uint32_t* w, uint32_t z2) {
     u.z = sub_f16x2((w[1] & 0x00ff00ffu) | 0x64006400u, z2);
     u.w = sub_f16x2(((w[1] >> 8) & 0x00ff00ffu) | 0x64006400u, z2);
   }
+  u.x = mul_f16x2(u.x, s2), u.y = mul_f16x2(u.y, s2), u.z = mul_f16x2(u.z, s2), u.w = mul_f16x2(u.w, s2);
   return u;
 }
 // where feature k of 8 lies among them
@@ -132,13 +135,13 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
   uint8_t* sQ = smem;
   uint8_t* sK = smem + QT * L::kQ;
   uint8_t* sV = sK + 2 * L::kTile;
-  float* k_scale = reinterpret_cast<float*>(sV + 2 * L::kTile);  // [4][64]
-  float* v_scale = k_scale + 4 * kManyKeys;                      // [4][64], over r, times 2^8
-  float* refs = v_scale + 4 * kManyKeys;                         // [4]
-  float* units = refs + 4;                                       // [QT][128]
+  float* v_ref = reinterpret_cast<float*>(sV + 2 * L::kTile);          // [4]: what values are multiples of
+  float* k_ref = v_ref + 4;                                            // [4]: and keys
+  uint32_t* v_nan = reinterpret_cast<uint32_t*>(k_ref + 4);            // [4][2]: keys whose values are NaN
+  float* units = reinterpret_cast<float*>(v_nan + 8);                  // [QT][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(units + QT * kManyRows);
   uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7;
-  uint64_t* scales_full = bars + 9;       // [4]: the scales of a tile are there; its place is written again only when the softmax is done with it
+  uint64_t* scales_full = bars + 9;       // [4]: a tile's entries are there; their place is written again only when the softmax is done with it
   uint64_t* s_full = bars + 13;           // [QT][2]
   uint64_t* p_full = s_full + 2 * QT;     // [QT][2]
   uint64_t* o_full = p_full + 2 * QT;     // [QT][2]
@@ -196,72 +199,94 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     constexpr int kLoads = kBytes / 16, kChunks = HD / 16, kWordsOf8 = BITS / 4;
     const int tid = threadIdx.x - kUnpack * 32, key = tid & 63, half = tid >> 6;
     const int64_t plane = ((int64_t)b * a.nkv + hk) * a.max_len + r.first;
-    uint4 kc[kLoads], vc[kLoads];
-    uint32_t kp = 0, vp = 0, vq = 0;
-    // Keys past the last one stand for zeros.  Each half is asked for as soon as the registers of the tile before are free.
-    auto request_k = [&](int t) {
+    // Two tiles are under way: what a tile's codes are asked into is free when the tile two before has been stored, so that a trip to
+    // memory has the time of a whole tile.
+    uint4 kc[2][kLoads], vc[2][kLoads];
+    uint32_t kp[2] = {}, kq[2] = {}, vp[2] = {}, vq[2] = {};
+    // Keys past the last one stand for zeros.
+    auto request_k = [&](int t, auto set) {
+      constexpr int S = decltype(set)::value;
       const int j0 = (t_begin + t) * kManyKeys, j = j0 + key, other = j0 + (key ^ 32);
-      const bool there = j < kv_end;
+      const bool there = t < n_tiles && j < kv_end;
       const uint8_t* k = a.k_codes + (plane + j) * (HD * BITS / 8) + half * kBytes;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) kc[i] = there ? reinterpret_cast<const uint4*>(k)[i] : make_uint4(0u, 0u, 0u, 0u);
-      kp = there ? a.k_params[plane + j] : 0u;
-      vp = there ? a.v_params[plane + j] : 0u;
-      vq = other < kv_end ? a.v_params[plane + other] : 0u;  // with vp: every warp knows all 64 scales of the values
+      for (int i = 0; i < kLoads; ++i) kc[S][i] = there ? reinterpret_cast<const uint4*>(k)[i] : make_uint4(0u, 0u, 0u, 0u);
+      kp[S] = there ? a.k_params[plane + j] : 0u;
+      vp[S] = there ? a.v_params[plane + j] : 0u;
+      // with kp, vp: every warp knows all 64 scales
+      kq[S] = t < n_tiles && other < kv_end ? a.k_params[plane + other] : 0u;
+      vq[S] = t < n_tiles && other < kv_end ? a.v_params[plane + other] : 0u;
     };
-    auto request_v = [&](int t) {
+    auto request_v = [&](int t, auto set) {
+      constexpr int S = decltype(set)::value;
       const int j = (t_begin + t) * kManyKeys + key;
+      const bool there = t < n_tiles && j < kv_end;
       const uint8_t* v = a.v_codes + (plane + j) * (HD * BITS / 8) + half * kBytes;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) vc[i] = j < kv_end ? reinterpret_cast<const uint4*>(v)[i] : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < kLoads; ++i) vc[S][i] = there ? reinterpret_cast<const uint4*>(v)[i] : make_uint4(0u, 0u, 0u, 0u);
     };
-    auto store = [&](uint8_t* tile, const uint4* c, uint32_t param) {
-      const uint32_t z2 = (0x6400u + param_zero(param)) * 0x10001u;
+    auto store = [&](uint8_t* tile, const uint4* c, uint32_t param, float scale) {
+      const uint32_t z2 = (0x6400u + param_zero(param)) * 0x10001u, s2 = pack_f16(scale, scale);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int chunk = half * kChunks + i;
         *reinterpret_cast<uint4*>(tile + (chunk >> 3) * (kManyKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)) =
-            unpack8<BITS>(reinterpret_cast<const uint32_t*>(c) + i * kWordsOf8, z2);
+            unpack8<BITS>(reinterpret_cast<const uint32_t*>(c) + i * kWordsOf8, z2, s2);
       }
     };
-    uint32_t top = 0;  // exponent bits of r: at least 2^-100
-    if (n_tiles > 0) {
-      request_k(0);
-      request_v(0);
-    }
-    for (int t = 0; t < n_tiles; ++t) {
-      if (t >= 2 && !warp_wait_or(&k_empty[t & 1], ((t - 2) >> 1) & 1, stop)) {
+    // The exponent bits of the largest of a warp's scales, at least 2^-100; scales are never negative, NaN counts as none.
+    auto largest = [&](uint32_t p, uint32_t q) {
+      const float x = param_scale(p), y = param_scale(q);
+      const uint32_t bits = max(x == x ? __float_as_uint(x) : 0u, y == y ? __float_as_uint(y) : 0u);
+      return max(27u << 23, __reduce_max_sync(0xffffffffu, bits) & 0x7f800000u);
+    };
+    // Scales are taken over 2^-kUp of that power of two: below 2 before, the products with codes stay below fp16's 2^16
+    constexpr uint32_t kUp = BITS == 4 ? 10 : 6;
+    uint32_t top = 0;
+    auto unpack = [&](int t, auto set) {
+      constexpr int S = decltype(set)::value;
+      if (t >= 2 && !warp_wait_or(&k_empty[S], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 1;
-        break;
+        return;
       }
-      store(sK + (t & 1) * L::kTile, kc, kp);
-      // scales are never negative; NaN counts as none
-      const float v0 = param_scale(vp), v1 = param_scale(vq);
-      const uint32_t bits = max(v0 == v0 ? __float_as_uint(v0) : 0u, v1 == v1 ? __float_as_uint(v1) : 0u);
-      top = max(max(top, 27u << 23), __reduce_max_sync(0xffffffffu, bits) & 0x7f800000u);
+      const uint32_t k_top = largest(kp[S], kq[S]);
+      store(sK + S * L::kTile, kc[S], kp[S], param_scale(kp[S]) * __uint_as_float(((254 + kUp) << 23) - k_top));
+      top = max(top, largest(vp[S], vq[S]));
+      float v = param_scale(vp[S]);
+      const uint32_t nan = __ballot_sync(0xffffffffu, v != v);
+      v = v != v ? 0.f : v * __uint_as_float(((254 + kUp) << 23) - top);
       // QK of tile t - 2 is done: it was issued when the softmax was through with tile t - 4, whose place this is
-      if (half == 0) {
-        k_scale[(t & 3) * kManyKeys + key] = param_scale(kp);
-        v_scale[(t & 3) * kManyKeys + key] = v0 * __uint_as_float((262u << 23) - top);  // 2^8 / r
-        if (key == 0) refs[t & 3] = __uint_as_float(top);
+      if (half == 0 && lane == 0) {
+        v_nan[(t & 3) * 2 + (key >> 5)] = nan;
+        if (key == 0) v_ref[t & 3] = __uint_as_float(top - (kUp << 23)), k_ref[t & 3] = __uint_as_float(k_top - (kUp << 23));
       }
-      const uint32_t vz = vp;
-      if (t + 1 < n_tiles) request_k(t + 1);
+      const uint32_t vz = vp[S];
+      request_k(t + 2, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&scales_full[t & 3]);
-        mbar_arrive(&k_full[t & 1]);
+        mbar_arrive(&k_full[S]);
       }
-      if (t >= 2 && !warp_wait_or(&v_empty[t & 1], ((t - 2) >> 1) & 1, stop)) {
+      if (t >= 2 && !warp_wait_or(&v_empty[S], ((t - 2) >> 1) & 1, stop)) {
         ok = false, site = 2;
-        break;
+        return;
       }
-      store(sV + (t & 1) * L::kTile, vc, vz);
-      if (t + 1 < n_tiles) request_v(t + 1);
+      store(sV + S * L::kTile, vc[S], vz, v);
+      request_v(t + 2, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[t & 1]);
+      if (lane == 0) mbar_arrive(&v_full[S]);
+    };
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    request_k(0, Even());
+    request_v(0, Even());
+    request_k(1, Odd());
+    request_v(1, Odd());
+    for (int t = 0; ok && t < n_tiles; t += 2) {
+      unpack(t, Even());
+      if (ok && t + 1 < n_tiles) unpack(t + 1, Odd());
     }
   } else if (warp == kIssue) {
     // ---------------- products ----------------
@@ -365,54 +390,50 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     const uint32_t taddr = tmem + tile * L::kCols + ((uint32_t)(quarter * 32) << 16);
     const int all_see = a.mode == RD_ATTN_CAUSAL ? min(kv_end, r.base + first_token + 1) : min(kv_end, r.base);
     float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
-    // One tile's weights (packed, 32 words) at the maximum m; returns their sum and the tile's largest score.
-    auto weigh = [&](auto whole, int t, uint64_t vis, float m, uint32_t* w, float& mx) {
+    // A tile's weights (packed, 32 words) at the maximum m, scores in units of u; returns their sum.  odd: keys whose values are NaN.
+    auto weigh = [&](auto whole, int t, uint64_t vis, uint64_t odd, float m, float u, uint32_t* w) {
       constexpr bool WHOLE = decltype(whole)::value;
-      const uint32_t ks = rd_umma::smem_u32(k_scale + (t & 3) * kManyKeys), vs = rd_umma::smem_u32(v_scale + (t & 3) * kManyKeys);
-      const float off = m == -INFINITY ? 0.f : -m;
-      const F2 unit2 = pack2(unit, unit), off2 = pack2(off, off);
+      const float off = m == -INFINITY ? 0.f : kWeightBits - m;
+      const F2 unit2 = pack2(u, u), off2 = pack2(off, off);
       F2 sum = 0;
-      float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         float s[32];
         rd_umma::tmem_ld32(taddr + L::kColS + (t & 1) * 64 + 32 * hf, s);
-        const uint32_t v = (uint32_t)(vis >> (32 * hf));
+        const uint32_t v = (uint32_t)(vis >> (32 * hf)), o = (uint32_t)(odd >> (32 * hf));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          F2 k[2], f[2];
-          lds_pairs(ks + 128 * hf + 16 * i, k[0], k[1]);
-          lds_pairs(vs + 128 * hf + 16 * i, f[0], f[1]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int n = 4 * i + 2 * e;
-            F2 x = mul2(pack2(s[n], s[n + 1]), k[e]);
-            float x0, x1;
-            unpack2(x, x0, x1);
-            if (!WHOLE) {
-              if (!((v >> n) & 1)) x0 = -INFINITY;
-              if (!((v >> (n + 1)) & 1)) x1 = -INFINITY;
-              x = pack2(x0, x1);
-            }
-            part[2 * e] = fmaxf(part[2 * e], x0);
-            part[2 * e + 1] = fmaxf(part[2 * e + 1], x1);
-            unpack2(fma2(x, unit2, off2), x0, x1);
-            x0 = ex2(x0), x1 = ex2(x1);
-            const F2 p = pack2(x0, x1);
-            sum = add2(sum, p);
-            unpack2(mul2(p, f[e]), x0, x1);
-            if (!WHOLE) {  // a hidden value counts for nothing, NaN or not
-              if (!((v >> n) & 1)) x0 = 0.f;
-              if (!((v >> (n + 1)) & 1)) x1 = 0.f;
-            }
-            w[16 * hf + 2 * i + e] = pack_f16(x0, x1);
+        for (int i = 0; i < 32; i += 2) {
+          float x0, x1;
+          unpack2(fma2(pack2(s[i], s[i + 1]), unit2, off2), x0, x1);
+          x0 = ex2(x0), x1 = ex2(x1);
+          if (!WHOLE) {
+            if (!((v >> i) & 1)) x0 = 0.f;
+            if (!((v >> (i + 1)) & 1)) x1 = 0.f;
           }
+          sum = add2(sum, pack2(x0, x1));
+          if (!WHOLE) {
+            if ((v & o) >> i & 1) x0 = __int_as_float(0x7fffffff);
+            if ((v & o) >> (i + 1) & 1) x1 = __int_as_float(0x7fffffff);
+          }
+          w[16 * hf + i / 2] = pack_f16(x0, x1);
         }
       }
-      mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       float s0, s1;
       unpack2(sum, s0, s1);
       return s0 + s1;
+    };
+    // the largest score that a row sees
+    auto largest = [&](int t, uint64_t vis) {
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[16];
+        tmem_ld16(taddr + L::kColS + (t & 1) * 64 + 16 * c, x);
+        const uint32_t v = (uint32_t)(vis >> (16 * c));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, (v >> i) & 1 ? __uint_as_float(x[i]) : -INFINITY);
+      }
+      return top;
     };
     for (int t = 0; t < n_tiles; ++t) {
       if (!warp_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !warp_wait_or(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
@@ -440,24 +461,27 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
         if (n_in < 64) vis &= (1ull << max(n_in, 0)) - 1ull;
         if (!live) vis = 0;
       }
-      const float ref_t = refs[t & 3];
+      const float ref_t = v_ref[t & 3], u = unit * k_ref[t & 3];
+      const uint64_t odd = *reinterpret_cast<const uint64_t*>(v_nan + (t & 3) * 2);
       float keep = ref_t != ref && t > 0 ? ref / ref_t : 1.f;  // what O is to be multiplied with
       ref = ref_t;
       uint32_t w[32];
-      float sum;
-      for (;;) {
-        float mx;
-        sum = whole ? weigh(std::true_type(), t, vis, m_run, w, mx) : weigh(std::false_type(), t, vis, m_run, w, mx);
-        const float mx2 = mx * unit;
-        const bool moved = mx2 > m_run + kManySlack;  // also for the first visible key
-        if (!__any_sync(0xffffffffu, moved)) break;
-        // again, at the tile's own maximum: not a second time
-        if (moved) {
-          const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - mx2);
-          l_run *= alpha;
-          if (m_run != -INFINITY) keep *= alpha;
-          m_run = mx2;
+      float sum = 0.f;
+      bool low = m_run == -INFINITY;  // the first keys that the row sees
+#pragma unroll 1
+      for (int again = 0; again < 2; ++again) {
+        if (__any_sync(0xffffffffu, low)) {
+          const float top = largest(t, vis) * u;
+          if (low && top > m_run) {
+            const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - top);
+            l_run *= alpha;
+            if (m_run != -INFINITY) keep *= alpha;
+            m_run = top;
+          }
         }
+        sum = whole && odd == 0 ? weigh(std::true_type(), t, vis, odd, m_run, u, w) : weigh(std::false_type(), t, vis, odd, m_run, u, w);
+        low = sum > kMostWeights;  // at the tile's own maximum 64 weights come to 2^13 at most
+        if (!__any_sync(0xffffffffu, low)) break;
       }
       l_run += sum;
       if (__any_sync(0xffffffffu, t > 0 && keep != 1.f)) {
@@ -491,7 +515,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       rd_umma::fence_after();
       const int64_t at = (int64_t)(r.start + token) * a.nh + hk * group + (live ? R % group : 0);
       float* to = partial + (at * n_split + split) * (HD + 2);
-      const float f = n_split > 1 ? ref * 0x1p-8f : (l_run == 0.f ? 0.f : ref * 0x1p-8f / l_run);
+      const float f = n_split > 1 ? ref : (l_run == 0.f ? 0.f : ref / l_run);  // the weights' 2^7 is in O and in l
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         float x[32], y[32];

@@ -76,10 +76,12 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
     """(out, bound): attention in 64 bits over the values that the codes stand for, [tokens, heads * dim], and how far a kernel may be off
     whose softmax weights are rounded by at most weight_step (relative) beside what fp32 sums of scores cost; a row that sees nothing is 0.
 
-    Weights in fp16 have a smallest step besides, which counts where a feature's large weights all meet values of 0.  A weight is p s / r
-    2^8 (2^14 in the kernel for few rows), s the value's scale, r a power of two (the scale) that is no more than the largest scale R of the keys;
-    the largest p is at least 1 and the sum l that the result is divided by too.  Half of fp16's smallest step is 2^-25, so a key adds at
-    most 2^-25 2^-8 r (code - zero) / l <= 2^-33 R (2^bits - 1).
+    Weights in fp16 have a smallest step besides, which counts where a feature's large weights all meet values of 0.  In the kernel for few rows a weight
+    is p s / r 2^14, s the value's scale, r the largest scale R of the keys; the largest p is at least 1 and the sum l that the result is divided
+    by too.  Half of fp16's smallest step is 2^-25, so a key adds at most 2^-25 2^-14 r (code - zero) / l <= 2^-39 R (2^bits - 1).
+
+    The kernel for many rows rounds keys and values, scales and all, to fp16: 2^-12 of each, so a score is off by 2^-12 sum |q k| scale.  Its
+    weights are 2^7 p, of values s / r 2^6 (code - zero) or more: a key adds 2^-25 2^-7 R (2^bits - 1), a value's own smallest step 2^-31 R.
 
     The kernel for few rows sums W code and W zero apart, in fp32, and takes one from the other, which shows where values cancel or are 0.  A
     product of 16 keys adds to a sum of at most (2^bits - 1) R times the weights' share; a tensor core's addition may cut 2^-23 of that, the sum
@@ -114,10 +116,12 @@ def attention(cache, layer, q, row_start, kv_begin, base_len, mode, tree_mask, s
                 # Sums in fp32 of hd products of a query and a code (up to `top`) and of zero * sum q: hd + 4 roundings of 2^-23 (the tensor
                 # core cuts) of their absolute sum; one 2^-22 for the scaling and e^x's argument, relative to the score.
                 err = (hd + 4) * 2.0 ** -23 * np.abs(x).sum() * 2 * top * ks[b, g, seen].max() * abs(scale) + 2.0 ** -22 * np.abs(sc).max()
+                if weight_step > 2.0 ** -12:
+                    err += 2.0 ** -12 * (np.abs(k[b, g, seen]) @ np.abs(x)).max() * abs(scale)
                 weight = weight_step + exp_step + 2 * err + seen.size * 2.0 ** -23
                 bound[s + i, h] = weight * (p @ np.abs(v[b, g, seen])) + weight * np.abs(out[s + i, h])
                 if weight_step > 2.0 ** -12:
-                    bound[s + i, h] += (seen.size * 2.0 ** -33 + (seen.size / 128 + 2) * 2.0 ** -22) * vs[b, g, seen].max() * top
+                    bound[s + i, h] += (seen.size * 2.0 ** -32 + (seen.size / 128 + 2) * 2.0 ** -22) * vs[b, g, seen].max() * top
     return out.reshape(m, -1), bound.reshape(m, -1)
 
 
