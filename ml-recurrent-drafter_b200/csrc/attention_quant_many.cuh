@@ -6,13 +6,13 @@
 //   4 QT warps  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), running
 //               maximum and sum, weights W = 2^7 p as fp16 to TMEM;
 //   4 warps     unpacking: codes minus their zeros (exact: 1024 + code is one masking instruction, minus 1024 + zero) times their scales
-//               over a power of two, fp16, into swizzled shared-memory tiles of 64 keys, two stages each for K and V.  For keys that power
+//               over a power of two, fp16, into swizzled shared-memory tiles of 64 keys, two or four stages each for K and V.  For keys that power
 //               is of the tile and goes into the scores' unit; for values it is r, that of the largest scale so far;
-//   1 warp      issues S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
+//   QT warps    issue S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
 // Keys, values and weights are thus rounded to fp16's 11 bits, each by at most 2^-12 of itself, an eighth of what a bf16 cache costs.  With the
 // scales left to the softmax instead (codes alone are exact) its 64 x 128 scores cost four instructions for two where they now take
 // two and a half, which bounded the kernel: a tile of 256 rows 2560 cycles.
-// S has two buffers, W of a tile takes the place of its S: QK of the next tile runs under the softmax of this one.  A tile is read from TMEM once,
+// S has two buffers, W of a tile takes the place of its S: QK of the next two tiles run under the softmax of this one.  A tile is read from TMEM once,
 // 32 scores at a time, and weighted by the maximum so far; only where the sum of the weights turns out too large the tile's maximum is
 // looked for and the tile weighted again.
 // Features lie in the order in which the masks deliver them (within 8 of 4 bits: 0 4 1 5 2 6 3 7, within 4 of 8 bits: 0 2 1 3); the queries
@@ -28,10 +28,12 @@ constexpr float kMostWeights = 32768.f;   // of a tile of a row: none is more, a
 
 template <int HD, int QT>
 struct Many {
-  static constexpr int kThreads = (4 * QT + 5) * 32;
+  static constexpr int kThreads = (5 * QT + 4) * 32;
+  static constexpr int kStages = QT == 1 ? 2 : 4;  // of unpacked keys, and of values
   static constexpr int kQ = kManyRows * HD * 2, kTile = kManyKeys * HD * 2;  // bytes
-  static constexpr int kVectors = 4 * 4 * 4;                                // of four tiles: r, the keys' power of two, which values are NaN
-  static constexpr int kBytes = 1024 + QT * kQ + 4 * kTile + kVectors + QT * kManyRows * 4 + 32 * 8;
+  static constexpr int kBars = 256;
+  static constexpr int kVectors = 8 * 4 * 4;                                // of eight tiles: r, the keys' power of two, which values are NaN
+  static constexpr int kBytes = 1024 + QT * kQ + 2 * kStages * kTile + kVectors + QT * kManyRows * 4 + kBars;
   // TMEM of a tile of rows: two buffers of 64 columns for S, then W; O
   static constexpr uint32_t kColS = 0, kColO = 128, kCols = 128 + HD;
   static constexpr uint32_t kTmem = QT * kCols <= 256 ? 256 : 512;
@@ -81,13 +83,24 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+// Sixteen columns of this thread's lane; there only after tmem_have16() of the same registers, which waits for all loads before it.
+__device__ __forceinline__ void tmem_ask16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
         "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_have16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  tmem_ask16(taddr, r);
+  tmem_have16(r);
 }
 // complete only after a wait::st
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -134,20 +147,21 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;
   uint8_t* sK = smem + QT * L::kQ;
-  uint8_t* sV = sK + 2 * L::kTile;
-  float* v_ref = reinterpret_cast<float*>(sV + 2 * L::kTile);          // [4]: what values are multiples of
-  float* k_ref = v_ref + 4;                                            // [4]: and keys
-  uint32_t* v_nan = reinterpret_cast<uint32_t*>(k_ref + 4);            // [4][2]: keys whose values are NaN
-  float* units = reinterpret_cast<float*>(v_nan + 8);                  // [QT][128]
+  constexpr int kSt = L::kStages;
+  uint8_t* sV = sK + kSt * L::kTile;
+  // entries of eight tiles: what their values are multiples of, and their keys; which of their values are NaN.  The place of a tile's is
+  // written again when the softmax is done with it.
+  float* entries = reinterpret_cast<float*>(sV + kSt * L::kTile);  // [8][4]
+  float* units = entries + 32;                                     // [QT][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(units + QT * kManyRows);
-  uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7;
-  uint64_t* scales_full = bars + 9;       // [4]: a tile's entries are there; their place is written again only when the softmax is done with it
-  uint64_t* s_full = bars + 13;           // [QT][2]
+  uint64_t *k_full = bars, *v_full = k_full + kSt, *k_empty = v_full + kSt, *v_empty = k_empty + kSt;
+  uint64_t* q_full = v_empty + kSt;       // [QT]
+  uint64_t* s_full = q_full + QT;         // [QT][2]
   uint64_t* p_full = s_full + 2 * QT;     // [QT][2]
   uint64_t* o_full = p_full + 2 * QT;     // [QT][2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2 * QT);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(13 + 6 * 2 + 1 <= 32, "barriers");
+  static_assert((4 * kSt + 7 * QT) * 8 + 8 <= L::kBars, "barriers");
 
   const int group = a.nh / a.nkv;
   // in causal calls later tiles see more keys: they start first
@@ -169,16 +183,15 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
   const int per_split = (all_tiles + n_split - 1) / n_split;
   const int t_begin = split * per_split, n_tiles = max(0, min(per_split, all_tiles - t_begin));
   if (threadIdx.x == 0) {
-    rd_umma::mbar_init(q_full, 4 * n_q);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < QT; ++s) rd_umma::mbar_init(&q_full[s], 4);
+    for (int s = 0; s < kSt; ++s) {
       rd_umma::mbar_init(&k_full[s], 4);
       rd_umma::mbar_init(&v_full[s], 4);
-      rd_umma::mbar_init(&k_empty[s], 1);
-      rd_umma::mbar_init(&v_empty[s], 1);
+      rd_umma::mbar_init(&k_empty[s], n_q);
+      rd_umma::mbar_init(&v_empty[s], n_q);
     }
-    for (int s = 0; s < 4; ++s) rd_umma::mbar_init(&scales_full[s], 4);
     for (int s = 0; s < 2 * QT; ++s) {
-      rd_umma::mbar_init(&s_full[s], 1);
+      rd_umma::mbar_init(&s_full[s], 2);  // the product, and its issuer, who has seen the tile's entries
       rd_umma::mbar_init(&p_full[s], 4);
       rd_umma::mbar_init(&o_full[s], 1);
     }
@@ -245,38 +258,38 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     uint32_t top = 0;
     auto unpack = [&](int t, auto set) {
       constexpr int S = decltype(set)::value;
-      if (t >= 2 && !warp_wait_or(&k_empty[S], ((t - 2) >> 1) & 1, stop)) {
+      const int st = t % kSt;
+      if (t >= kSt && !warp_wait_or(&k_empty[st], (t / kSt - 1) & 1, stop)) {
         ok = false, site = 1;
         return;
       }
       const uint32_t k_top = largest(kp[S], kq[S]);
-      store(sK + S * L::kTile, kc[S], kp[S], param_scale(kp[S]) * __uint_as_float(((254 + kUp) << 23) - k_top));
+      store(sK + st * L::kTile, kc[S], kp[S], param_scale(kp[S]) * __uint_as_float(((254 + kUp) << 23) - k_top));
       top = max(top, largest(vp[S], vq[S]));
       float v = param_scale(vp[S]);
       const uint32_t nan = __ballot_sync(0xffffffffu, v != v);
       v = v != v ? 0.f : v * __uint_as_float(((254 + kUp) << 23) - top);
-      // QK of tile t - 2 is done: it was issued when the softmax was through with tile t - 4, whose place this is
+      // QK of tile t - kSt is done: it was issued when the softmax was through with tile t - kSt - 2, so that this place, tile t - 8's, is free
+      static_assert(kSt + 2 <= 8, "entries of eight tiles");
       if (half == 0 && lane == 0) {
-        v_nan[(t & 3) * 2 + (key >> 5)] = nan;
-        if (key == 0) v_ref[t & 3] = __uint_as_float(top - (kUp << 23)), k_ref[t & 3] = __uint_as_float(k_top - (kUp << 23));
+        float* e = entries + (t & 7) * 4;
+        e[2 + (key >> 5)] = __uint_as_float(nan);
+        if (key == 0) e[0] = __uint_as_float(top - (kUp << 23)), e[1] = __uint_as_float(k_top - (kUp << 23));
       }
       const uint32_t vz = vp[S];
       request_k(t + 2, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&scales_full[t & 3]);
-        mbar_arrive(&k_full[S]);
-      }
-      if (t >= 2 && !warp_wait_or(&v_empty[S], ((t - 2) >> 1) & 1, stop)) {
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      if (t >= kSt && !warp_wait_or(&v_empty[st], (t / kSt - 1) & 1, stop)) {
         ok = false, site = 2;
         return;
       }
-      store(sV + S * L::kTile, vc[S], vz, v);
+      store(sV + st * L::kTile, vc[S], vz, v);
       request_v(t + 2, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[S]);
+      if (lane == 0) mbar_arrive(&v_full[st]);
     };
     using Even = std::integral_constant<int, 0>;
     using Odd = std::integral_constant<int, 1>;
@@ -288,50 +301,41 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       unpack(t, Even());
       if (ok && t + 1 < n_tiles) unpack(t + 1, Odd());
     }
-  } else if (warp == kIssue) {
-    // ---------------- products ----------------
-    if (rd::elect_one()) {
+  } else if (warp >= kIssue) {
+    // ---------------- products: a warp for each tile of rows, so that neither waits for the other's softmax ----------------
+    const int x = warp - kIssue;
+    if (x < n_q && rd::elect_one()) {
       const uint32_t idesc_qk = idesc_fp16(kManyKeys, false), idesc_pv = idesc_fp16(HD, true);
-      auto issue_qk = [&](int t) {
-        const uint32_t k = rd_umma::smem_u32(sK + (t & 1) * L::kTile);
-        for (int x = 0; x < n_q; ++x) {
-          const uint32_t q = rd_umma::smem_u32(sQ + x * L::kQ);
+      const uint32_t q = rd_umma::smem_u32(sQ + x * L::kQ), base = tmem + x * L::kCols;
+      // S of tile t: its buffer held W of tile t - 2, whose product has been issued before; products run in that order
+      auto scores = [&](int t) {
+        const int st = t % kSt;
+        if (!mbar_wait_or(&k_full[st], (t / kSt) & 1, stop)) return false;
+        rd_umma::fence_after();
+        const uint32_t k = rd_umma::smem_u32(sK + st * L::kTile);
 #pragma unroll
-          for (int kd = 0; kd < HD / 16; ++kd)
-            rd_umma::mma_ss(tmem + x * L::kCols + L::kColS + (t & 1) * 64, rd_umma::desc_k_major(q + (kd >> 2) * (kManyRows * 128) + (kd & 3) * 32),
-                            rd_umma::desc_k_major(k + (kd >> 2) * (kManyKeys * 128) + (kd & 3) * 32), idesc_qk, kd != 0);
-          rd_umma::commit(&s_full[2 * x + (t & 1)]);
-        }
-        rd_umma::commit(&k_empty[t & 1]);
+        for (int kd = 0; kd < HD / 16; ++kd)
+          rd_umma::mma_ss(base + L::kColS + (t & 1) * 64, rd_umma::desc_k_major(q + (kd >> 2) * (kManyRows * 128) + (kd & 3) * 32),
+                          rd_umma::desc_k_major(k + (kd >> 2) * (kManyKeys * 128) + (kd & 3) * 32), idesc_qk, kd != 0);
+        mbar_arrive(&s_full[2 * x + (t & 1)]);
+        rd_umma::commit(&s_full[2 * x + (t & 1)]);
+        rd_umma::commit(&k_empty[st]);
+        return true;
       };
-      ok = mbar_wait_or(q_full, 0, stop);
-      if (ok && n_tiles > 0) {
-        ok = mbar_wait_or(&k_full[0], 0, stop);
-        if (ok) {
-          rd_umma::fence_after();
-          issue_qk(0);
-        }
-      }
+      ok = mbar_wait_or(&q_full[x], 0, stop);
+      for (int t = 0; ok && t < 2 && t < n_tiles; ++t) ok = scores(t);
       for (int t = 0; ok && t < n_tiles; ++t) {
-        if (t + 1 < n_tiles) {
-          // its buffer held W of tile t - 1, whose product has been issued before: products run in that order
-          ok = mbar_wait_or(&k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, stop);
-          if (!ok) break;
-          rd_umma::fence_after();
-          issue_qk(t + 1);
-        }
-        for (int x = 0; ok && x < n_q; ++x) {
-          ok = mbar_wait_or(&p_full[2 * x + (t & 1)], (t >> 1) & 1, stop) && (x > 0 || mbar_wait_or(&v_full[t & 1], (t >> 1) & 1, stop));
-          if (!ok) break;
-          rd_umma::fence_after();
-          const uint32_t v = rd_umma::smem_u32(sV + (t & 1) * L::kTile);
+        const int st = t % kSt;
+        ok = mbar_wait_or(&p_full[2 * x + (t & 1)], (t >> 1) & 1, stop) && mbar_wait_or(&v_full[st], (t / kSt) & 1, stop);
+        if (!ok) break;
+        rd_umma::fence_after();
+        const uint32_t v = rd_umma::smem_u32(sV + st * L::kTile);
 #pragma unroll
-          for (int ks = 0; ks < kManyKeys / 16; ++ks)
-            mma_ts(tmem + x * L::kCols + L::kColO, tmem + x * L::kCols + L::kColS + (t & 1) * 64 + ks * 8, rd_umma::desc_mn_major(v + ks * 2048, kManyKeys * 128),
-                   idesc_pv, (t | ks) != 0);
-          rd_umma::commit(&o_full[2 * x + (t & 1)]);
-        }
-        if (ok) rd_umma::commit(&v_empty[t & 1]);
+        for (int ks = 0; ks < kManyKeys / 16; ++ks)
+          mma_ts(base + L::kColO, base + L::kColS + (t & 1) * 64 + ks * 8, rd_umma::desc_mn_major(v + ks * 2048, kManyKeys * 128), idesc_pv, (t | ks) != 0);
+        rd_umma::commit(&o_full[2 * x + (t & 1)]);
+        rd_umma::commit(&v_empty[st]);
+        if (t + 2 < n_tiles) ok = scores(t + 2);
       }
       if (!ok) site = 3;
     }
@@ -342,45 +346,52 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     // ---------------- queries: eight lanes a row ----------------
     {
       const int part = lane & 7;
-      constexpr int kPart = HD / 8;  // features of a lane: 8 or 16
-#pragma unroll 2
-      for (int i = 0; i < 8; ++i) {
-        const int row = quarter * 32 + i * 4 + (lane >> 3), R = q0 + tile * kManyRows + row;
-        const bool live = R < rows;
-        const __nv_bfloat16* src =
-            (const __nv_bfloat16*)a.q + (int64_t)(r.start + (live ? R / group : 0)) * a.ldq + (hk * group + (live ? R % group : 0)) * HD + part * kPart;
-        float x[kPart];
+      constexpr int kPart = HD / 8, kAtOnce = 8;  // features of a lane: 8 or 16; rows
+#pragma unroll 1
+      for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
+        uint4 u[kAtOnce][kPart / 8];  // asked for before the first is looked at
 #pragma unroll
-        for (int c = 0; c < kPart / 8; ++c) {
-          const uint4 u = live ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int R = q0 + tile * kManyRows + quarter * 32 + (i0 + i) * 4 + (lane >> 3);
+          const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)(r.start + R / group) * a.ldq + (hk * group + R % group) * HD + part * kPart);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[8 * c + 2 * e] = __uint_as_float(w[e] << 16), x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          for (int c = 0; c < kPart / 8; ++c) u[i][c] = R < rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
         }
-        float most = 0.f;
 #pragma unroll
-        for (int e = 0; e < kPart; ++e) most = fmaxf(most, fabsf(x[e]));
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int row = quarter * 32 + (i0 + i) * 4 + (lane >> 3);
+          float x[kPart];
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // the row's largest to [2^14, 2^15): see the few-rows kernel
-        const int e2 = most > 0.f && most < INFINITY ? (int)(__float_as_uint(most) >> 23) : 141;
-        const int up = 141 - e2, h1 = up / 2, h2 = up - h1;
-        const float f1 = __uint_as_float((uint32_t)(127 + h1) << 23), f2 = __uint_as_float((uint32_t)(127 + h2) << 23);
+          for (int c = 0; c < kPart / 8; ++c) {
+            const uint32_t w[4] = {u[i][c].x, u[i][c].y, u[i][c].z, u[i][c].w};
 #pragma unroll
-        for (int c = 0; c < kPart / 8; ++c) {
-          float y[8];
+            for (int e = 0; e < 4; ++e) x[8 * c + 2 * e] = __uint_as_float(w[e] << 16), x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+          float most = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[order8<BITS>(k)] = x[8 * c + k] * f1 * f2;
-          const int chunk = part * (kPart / 8) + c;
-          *reinterpret_cast<uint4*>(myQ + (chunk >> 3) * (kManyRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-              make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7]));
+          for (int e = 0; e < kPart; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          // the row's largest to [2^14, 2^15): see the few-rows kernel
+          const int e2 = most > 0.f && most < INFINITY ? (int)(__float_as_uint(most) >> 23) : 141;
+          const int up = 141 - e2, h1 = up / 2, h2 = up - h1;
+          const float f1 = __uint_as_float((uint32_t)(127 + h1) << 23), f2 = __uint_as_float((uint32_t)(127 + h2) << 23);
+#pragma unroll
+          for (int c = 0; c < kPart / 8; ++c) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[order8<BITS>(k)] = x[8 * c + k] * f1 * f2;
+            const int chunk = part * (kPart / 8) + c;
+            *reinterpret_cast<uint4*>(myQ + (chunk >> 3) * (kManyRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+                make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7]));
+          }
+          if (part == 0)
+            units[tile * kManyRows + row] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
         }
-        if (part == 0)
-          units[tile * kManyRows + row] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
       }
       rd_umma::fence_async_proxy();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (lane == 0) mbar_arrive(&q_full[tile]);
     }
     // ---------------- softmax: a thread a row ----------------
     const int row = quarter * 32 + lane, R = q0 + tile * kManyRows + row;
@@ -396,15 +407,20 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       const float off = m == -INFINITY ? 0.f : kWeightBits - m;
       const F2 unit2 = pack2(u, u), off2 = pack2(off, off);
       F2 sum = 0;
+      // sixteen scores are on their way while sixteen are weighted
+      uint32_t s[2][16];
+      const uint32_t from = taddr + L::kColS + (t & 1) * 64;
+      tmem_ask16(from, s[0]);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float s[32];
-        rd_umma::tmem_ld32(taddr + L::kColS + (t & 1) * 64 + 32 * hf, s);
-        const uint32_t v = (uint32_t)(vis >> (32 * hf)), o = (uint32_t)(odd >> (32 * hf));
+      for (int c = 0; c < 4; ++c) {
+        uint32_t* y = s[c & 1];
+        tmem_have16(y);
+        if (c < 3) tmem_ask16(from + 16 * (c + 1), s[(c + 1) & 1]);
+        const uint32_t v = (uint32_t)(vis >> (16 * c)), o = (uint32_t)(odd >> (16 * c));
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int i = 0; i < 16; i += 2) {
           float x0, x1;
-          unpack2(fma2(pack2(s[i], s[i + 1]), unit2, off2), x0, x1);
+          unpack2(fma2(pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), unit2, off2), x0, x1);
           x0 = ex2(x0), x1 = ex2(x1);
           if (!WHOLE) {
             if (!((v >> i) & 1)) x0 = 0.f;
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
             if ((v & o) >> i & 1) x0 = __int_as_float(0x7fffffff);
             if ((v & o) >> (i + 1) & 1) x1 = __int_as_float(0x7fffffff);
           }
-          w[16 * hf + i / 2] = pack_f16(x0, x1);
+          w[8 * c + i / 2] = pack_f16(x0, x1);
         }
       }
       float s0, s1;
@@ -436,7 +452,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       return top;
     };
     for (int t = 0; t < n_tiles; ++t) {
-      if (!warp_wait_or(&scales_full[t & 3], (t >> 2) & 1, stop) || !warp_wait_or(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
+      if (!warp_wait_or(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
         ok = false, site = 4;
         break;
       }
@@ -461,31 +477,28 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
         if (n_in < 64) vis &= (1ull << max(n_in, 0)) - 1ull;
         if (!live) vis = 0;
       }
-      const float ref_t = v_ref[t & 3], u = unit * k_ref[t & 3];
-      const uint64_t odd = *reinterpret_cast<const uint64_t*>(v_nan + (t & 3) * 2);
-      float keep = ref_t != ref && t > 0 ? ref / ref_t : 1.f;  // what O is to be multiplied with
-      ref = ref_t;
+      const float4 entry = *reinterpret_cast<const float4*>(entries + (t & 7) * 4);
+      const float ref_t = entry.x, u = unit * entry.y;
+      const uint64_t odd = (uint64_t)__float_as_uint(entry.z) | (uint64_t)__float_as_uint(entry.w) << 32;
       uint32_t w[32];
-      float sum = 0.f;
-      bool low = m_run == -INFINITY;  // the first keys that the row sees
+      float sum;
 #pragma unroll 1
-      for (int again = 0; again < 2; ++again) {
-        if (__any_sync(0xffffffffu, low)) {
-          const float top = largest(t, vis) * u;
-          if (low && top > m_run) {
-            const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - top);
-            l_run *= alpha;
-            if (m_run != -INFINITY) keep *= alpha;
-            m_run = top;
-          }
-        }
+      for (bool again = false;; again = true) {
         sum = whole && odd == 0 ? weigh(std::true_type(), t, vis, odd, m_run, u, w) : weigh(std::false_type(), t, vis, odd, m_run, u, w);
-        low = sum > kMostWeights;  // at the tile's own maximum 64 weights come to 2^13 at most
-        if (!__any_sync(0xffffffffu, low)) break;
-      }
-      l_run += sum;
-      if (__any_sync(0xffffffffu, t > 0 && keep != 1.f)) {
-        // O has to be quiet while it is brought to the new maximum or r
+        // seldom: the first keys that a row sees, weights too large, a larger r.  At the tile's own maximum 64 weights come to 2^13 at most.
+        const bool low = m_run == -INFINITY || sum > kMostWeights;
+        if (again || !__any_sync(0xffffffffu, low || ref_t != ref)) break;
+        const float top = largest(t, vis) * u;
+        float keep = ref / ref_t;  // what O is to be multiplied with
+        if (low && top > m_run) {
+          const float alpha = m_run == -INFINITY ? 0.f : ex2(m_run - top);
+          l_run *= alpha;
+          if (m_run != -INFINITY) keep *= alpha;
+          m_run = top;
+        }
+        ref = ref_t;
+        if (t == 0) continue;
+        // O has to be quiet
         if (!warp_wait_or(&o_full[2 * tile + ((t - 1) & 1)], ((t - 1) >> 1) & 1, stop)) {
           ok = false, site = 5;
           break;
@@ -500,6 +513,8 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
           tmem_st16(taddr + L::kColO + c * 16, x);
         }
       }
+      if (!ok) break;
+      l_run += sum;
       tmem_st16(taddr + L::kColS + (t & 1) * 64, w);
       tmem_st16(taddr + L::kColS + (t & 1) * 64 + 16, w + 16);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
