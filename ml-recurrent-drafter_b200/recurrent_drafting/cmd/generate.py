@@ -75,6 +75,8 @@ def define_flags() -> argparse.ArgumentParser:
     ap.add_argument("--rng_seed", type=int, default=123)
     ap.add_argument("--use_gpu", type=int, default=0)
     ap.add_argument("--dtype", default="bf16", choices=["fp32", "bf16"])
+    ap.add_argument("--cache_bits", type=int, default=None, choices=[4, 8], help="Llama: keys and values are cached in codes of so many bits.")
+    ap.add_argument("--int8_weights", action="store_true", help="Llama: projections in 8-bit integers.")
     ap.add_argument("--pad_token_id", type=int, default=0)
     ap.add_argument("--eos_token_id", type=int, default=-1, help="Negative: never stop early.")
     return ap
@@ -133,6 +135,12 @@ def load_models(args, device):
         llm.init_random(0.02, seed=args.rng_seed)
     else:
         llm = registry.load_model(args.hf_llm, torch_dtype=dtype, device=device)
+    if args.cache_bits is not None or args.int8_weights:
+        if not isinstance(llm, modeling_llama.LlamaForCausalLM):
+            raise SystemExit("--cache_bits and --int8_weights are for Llama models")
+        llm.hold_cache_in(args.cache_bits)
+        if args.int8_weights:
+            llm.hold_weights_in_int8()
     if args.hf_drafter is None:
         return llm, None
     if args.hf_drafter.startswith("random:"):

@@ -14,15 +14,15 @@ Two entry points share one token-major implementation:
 """
 import math
 import os
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 from torch import nn
 from transformers.modeling_outputs import CausalLMOutput
 
 from . import _lib, attention, checkpoint, kv_cache
+from .modeling_common import Int8Linear, LMHead
 from .modeling_common import Linear as _Linear
-from .modeling_common import LMHead
 
 
 def rope_tables(head_dim: int, n_pos: int, base: float, device) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -91,6 +91,9 @@ class LlamaForCausalLM(LMHead, nn.Module):
         self._attn_split_ws: Optional[torch.Tensor] = None
         self._head_ws: Optional[torch.Tensor] = None
         self.gemm_status: Optional[torch.Tensor] = None
+        self.cache_bits: Optional[int] = None  # of the caches that new_cache() makes; None: the model's type
+        self._int8: Optional[Dict[str, List[Int8Linear]]] = None
+        self._stage: Optional[Dict[str, torch.Tensor]] = None
 
     # ----------------------------------------------------------------- reference-compatible surface
     @property
@@ -111,15 +114,44 @@ class LlamaForCausalLM(LMHead, nn.Module):
         return self.dtype == torch.bfloat16 and self.head_dim == 128 and self.fused_head_ok()
 
     def held_buffers(self) -> List[torch.Tensor]:
-        return super().held_buffers() + [t for t in (self._attn_split_ws, *(self._rope or ())) if t is not None]
+        return super().held_buffers() + [t for t in (self._attn_split_ws, *(self._rope or ()), *(self._stage or {}).values()) if t is not None]
 
-    def new_cache(self, batch_size: int, max_length: int, draft_tokens: int = 0, device=None) -> kv_cache.Cache:
+    def hold_cache_in(self, bits: Optional[int]) -> "LlamaForCausalLM":
+        """The caches of later requests hold keys and values in codes of 8 or 4 bits (None: in the model's type again)."""
+        if bits not in (None, 4, 8):
+            raise _lib.RedrafterError(f"a cache is held in 4 or 8 bits, not in {bits}")
+        if bits is not None and (self.head_dim % 8 or self.head_dim > 256):
+            raise _lib.RedrafterError(f"heads of {self.head_dim} features: a cache in codes wants a multiple of 8 up to 256")
+        self.cache_bits = bits
+        return self
+
+    def hold_weights_in_int8(self) -> "LlamaForCausalLM":
+        """Replaces the projections of all layers by 8-bit integers with a scale for each output feature, and gives their memory back; at
+        each call the rows that they are applied to become 8-bit integers too.  Embedding, norms and the language-model head stay.  The weights
+        as they were are gone: the model can be neither saved nor moved afterwards, and load_state_dict() needs a new one."""
+        if self._int8 is None:
+            self._int8 = {}
+            self._linears = None
+            for name, weights in (("qkv", self.wqkv), ("o", self.wo), ("gu", self.wgu), ("down", self.wdown)):
+                self._int8[name] = []
+                for w in weights:
+                    self._int8[name].append(Int8Linear(w.detach()))
+                    w.data = torch.empty(0, dtype=w.dtype, device=w.device)
+            self._invalidate()
+        return self
+
+    def new_cache(self, batch_size: int, max_length: int, draft_tokens: int = 0, device=None) -> Union[kv_cache.Cache, kv_cache.QuantizedCache]:
         """A cache for batch_size rows of at most max_length tokens (packed draft tokens included)."""
+        if self.cache_bits is not None:
+            return kv_cache.QuantizedCache(batch_size, max_length, self.n_layers, self.n_kv_heads, self.head_dim, self.cache_bits,
+                                           self.device if device is None else device)
         return kv_cache.Cache(batch_size, max_length, self.n_layers, self.n_kv_heads, self.head_dim, self.dtype,
                               self.device if device is None else device)
 
     def commit_draft(self, cache, fp, n_accepted, seq_in_beam, beam_shape, kv_begin=None) -> None:
-        """The acceptance kernel itself moves the accepted rows of this model's cache: nothing is left to do."""
+        """The acceptance kernel itself moves the accepted rows of a plain cache: nothing is left to do.  Rows in codes are moved here."""
+        if isinstance(cache, kv_cache.QuantizedCache):
+            cache.commit_draft(fp, n_accepted, seq_in_beam, beam_shape, kv_begin)
 
     def get_input_embeddings(self):
         return self.model.embed_tokens
@@ -140,6 +172,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
 
     def load_state_dict(self, state_dict, strict: bool = True, assign: bool = False):
         """Accepts the HF / reference names and packs them into the kernel layouts."""
+        self._weights_as_they_were()
         sd = state_dict if isinstance(state_dict, checkpoint.LazyCheckpoint) else dict(state_dict)
         if any(k.startswith("wqkv.") for k in sd):
             out = super().load_state_dict(sd, strict=strict)
@@ -190,6 +223,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
 
     def reference_state_dict(self) -> Dict[str, torch.Tensor]:
         """The weights under the HF / reference names."""
+        self._weights_as_they_were()
         nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
         sd = {"model.embed_tokens.weight": self.model.embed_tokens.weight.detach().clone()}
         for l in range(self.n_layers):
@@ -206,7 +240,12 @@ class LlamaForCausalLM(LMHead, nn.Module):
         sd["lm_head.weight"] = self.lm_head.weight.detach().clone()
         return sd
 
+    def _weights_as_they_were(self) -> None:
+        if self._int8 is not None:
+            raise _lib.RedrafterError("the projections of this model are held in 8-bit integers: its weights cannot be loaded, saved or moved any more")
+
     def _apply(self, fn, *args, **kwargs):
+        self._weights_as_they_were()
         out = super()._apply(fn, *args, **kwargs)
         self._invalidate()
         return out
@@ -218,6 +257,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
         self._ws_cap = (0, 0)
         self._rope = None
         self._head_ws = None
+        self._stage = None
         self._drop_attn_plans()
 
     def _drop_attn_plans(self):
@@ -275,7 +315,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
     # ----------------------------------------------------------------- kernels
     def _lin(self):
         if self._linears is None:
-            self._linears = {
+            self._linears = dict(self._int8, head=_Linear(self.lm_head.weight)) if self._int8 is not None else {
                 "qkv": [_Linear(w) for w in self.wqkv],
                 "o": [_Linear(w) for w in self.wo],
                 "gu": [_Linear(w) for w in self.wgu],
@@ -308,7 +348,8 @@ class LlamaForCausalLM(LMHead, nn.Module):
                                 ("act", self.config.intermediate_size), ("hidden", H)):
                 full[name] = torch.empty(cap_m, width, dtype=dt, device=dev)
             # shares of the projections with a residual
-            most = max((lin.shares_bytes(min(cap_m, _Linear.MAX_SHARE_ROWS)) for lin in self._lin()["o"] + self._lin()["down"]), default=0)
+            most = max((lin.shares_bytes(min(cap_m, _Linear.MAX_SHARE_ROWS)) for lin in self._lin()["o"] + self._lin()["down"]
+                        if isinstance(lin, _Linear)), default=0)
             full["parts"] = torch.empty(most // 4, dtype=torch.float32, device=dev)
             # folded RMS norm: per-token sums of squares by 128-feature slice
             full["ss"] = torch.empty(cap_m, ((H + 127) // 128 + 3) // 4 * 4, dtype=torch.float32, device=dev)
@@ -333,17 +374,38 @@ class LlamaForCausalLM(LMHead, nn.Module):
                     lin.drop_plans()
         self._drop_attn_plans()
 
-    def backbone(self, ws, cache_tensor: torch.Tensor, m_max: int, m_dev, tok_ids, tok_row, tok_pos, tok_slot, row_start,
+    def _stage_of(self, m_max: int) -> Dict[str, torch.Tensor]:
+        """Where the keys and values of m_max new tokens lie between their projection and a cache in codes: [1, heads, m_max, head_dim] each, token t
+        at slot t of row 0."""
+        st = self._stage
+        if st is None or st["slot"].shape[0] != m_max:
+            kv = dict(dtype=self.dtype, device=self.device)
+            st = self._stage = {
+                "k": torch.empty(1, self.n_kv_heads, m_max, self.head_dim, **kv), "v": torch.empty(1, self.n_kv_heads, m_max, self.head_dim, **kv),
+                "row": torch.zeros(m_max, dtype=torch.int32, device=self.device),
+                "slot": torch.arange(m_max, dtype=torch.int32, device=self.device),
+            }
+        return st
+
+    def backbone(self, ws, cache_tensor: Union[torch.Tensor, kv_cache.QuantizedCache], m_max: int, m_dev, tok_ids, tok_row, tok_pos, tok_slot, row_start,
                  kv_begin, base_len, batch: int, max_new: int, max_kv: int, mode: int, tree_mask=None, mask_words: int = 0,
                  dense_mask=None, n_pos: int = 4096) -> torch.Tensor:
         """Embedding + all decoder layers + final norm over m_max (or *m_dev) packed tokens.
-        K/V of the tokens are written into cache_tensor [NL,2,B,nkv,max_len,hd].  Returns the
+        K/V of the tokens are written into cache_tensor [NL,2,B,nkv,max_len,hd], or quantised into a cache in codes.  Returns the
         post-norm hidden states ws["hidden"] (modeling_llama.py:207-237)."""
         code = _lib.dtype_code(self.dtype)
         lin = self._lin()
         H = self.config.hidden_size
         nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
-        max_len = cache_tensor.shape[4]
+        codes = cache_tensor if isinstance(cache_tensor, kv_cache.QuantizedCache) else None
+        if codes is not None:
+            if mode == _lib.ATTN_DENSE:
+                raise _lib.RedrafterError("a cache in codes is attended to causally or through a prefix tree, not through an explicit mask")
+            stage = self._stage_of(m_max)
+            row_of, slot_of, max_len = stage["row"], stage["slot"], m_max
+        else:
+            row_of, slot_of, max_len = tok_row, tok_slot, cache_tensor.shape[4]
+        int8 = self._int8 is not None
         cos, sin = self._rope_tables(n_pos)
         st = _lib.stream()
         md = _lib.ptr(m_dev)
@@ -358,7 +420,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
             # batch has one query, because torch calls a tensor contiguous whatever the stride of a dimension of size 1.
             dense_bits = torch.empty(m_max, (max_kv + 63) // 64, dtype=torch.int64, device=h.device)
             _lib.call("rd_mask_bits", _lib.ptr(dense_mask), max_kv, m_max, max_kv, _lib.ptr(dense_bits), dense_bits.shape[1], st)
-        fused_rope = (self.dtype == torch.bfloat16 and hd == 128 and H % 64 == 0 and xn.data_ptr() % 16 == 0
+        fused_rope = (not int8 and self.dtype == torch.bfloat16 and hd == 128 and H % 64 == 0 and xn.data_ptr() % 16 == 0
                       and os.environ.get("RD_FUSED_ROPE", "1") != "0")
         # RMS norms between the projections folded into them (RD_FUSED_NORM=1): o_proj / down_proj also write the
         # gamma-scaled row and its sums of squares, gate/up and the next layer's QKV apply 1 / rms in their epilogues;
@@ -377,25 +439,33 @@ class LlamaForCausalLM(LMHead, nn.Module):
                           _lib.ptr(weight), _lib.ptr(y), m_max, md, H, self.eps, st)
 
         def add_residual(lin_l, a):
+            if int8:
+                lin_l(a, h, _lib.EPI_RES, residual=h, m_dev=m_dev, m_max=m_max, status=self.gemm_status)
+                return None
             return lin_l.add_residual(a, h, h, m_dev, m_max, self.gemm_status, parts, early=True)
 
         # `early`: everything below follows the embedding kernel, and nothing in it writes a weight
+        early = {} if int8 else {"early": True}
         pending = None
         for l in range(self.n_layers):
             if not fused_norm or l == 0:
                 norm(self.ln1[l], xn, pending)
-            kc, vc = cache_tensor[l, 0], cache_tensor[l, 1]
+            kc, vc = (stage["k"], stage["v"]) if codes is not None else (cache_tensor[l, 0], cache_tensor[l, 1])
             if fused_rope:
                 # rotary embedding and the cache append ride on the projection's epilogue
-                lin["qkv"][l].qkv_rope(xn, q, kc, vc, tok_row, tok_pos, tok_slot, cos, sin, nh, nkv, hd, m_dev, m_max,
+                lin["qkv"][l].qkv_rope(xn, q, kc, vc, row_of, tok_pos, slot_of, cos, sin, nh, nkv, hd, m_dev, m_max,
                                        self.gemm_status, norm=(ss, H, self.eps) if fused_norm and l > 0 else None, early=True)
             else:
-                lin["qkv"][l](xn, qkv, _lib.EPI_NONE, m_dev=m_dev, m_max=m_max, status=self.gemm_status, early=True)
-                _lib.call("rd_rope_kv_write", code, _lib.ptr(qkv), _lib.ptr(q), _lib.ptr(kc), _lib.ptr(vc), _lib.ptr(tok_row),
-                          _lib.ptr(tok_pos), _lib.ptr(tok_slot), _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], m_max, md, nh, nkv,
+                lin["qkv"][l](xn, qkv, _lib.EPI_NONE, m_dev=m_dev, m_max=m_max, status=self.gemm_status, **early)
+                _lib.call("rd_rope_kv_write", code, _lib.ptr(qkv), _lib.ptr(q), _lib.ptr(kc), _lib.ptr(vc), _lib.ptr(row_of),
+                          _lib.ptr(tok_pos), _lib.ptr(slot_of), _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], m_max, md, nh, nkv,
                           hd, max_len, st)
-            self._attention(code, q, kc, vc, attn, row_start, kv_begin, base_len, batch, m_max, max_new, max_kv, mode, tree_mask,
-                            mask_words, dense_mask, dld_q, dld_b, dense_bits, st)
+            if codes is not None:
+                codes.append(l, kc[0].transpose(0, 1), vc[0].transpose(0, 1), tok_row, tok_slot, m_dev)
+                codes.attend(l, q, attn, row_start, kv_begin, base_len, max_new, max_kv, mode, tree_mask, status=self.gemm_status)
+            else:
+                self._attention(code, q, kc, vc, attn, row_start, kv_begin, base_len, batch, m_max, max_new, max_kv, mode, tree_mask,
+                                mask_words, dense_mask, dld_q, dld_b, dense_bits, st)
             if fused_norm:
                 lin["o"][l].residual_with_norm(attn, h, h, self.ln2[l], xn, ss, m_dev, m_max, self.gemm_status)
                 lin["gu"][l].swiglu_normed(xn, act, ss, H, self.eps, m_dev, m_max, self.gemm_status)
@@ -406,7 +476,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
                 continue
             pending = add_residual(lin["o"][l], attn)
             norm(self.ln2[l], xn, pending)
-            lin["gu"][l](xn, act, _lib.EPI_SWIGLU, m_dev=m_dev, m_max=m_max, status=self.gemm_status, early=True)
+            lin["gu"][l](xn, act, _lib.EPI_SWIGLU, m_dev=m_dev, m_max=m_max, status=self.gemm_status, **early)
             pending = add_residual(lin["down"][l], act)
         norm(self.norm, ws["hidden"], pending)
         return ws["hidden"]
