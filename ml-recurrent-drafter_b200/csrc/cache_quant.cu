@@ -14,33 +14,55 @@ using namespace rd_quant;
 
 constexpr int kThreads = 256;
 
-// VEC consecutive values from a 16-byte boundary
-template <int VEC, typename T>
-__device__ __forceinline__ void load_values(const T* p, float* x) {
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int v = 0; v < VEC; v += 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + v);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[v + 2 * i] = __uint_as_float(w[i] << 16);
-        x[v + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < VEC; v += 4) *reinterpret_cast<float4*>(x + v) = *reinterpret_cast<const float4*>(p + v);
-  }
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
 }
 
-// One row by `lanes` lanes (a power of two), VEC features each; lanes past hd hold zeros, which change no range.
-template <int BITS, int VEC>
-__device__ __forceinline__ void quantise_row(const float* x, int lanes, bool mine, bool first, uint8_t* codes, uint32_t* param) {
+// A lane's VEC features of a row, as they lie
+template <typename T, int VEC>
+struct Piece {
+  static constexpr int kWords = VEC * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(p + i * 4 / sizeof(T));
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  // widens [low, high]; NaN stays
+  __device__ __forceinline__ void range(float& low, float& high) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) low = min_nan(low, value(i)), high = max_nan(high, value(i));
+    } else {
+      uint32_t l = 0, h = 0;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) l = min_nan2(l, w[i]), h = max_nan2(h, w[i]);
+      low = min_nan(low, min_nan(__uint_as_float(l << 16), __uint_as_float(l & 0xffff0000u)));
+      high = max_nan(high, max_nan(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)));
+    }
+  }
+};
+
+// One row by `lanes` lanes (a power of two); lanes past hd hold zeros, which change no range.
+template <int BITS, typename T, int VEC>
+__device__ __forceinline__ void quantise_row(const Piece<T, VEC>& x, int lanes, bool mine, bool first, uint8_t* codes, uint32_t* param) {
   constexpr int kQ = (1 << BITS) - 1;
   float low = 0.f, high = 0.f;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) low = min_nan(low, x[i]), high = max_nan(high, x[i]);
+  x.range(low, high);
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
     high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
@@ -50,17 +72,16 @@ __device__ __forceinline__ void quantise_row(const float* x, int lanes, bool min
   const __nv_bfloat16 s = __float2bfloat16_rn(range / (float)kQ);
   const float scale = __bfloat162float(s);
   const bool some = fine && scale > 0.f;
-  const Divider by(some ? scale : 1.f);
+  const Divider<sizeof(T) == 2> by(some ? scale : 1.f);
   const int zero = some ? min((int)(by.rint_bits(-low) - kRintBias), kQ) : 0;
   uint32_t w[VEC * BITS / 32];
 #pragma unroll
   for (int i = 0; i < VEC * BITS / 32; ++i) w[i] = 0;
   if (some) {
+    const int shift = zero - (int)kRintBias;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const uint32_t c = (uint32_t)__vimin_s32_relu((int)(by.rint_bits(x[i]) - kRintBias) + zero, kQ);
-      w[i * BITS / 32] |= c << (i * BITS % 32);
-    }
+    for (int i = 0; i < VEC; ++i)  // cut to 0 .. Q, added up by multiplications
+      w[i * BITS / 32] += (uint32_t)__vimin_s32_relu((int)by.rint_bits(x.value(i)) + shift, kQ) * (1u << (i * BITS % 32));
   }
   if (mine) {
     if constexpr (VEC * BITS == 32) *reinterpret_cast<uint32_t*>(codes) = w[0];
@@ -89,13 +110,13 @@ __global__ void __launch_bounds__(kThreads) cache_quant_append_kernel(const T* k
   const uint32_t t = live ? unit / (uint32_t)nkv : 0;
   const int head = live ? (int)(unit - t * nkv) : 0;
   const bool mine = live && d < hd;
-  float xk[VEC], xv[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) xk[i] = xv[i] = 0.f;
+  Piece<T, VEC> xk, xv;
+  xk.clear();
+  xv.clear();
   if (mine) {
     const int64_t from = (int64_t)t * tok_stride + head * head_stride + d;
-    load_values<VEC>(k + from, xk);
-    load_values<VEC>(v + from, xv);
+    xk.load(k + from);
+    xv.load(v + from);
   }
   int row = 0, slot = 0;
   if (live) {
@@ -105,8 +126,8 @@ __global__ void __launch_bounds__(kThreads) cache_quant_append_kernel(const T* k
   }
   const int64_t at = ((int64_t)row * nkv + head) * max_len + slot;  // row of the planes
   const int64_t byte = at * (hd * BITS / 8) + d * BITS / 8;
-  quantise_row<BITS, VEC>(xk, lanes, mine && live, live && part == 0, to.k_codes + byte, to.k_params + at);
-  quantise_row<BITS, VEC>(xv, lanes, mine && live, live && part == 0, to.v_codes + byte, to.v_params + at);
+  quantise_row<BITS>(xk, lanes, mine && live, live && part == 0, to.k_codes + byte, to.k_params + at);
+  quantise_row<BITS>(xv, lanes, mine && live, live && part == 0, to.v_codes + byte, to.v_params + at);
 }
 
 constexpr int kReadRows = 8;  // rows of a thread, all asked for before the first is written
@@ -158,9 +179,9 @@ __global__ void __launch_bounds__(kThreads) cache_quant_read_kernel(Planes from,
         __nv_bfloat162 h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        *reinterpret_cast<uint4*>(out + (int64_t)j * hd) = *reinterpret_cast<const uint4*>(h);
+        __stcs(reinterpret_cast<uint4*>(out + (int64_t)j * hd), *reinterpret_cast<const uint4*>(h));
       } else {
-        *reinterpret_cast<float4*>(out + (int64_t)j * hd) = *reinterpret_cast<const float4*>(x);
+        __stcs(reinterpret_cast<float4*>(out + (int64_t)j * hd), *reinterpret_cast<const float4*>(x));
       }
     }
   }

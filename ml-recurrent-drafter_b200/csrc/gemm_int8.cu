@@ -14,7 +14,8 @@ namespace {
 // codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows: these have blocks of 1024 threads.  VEC: rows on
 // 16-byte boundaries, K a multiple of 8.
 
-__device__ __forceinline__ uint32_t int8_code(float x, const rd_quant::Divider& by) {
+template <bool Bits8>
+__device__ __forceinline__ uint32_t int8_code(float x, const rd_quant::Divider<Bits8>& by) {
   return (uint32_t)min(max((int)(by.rint_bits(x) - rd_quant::kRintBias), -127), 127) & 0xffu;
 }
 template <typename T, bool VEC>
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const T* x, int64_t
   const bool fine = top <= 3.402823466e38f;  // not so for NaN either
   const float scale = __bfloat162float(__float2bfloat16_rn(top / 127.f));
   const bool some = fine && scale > 0.f;
-  const rd_quant::Divider by(some ? scale : 1.f);
+  const rd_quant::Divider<sizeof(T) == 2> by(some ? scale : 1.f);
   if (threadIdx.x == 0) scales[t] = fine ? scale : __int_as_float(0x7fffffff);
   auto put = [&](int i, const float* v) {
     uint2 w = make_uint2(0u, 0u);

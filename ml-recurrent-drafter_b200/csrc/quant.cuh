@@ -26,23 +26,25 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return y;
 }
 
-// rint(x / scale) for a scale of 8 significant bits and |x / scale| < 2^22, as the bits of 12582912 + it: subtract kRintBias for the integer.
-// q = x r is within two units of the quotient; what is left, x - q scale, has few bits and is exact, so the second step gives the
-// quotient rounded once but for an error of 2^-46: quotients half way between two integers come out exactly, and others are
-// further from half way than half a unit (cache_quant.cu), by 2^-9 of it at least.  Three instructions of the full rate; the compiler's
-// division takes some ten and was what the quantising kernels spent their time on (20235 tokens of 8 heads, 63 us).
+// rint(x / scale) for a scale of 8 significant bits and |x / scale| < 2^22 (256 for Bits8), as the bits of 12582912 + it: subtract kRintBias for
+// the integer.
+// x of up to 24 bits: q = x r is within two units of the quotient; what is left, x - q scale, has few bits and is exact, so the second step
+// gives the quotient rounded once but for an error of 2^-46: quotients half way between two integers come out exactly, and others are
+// further from half way than half a unit (cache_quant.cu), by 2^-9 of it at least.
+// x of 8 bits (Bits8): a quotient that is not half way is 2^-9 or more away from there, for then 2 x - (2 k + 1) scale is at least the last place of
+// the scale; x r is off by 2^-15 at most, and rounded to a multiple of 2^-10, which adding 1.5 2^13 does, it is half way where the quotient is.
+// The compiler's division takes some ten instructions and was what the quantising kernels spent their time on (20235 tokens of 8
+// heads: 63 us, 40 with four, now two for bf16).
+template <bool Bits8>
 struct Divider {
   float scale, inverse;
   bool fast;  // neither the inverse nor what is left leaves fp32's normal range
   __device__ __forceinline__ explicit Divider(float s) : scale(s), inverse(1.f / s), fast(s >= 0x1p-100f && s <= 0x1p100f) {}
   __device__ __forceinline__ uint32_t rint_bits(float x) const {
-    float q;
-    if (fast) {
-      q = x * inverse;
-      q = fmaf(fmaf(-q, scale, x), inverse, q);
-    } else {
-      q = x / scale;
-    }
+    if (!fast) return __float_as_uint(x / scale + 12582912.f);
+    if constexpr (Bits8) return __float_as_uint(fmaf(x, inverse, 12288.f) + (12582912.f - 12288.f));
+    float q = x * inverse;
+    q = fmaf(fmaf(-q, scale, x), inverse, q);
     return __float_as_uint(q + 12582912.f);
   }
 };
