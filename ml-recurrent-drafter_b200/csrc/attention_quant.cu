@@ -200,8 +200,8 @@ int launch_few(const Args& a, const FewPlan& p, void* workspace, int32_t* status
   cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kFewThreads), Sm::kBytes, s, 1, mk, mv, a, partial, p.slots, cut ? header : nullptr, status);
   RD_CHECK_CHAINED(err);
   if (!cut) return RD_OK;
-  err = rd::launch_chained(attention_quant_merge_kernel<HD>, dim3((unsigned)(a.nkv * p.rows), (unsigned)a.B), dim3(256), 0, s, 1, a, (const float*)partial,
-                           (const int*)header, p.keys, p.rows);
+  err = rd::launch_chained(attention_quant_merge_kernel<HD, Shape<HD, BITS>::kKeys>, dim3((unsigned)(a.nkv * p.rows), (unsigned)a.B), dim3(256), 0, s, 1, a, (const float*)partial,
+                           (const int*)header, p.rows);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }

@@ -98,53 +98,67 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Rounds of row b: its tiles (at multiples of `keys` slots) over the warps of a CTA.
-__device__ __forceinline__ int rounds_of(const Args& a, int b, int keys) {
+// Rounds of row b: its tiles (at multiples of KEYS slots) over the warps of a CTA.
+template <int KEYS>
+__device__ __forceinline__ int rounds_of(const Args& a, int b) {
   const Row r = row_of(a, b);
   if (r.n_new <= 0 || r.end <= 0) return 0;
-  const int tiles = (r.first + r.end + keys - 1) / keys - r.first / keys;
+  const int tiles = (int)((uint32_t)(r.first + r.end + KEYS - 1) / KEYS - (uint32_t)r.first / KEYS);
   return (tiles + kFewWarps - 1) / kFewWarps;
 }
+// All rows' rounds, those of the first kListed rows in shared memory: the choice below asks for them again and again.  (Reading the rows' lengths anew
+// each time cost a call of one row 2.6 us, one of 131072 keys 5.)
+constexpr int kListed = 512;
+template <int KEYS>
+struct Rounds {
+  const Args& a;
+  const int* listed;
+  __device__ __forceinline__ int operator()(int b) const { return b < kListed ? listed[b] : rounds_of<KEYS>(a, b); }
+};
+__device__ __forceinline__ int chunks_of(int rounds, int chunk) { return (int)((uint32_t)(rounds + chunk - 1) / (uint32_t)chunk); }
 // Items of all rows at this chunk; one warp.
-__device__ __forceinline__ int count_items(const Args& a, int keys, int chunk) {
+template <typename R>
+__device__ __forceinline__ int count_items(const Args& a, const R& rounds, int chunk) {
   int n = 0;
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) n += (rounds_of(a, b, keys) + chunk - 1) / chunk;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) n += chunks_of(rounds(b), chunk);
   return rd::warp_sum_i(n) * a.nkv;
 }
 // The chunk of a launch of `slots` CTAs; one warp, the same answer in every CTA.  One item to a CTA if that fills them evenly: the smallest chunk that
 // leaves no more items than CTAs is at most 1.25 times what an even share would be.  Otherwise four items to a CTA, one after another.
-__device__ __forceinline__ int choose_chunk(const Args& a, int keys, int slots) {
+template <typename R>
+__device__ __forceinline__ int choose_chunk(const Args& a, const R& rounds, int slots) {
   int total = 0, most = 0;
   for (int b = threadIdx.x & 31; b < a.B; b += 32) {
-    const int r = rounds_of(a, b, keys);
+    const int r = rounds(b);
     total += r;
     most = max(most, r);
   }
   total = rd::warp_sum_i(total);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
   if (most == 0) return 1;
   const int64_t work = (int64_t)total * a.nkv;
-  int lo = (int)max((work + slots - 1) / slots, (int64_t)1), hi = min(most, lo + lo / 4);  // a chunk in (lo - 1, hi] is looked for
+  int lo = (int)max((work + slots - 1) / slots, (int64_t)1);  // a chunk in [lo, hi] is looked for
   if (lo >= most) return most;
-  if (count_items(a, keys, hi) > slots) return (int)max((work + 4 * slots - 1) / (4 * slots), (int64_t)1);
+  int hi = min(most, lo + lo / 4);
+  if (count_items(a, rounds, hi) > slots) return (int)max((work + 4 * slots - 1) / (4 * slots), (int64_t)1);
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
-    if (count_items(a, keys, mid) <= slots) hi = mid;
+    if (count_items(a, rounds, mid) <= slots) hi = mid;
     else lo = mid + 1;
   }
   return hi;
 }
 struct Item {
-  int b, head, index, of, before;  // row, key/value head, chunk of the chain, chunks of the chain, items of the rows before
+  int b, head, index, of;  // row, key/value head, chunk of the chain, chunks of the chain
 };
 // Item i; one warp, all lanes the same answer.  b = -1: there are fewer.  The heads of a chunk come one after another.
-__device__ __forceinline__ Item find_item(const Args& a, int keys, int chunk, int i) {
-  Item it{-1, 0, 0, 0, 0};
+template <typename R>
+__device__ __forceinline__ Item find_item(const Args& a, const R& rounds, int chunk, int i) {
+  Item it{-1, 0, 0, 0};
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int chunks = b0 + lane < a.B ? (rounds_of(a, b0 + lane, keys) + chunk - 1) / chunk : 0;
+    const int chunks = b0 + lane < a.B ? chunks_of(rounds(b0 + lane), chunk) : 0;
     int sum = chunks * a.nkv;
     const int mine = sum;
 #pragma unroll
@@ -158,8 +172,7 @@ __device__ __forceinline__ Item find_item(const Args& a, int keys, int chunk, in
       const int start = before + __shfl_sync(0xffffffffu, sum - mine, who);
       it.of = __shfl_sync(0xffffffffu, chunks, who);
       it.b = b0 + who;
-      it.before = start;
-      it.index = (i - start) / a.nkv;
+      it.index = (int)((uint32_t)(i - start) / (uint32_t)a.nkv);
       it.head = (i - start) - it.index * a.nkv;
       return it;
     }
@@ -176,7 +189,7 @@ template <int HD, int BITS, int NT>
 struct FewSmem {
   static constexpr int kRing = kFewWarps * kFewStages * Shape<HD, BITS>::kStage;
   static constexpr int kMerge = kFewWarps * 8 * NT * (HD + 4) * 4;  // outputs, then maxima and sums, of all warps
-  static constexpr int kBytes = 1024 + (kRing > kMerge ? kRing : kMerge) + kFewWarps * kFewStages * 8 + 64;
+  static constexpr int kBytes = 1024 + (kRing > kMerge ? kRing : kMerge) + kFewWarps * kFewStages * 8 + 16;
 };
 
 template <int HD, int BITS, int NT>
@@ -187,6 +200,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   constexpr int kKeys = S::kKeys, kSub = kKeys / 16, kMT = HD / 16;
   constexpr int kRows = 8 * NT;
   extern __shared__ uint8_t raw[];
+  __shared__ int listed[kListed];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   using Sm = FewSmem<HD, BITS, NT>;
   constexpr int kData = Sm::kRing > Sm::kMerge ? Sm::kRing : Sm::kMerge;
@@ -203,9 +217,11 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
     for (int s = 0; s < kFewStages; ++s) rd_umma::mbar_init(&full[s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
   rd::pdl_wait();
-  const int chunk = choose_chunk(a, kKeys, slots);
+  for (int b = threadIdx.x; b < a.B && b < kListed; b += kFewThreads) listed[b] = rounds_of<kKeys>(a, b);
+  __syncthreads();
+  const Rounds<kKeys> rounds{a, listed};
+  const int chunk = choose_chunk(a, rounds, slots);
   if (blockIdx.x == 0 && threadIdx.x == 0 && header != nullptr) *header = chunk;
   const int group = a.nh / a.nkv;
   const int64_t plane_rows = (int64_t)a.B * a.nkv * a.max_len;
@@ -219,7 +235,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
   uint32_t used = 0;  // tiles that this warp has waited for so far: stage and phase
   bool ok = true;
   for (int item = blockIdx.x; ok; item += gridDim.x) {
-    const Item it = find_item(a, kKeys, chunk, item);
+    const Item it = find_item(a, rounds, chunk, item);
     if (it.b < 0) break;
     const Row r = row_of(a, it.b);
     const int64_t chain = (int64_t)it.b * a.nkv + it.head;
@@ -567,8 +583,8 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
 
 // Sums the chunks of the chains that have several.  A CTA for each query row of each chain, its warps a share of the chunks each: a trip to
 // memory for every eight chunks.
-template <int HD>
-__global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a, const float* partial, const int* header, int keys, int item_rows) {
+template <int HD, int KEYS>
+__global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a, const float* partial, const int* header, int item_rows) {
   __shared__ float vs[8][HD], sums[8][2];
   rd::pdl_launch_dependents();
   rd::pdl_wait();
@@ -577,10 +593,10 @@ __global__ void __launch_bounds__(256) attention_quant_merge_kernel(const Args a
   const int chunk = *reinterpret_cast<const volatile int*>(header);
   const Row r = row_of(a, b);
   if (row >= r.n_new * group) return;
-  const int n = (rounds_of(a, b, keys) + chunk - 1) / chunk;
+  const int n = chunks_of(rounds_of<KEYS>(a, b), chunk);
   if (n <= 1) return;
   int before = 0;
-  for (int x = lane; x < b; x += 32) before += (rounds_of(a, x, keys) + chunk - 1) / chunk;
+  for (int x = lane; x < b; x += 32) before += chunks_of(rounds_of<KEYS>(a, x), chunk);
   before = rd::warp_sum_i(before) * a.nkv;
   const int64_t step = few_item_floats(HD, item_rows) * a.nkv;
   const float* p = partial + (before + head) * few_item_floats(HD, item_rows) + row * (HD + 2);
