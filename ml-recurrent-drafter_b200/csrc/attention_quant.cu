@@ -138,30 +138,6 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const
 #include "attention_quant_few.cuh"
 #include "attention_quant_many.cuh"
 
-// Lets a kernel have its dynamic shared memory on the current device; once for each.
-template <auto Kernel>
-bool allow_smem(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return true;
-  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err != cudaSuccess) {
-    rd_set_last_cuda_error((int)err);
-    return false;
-  }
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-int sm_count() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
-  }();
-  return n;
-}
-
 // The few-rows kernel serves 16-bit queries of heads of 64 or 128 features whose group has at most kFewRows rows.
 struct FewPlan {
   int rows;          // of an item: 8 or 16; 0: not for this call
@@ -174,7 +150,7 @@ FewPlan few_plan(int dtype, int bits, int B, int nh, int nkv, int hd, int max_ne
   if (dtype != RD_BF16 || (hd != 64 && hd != 128) || rows > kFewRows) return p;
   p.rows = rows <= 8 ? 8 : 16;
   p.keys = kTileBytes * 8 / (hd * bits);
-  p.slots = sm_count() * (p.rows == 8 ? 2 : 1);
+  p.slots = rd_quant::sm_count() * (p.rows == 8 ? 2 : 1);
   const int64_t tiles = ((int64_t)max_kv + p.keys - 1) / p.keys + 1, chains = (int64_t)B * nkv;  // one more: rows begin inside a tile
   const int64_t all = chains * ((tiles + kFewWarps - 1) / kFewWarps);
   p.items = all < chains + 4 * p.slots ? all : chains + 4 * p.slots;
@@ -187,7 +163,7 @@ template <int HD, int BITS, int NT>
 int launch_few(const Args& a, const FewPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
   constexpr auto kernel = attention_quant_few_kernel<HD, BITS, NT>;
   using Sm = FewSmem<HD, BITS, NT>;
-  RD_REQUIRE(allow_smem<kernel>(Sm::kBytes), RD_ERR_LAUNCH);
+  RD_REQUIRE(rd_quant::allow_smem<kernel>(Sm::kBytes), RD_ERR_LAUNCH);
   CUtensorMap mk, mv;
   const int64_t lines = (int64_t)a.B * a.nkv * a.max_len * (HD * BITS / 8) / 128;
   RD_REQUIRE(lines <= 0x7fffffff, RD_ERR_SIZE);
@@ -216,10 +192,11 @@ ManyPlan many_plan(int dtype, int B, int nh, int nkv, int hd, int max_new, int m
   const int64_t rows = (int64_t)max_new * (nh / nkv), chains = (int64_t)B * nkv;
   ManyPlan p{dtype == RD_BF16 && (hd == 64 || hd == 128) && rows > kFewRows, 1, 1};
   if (!p.here) return p;
-  // two tiles to a CTA where these CTAs, one on an SM, still fill the SMs
-  if (chains * ((rows + 2 * kManyRows - 1) / (2 * kManyRows)) >= sm_count() && rows > kManyRows) p.tiles = 2;
+  // Two tiles that share their keys cost 0.7 to 0.85 of two that do not, if both are there and such pairs fill the SMs.  Where the bound is one of several
+  // rows' it is taken for half as much again as most have: eight draft trees of 64 to 140 query rows take 38 us in such pairs and 32 without.
+  if (chains * ((rows + 2 * kManyRows - 1) / (2 * kManyRows)) >= rd_quant::sm_count() && rows > (B == 1 ? kManyRows : kManyRows * 3 / 2)) p.tiles = 2;
   // Shares of the keys where the query tiles leave CTAs idle: enough to fill two to an SM, each of at least four tiles of keys.
-  const int64_t ctas = chains * ((rows + p.tiles * kManyRows - 1) / (p.tiles * kManyRows)), slots = 2 * sm_count() / p.tiles;
+  const int64_t ctas = chains * ((rows + p.tiles * kManyRows - 1) / (p.tiles * kManyRows)), slots = 2 * rd_quant::sm_count() / p.tiles;
   if (2 * ctas >= slots) return p;
   const int64_t by_fill = slots / ctas, by_length = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys / 4;
   int64_t n = by_fill < by_length ? by_fill : by_length;
@@ -232,10 +209,12 @@ template <int HD, int BITS, int QT>
 int launch_many(const Args& a, const ManyPlan& p, void* workspace, int32_t* status, cudaStream_t s) {
   constexpr auto kernel = attention_quant_many_kernel<HD, BITS, QT>;
   using L = Many<HD, QT>;
-  RD_REQUIRE(allow_smem<kernel>(L::kBytes), RD_ERR_LAUNCH);
-  const int64_t tiles = ((int64_t)a.max_new * (a.nh / a.nkv) + QT * kManyRows - 1) / (QT * kManyRows) * p.n_split;
-  RD_REQUIRE(tiles <= 0x7fffffff, RD_ERR_SIZE);
-  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)tiles, a.nkv, a.B), dim3(L::kThreads), L::kBytes, s, 1, a, (float*)workspace, p.n_split, status);
+  RD_REQUIRE(rd_quant::allow_smem<kernel>(L::kBytes), RD_ERR_LAUNCH);
+  const int64_t tiles = ((int64_t)a.max_new * (a.nh / a.nkv) + QT * kManyRows - 1) / (QT * kManyRows), items = tiles * p.n_split * a.nkv * a.B;
+  RD_REQUIRE(items <= 0x7fffffff, RD_ERR_SIZE);
+  const int64_t grid = items <= rd_quant::sm_count() ? items : (items + L::kParts - 1) / L::kParts;
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)grid), dim3(L::kThreads), L::kBytes, s, 1, a, (float*)workspace, (int)tiles, p.n_split,
+                                       (unsigned)items, status);
   RD_CHECK_CHAINED(err);
   if (p.n_split == 1) return RD_OK;
   err = rd::launch_chained(attention_quant_merge_shares_kernel<HD>, dim3((unsigned)(((int64_t)a.max_new * a.nh + 7) / 8), a.B), dim3(256), 0, s, 1, a,

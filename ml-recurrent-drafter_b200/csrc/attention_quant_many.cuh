@@ -1,7 +1,7 @@
 // Attention over a cache in codes for many query rows to a key/value head (packed drafts, prompts), on the 5th-generation tensor cores:
 // included by attention_quant.cu.
 //
-// One CTA serves QT tiles of 128 query rows of one (batch row, key/value head): row R is head R % group of new token R / group, so that the codes of
+// One part of a CTA serves QT tiles of 128 query rows of one (batch row, key/value head): row R is head R % group of new token R / group, so that the codes of
 // a tile of keys are unpacked once for all of them.
 //   4 QT warps  the queries, scaled by a power of two to fp16, into shared memory; then softmax: a thread owns a row (= TMEM lane), running
 //               maximum and sum, weights W = 2^7 p as fp16 to TMEM;
@@ -16,7 +16,7 @@
 // 32 scores at a time, and weighted by the maximum so far; only where the sum of the weights turns out too large the tile's maximum is
 // looked for and the tile weighted again.
 // Features lie in the order in which the masks deliver them (within 8 of 4 bits: 0 4 1 5 2 6 3 7, within 4 of 8 bits: 0 2 1 3); the queries
-// take the same order, the output undoes it.  QT = 1: two CTAs on an SM overlap each other's waits; QT = 2: one, which unpacks half as often.
+// take the same order, the output undoes it.  QT = 2 unpacks half as often; with QT = 1 an SM works at two of these at once all the same.
 // With n_split > 1 a CTA walks its share of the tiles and leaves its sums for attention_quant_merge_shares_kernel.
 //
 // Every wait is bounded; on give-up the kernel records a code in *status, frees its TMEM and returns.
@@ -26,17 +26,23 @@ constexpr int kManyMaxSplit = 16;
 constexpr float kWeightBits = 7.f;        // weights are 2^7 p
 constexpr float kMostWeights = 32768.f;   // of a tile of a row: none is more, and fp16 holds it
 
+// A CTA is kParts of what the head of this file describes: one of two tiles, or two of one tile that share nothing but the SM.  (The driver places
+// one CTA on an SM where a kernel uses tensor memory, whatever its registers and shared memory.)
 template <int HD, int QT>
 struct Many {
-  static constexpr int kThreads = (5 * QT + 4) * 32;
+  static constexpr int kParts = QT == 1 ? 2 : 1;
+  static constexpr int kTiles = QT * kParts;
+  static constexpr int kUnpack = 4 * kTiles, kIssue = kUnpack + 4 * kParts;  // first warps of these roles; softmax first: its warps' lanes in TMEM
+  static constexpr int kThreads = (kIssue + kTiles) * 32;
   static constexpr int kStages = QT == 1 ? 2 : 4;  // of unpacked keys, and of values
   static constexpr int kQ = kManyRows * HD * 2, kTile = kManyKeys * HD * 2;  // bytes
   static constexpr int kBars = 256;
   static constexpr int kVectors = 8 * 4 * 4;                                // of eight tiles: r, the keys' power of two, which values are NaN
-  static constexpr int kBytes = 1024 + QT * kQ + 2 * kStages * kTile + kVectors + QT * kManyRows * 4 + kBars;
+  static constexpr int kPart = (QT * kQ + 2 * kStages * kTile + kVectors + QT * kManyRows * 4 + kBars + 1023) / 1024 * 1024;
+  static constexpr int kBytes = 1024 + kParts * kPart;
   // TMEM of a tile of rows: two buffers of 64 columns for S, then W; O
-  static constexpr uint32_t kColS = 0, kColO = 128, kCols = 128 + HD;
-  static constexpr uint32_t kTmem = QT * kCols <= 256 ? 256 : 512;
+  static constexpr uint32_t kColS = 0, kColO = 128, kCols = 256;
+  static constexpr uint32_t kTmem = kTiles * kCols;
 };
 
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
@@ -139,12 +145,17 @@ __device__ __forceinline__ constexpr int order8(int k) {
 }
 
 template <int HD, int BITS, int QT>
-__global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
-    attention_quant_many_kernel(const Args a, float* partial, int n_split, int32_t* status) {
+__global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
+    attention_quant_many_kernel(const Args a, float* partial, int n_row_tiles, int n_split, unsigned n_items, int32_t* status) {
   using L = Many<HD, QT>;
-  constexpr int kUnpack = 4 * QT, kIssue = kUnpack + 4;  // first warps of these roles
+  constexpr int kUnpack = L::kUnpack, kIssue = L::kIssue;
   extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint32_t tmem_slot;
+  __shared__ int stop_flag;
+  volatile int* stop = &stop_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = L::kParts == 1 ? 0 : warp < kUnpack ? warp >> 2 : warp < kIssue ? (warp - kUnpack) >> 2 : warp - kIssue;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023) + part * L::kPart;
   uint8_t* sQ = smem;
   uint8_t* sK = smem + QT * L::kQ;
   constexpr int kSt = L::kStages;
@@ -159,30 +170,30 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
   uint64_t* s_full = q_full + QT;         // [QT][2]
   uint64_t* p_full = s_full + 2 * QT;     // [QT][2]
   uint64_t* o_full = p_full + 2 * QT;     // [QT][2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2 * QT);
-  volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((4 * kSt + 7 * QT) * 8 + 8 <= L::kBars, "barriers");
+  static_assert((4 * kSt + 7 * QT) * 8 <= L::kBars, "barriers");
 
   const int group = a.nh / a.nkv;
-  // in causal calls later tiles see more keys: they start first
-  const bool late_first = a.mode == RD_ATTN_CAUSAL && n_split == 1 && gridDim.x > 1;
-  const int linear = (int)(blockIdx.x + gridDim.x * blockIdx.y);
-  const int bx = late_first ? (int)gridDim.x - 1 - linear / (int)gridDim.y : (int)blockIdx.x;
-  const int hk = late_first ? linear % (int)gridDim.y : (int)blockIdx.y;
-  const int b = blockIdx.z, split = bx % n_split, q0 = bx / n_split * (QT * kManyRows);
+  // Which tile of which head of which row, and which share of its keys.  In causal calls later tiles see more keys: they start first.
+  const int n_tiles_all = n_row_tiles * n_split;
+  const unsigned index = gridDim.x < n_items ? blockIdx.x * L::kParts + part : blockIdx.x;
+  const bool none = index >= n_items || (gridDim.x >= n_items && part > 0);
+  const int b = none ? 0 : index / ((unsigned)n_tiles_all * a.nkv), in_row = none ? 0 : index % ((unsigned)n_tiles_all * a.nkv);
+  const bool late_first = a.mode == RD_ATTN_CAUSAL && n_split == 1;
+  const int hk = in_row % a.nkv, bx = late_first ? n_tiles_all - 1 - in_row / a.nkv : in_row / a.nkv;
+  const int split = bx % n_split, q0 = bx / n_split * (QT * kManyRows);
   rd::pdl_launch_dependents();
   rd::pdl_wait();
   const Row r = row_of(a, b);
-  const int rows = r.n_new * group;
-  if (q0 >= rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_q = QT == 1 ? 1 : min(QT, (rows - q0 + kManyRows - 1) / kManyRows);  // tiles of rows that there are
+  const int rows = none ? 0 : r.n_new * group;
+  if (!__syncthreads_or(q0 < rows)) return;
+  const bool here = q0 < rows;
+  const int n_q = !here ? 0 : QT == 1 ? 1 : min(QT, (rows - q0 + kManyRows - 1) / kManyRows);  // tiles of rows that there are
   const int first_token = q0 / group, last_token = (min(q0 + QT * kManyRows, rows) - 1) / group;
   const int kv_end = a.mode == RD_ATTN_CAUSAL ? min(r.end, r.base + last_token + 1) : r.end;
   const int all_tiles = (max(kv_end, 0) + kManyKeys - 1) / kManyKeys;
   const int per_split = (all_tiles + n_split - 1) / n_split;
-  const int t_begin = split * per_split, n_tiles = max(0, min(per_split, all_tiles - t_begin));
-  if (threadIdx.x == 0) {
+  const int t_begin = split * per_split, n_tiles = here ? max(0, min(per_split, all_tiles - t_begin)) : 0;
+  if (here && lane == 0 && warp == part * 4) {
     for (int s = 0; s < QT; ++s) rd_umma::mbar_init(&q_full[s], 4);
     for (int s = 0; s < kSt; ++s) {
       rd_umma::mbar_init(&k_full[s], 4);
@@ -195,14 +206,14 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       rd_umma::mbar_init(&p_full[s], 4);
       rd_umma::mbar_init(&o_full[s], 1);
     }
-    *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kIssue) rd_umma::tmem_alloc(tmem_slot, L::kTmem);
+  if (threadIdx.x == 0) *stop = 0;
+  if (warp == kIssue) rd_umma::tmem_alloc(&tmem_slot, L::kTmem);
   rd_umma::fence_before();
   __syncthreads();
   rd_umma::fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = tmem_slot + part * L::kCols;
   bool ok = true;
   int site = 0;
 
@@ -210,12 +221,13 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     // ---------------- unpacking ----------------
     constexpr int kBytes = HD * BITS / 16;  // a thread's half of a key: 16, 32 or 64 bytes
     constexpr int kLoads = kBytes / 16, kChunks = HD / 16, kWordsOf8 = BITS / 4;
-    const int tid = threadIdx.x - kUnpack * 32, key = tid & 63, half = tid >> 6;
+    const int tid = (threadIdx.x - kUnpack * 32) & 127, key = tid & 63, half = tid >> 6;
     const int64_t plane = ((int64_t)b * a.nkv + hk) * a.max_len + r.first;
-    // Two tiles are under way: what a tile's codes are asked into is free when the tile two before has been stored, so that a trip to
-    // memory has the time of a whole tile.
-    uint4 kc[2][kLoads], vc[2][kLoads];
-    uint32_t kp[2] = {}, kq[2] = {}, vp[2] = {}, vq[2] = {};
+    // With two tiles under way, what a tile's codes are asked into is free when the tile two before has been stored, so that a trip to memory has the
+    // time of a whole tile (2048 rows of 8192 keys: 313 us with one, 305 with two).  QT = 1 has no registers for that.
+    constexpr int kDeep = QT;
+    uint4 kc[kDeep][kLoads], vc[kDeep][kLoads];
+    uint32_t kp[kDeep] = {}, kq[kDeep] = {}, vp[kDeep] = {}, vq[kDeep] = {};
     // Keys past the last one stand for zeros.
     auto request_k = [&](int t, auto set) {
       constexpr int S = decltype(set)::value;
@@ -277,7 +289,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
         if (key == 0) e[0] = __uint_as_float(top - (kUp << 23)), e[1] = __uint_as_float(k_top - (kUp << 23));
       }
       const uint32_t vz = vp[S];
-      request_k(t + 2, set);
+      request_k(t + kDeep, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[st]);
@@ -286,24 +298,26 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
         return;
       }
       store(sV + st * L::kTile, vc[S], vz, v);
-      request_v(t + 2, set);
+      request_v(t + kDeep, set);
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[st]);
     };
-    using Even = std::integral_constant<int, 0>;
-    using Odd = std::integral_constant<int, 1>;
-    request_k(0, Even());
-    request_v(0, Even());
-    request_k(1, Odd());
-    request_v(1, Odd());
+    using First = std::integral_constant<int, 0>;
+    using Last = std::integral_constant<int, kDeep - 1>;
+    request_k(0, First());
+    request_v(0, First());
+    if (kDeep == 2) {
+      request_k(1, Last());
+      request_v(1, Last());
+    }
     for (int t = 0; ok && t < n_tiles; t += 2) {
-      unpack(t, Even());
-      if (ok && t + 1 < n_tiles) unpack(t + 1, Odd());
+      unpack(t, First());
+      if (ok && t + 1 < n_tiles) unpack(t + 1, Last());
     }
   } else if (warp >= kIssue) {
     // ---------------- products: a warp for each tile of rows, so that neither waits for the other's softmax ----------------
-    const int x = warp - kIssue;
+    const int x = L::kParts == 1 ? warp - kIssue : 0;
     if (x < n_q && rd::elect_one()) {
       const uint32_t idesc_qk = idesc_fp16(kManyKeys, false), idesc_pv = idesc_fp16(HD, true);
       const uint32_t q = rd_umma::smem_u32(sQ + x * L::kQ), base = tmem + x * L::kCols;
@@ -340,63 +354,66 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
       if (!ok) site = 3;
     }
     __syncwarp();
-  } else if (warp < 4 * n_q) {
-    const int tile = warp >> 2, quarter = warp & 3;
+  } else if ((L::kParts == 1 ? warp >> 2 : 0) < n_q) {
+    const int tile = L::kParts == 1 ? warp >> 2 : 0, quarter = warp & 3;
     uint8_t* myQ = sQ + tile * L::kQ;
-    // ---------------- queries: eight lanes a row ----------------
+    const int row = quarter * 32 + lane, R = q0 + tile * kManyRows + row;
+    const bool live = R < rows;
+    const int token = live ? R / group : 0, head = hk * group + (live ? R % group : 0);
+    // ---------------- queries: eight lanes a row; bf16 goes where fp16 is to stand, and is converted there by who brought it ----------------
     {
-      const int part = lane & 7;
-      constexpr int kPart = HD / 8, kAtOnce = 8;  // features of a lane: 8 or 16; rows
-#pragma unroll 1
-      for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
-        uint4 u[kAtOnce][kPart / 8];  // asked for before the first is looked at
+      constexpr int kPart = HD / 8;  // features of a lane: 8 or 16
+      const int eighth = lane & 7;
+      const int64_t mine = (int64_t)(r.start + token) * a.ldq + head * HD;
+      auto place = [&](int i, int c) {
+        const int of = quarter * 32 + i * 4 + (lane >> 3), chunk = eighth * (kPart / 8) + c;
+        return myQ + (chunk >> 3) * (kManyRows * 128) + of * 128 + (((chunk & 7) ^ (of & 7)) << 4);
+      };
+#pragma unroll 2
+      for (int i = 0; i < 8; ++i) {
+        const int64_t from = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
+        const int there = __shfl_sync(0xffffffffu, live ? 16 : 0, i * 4 + (lane >> 3));  // bytes; zeros for the others
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-          const int R = q0 + tile * kManyRows + quarter * 32 + (i0 + i) * 4 + (lane >> 3);
-          const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (int64_t)(r.start + R / group) * a.ldq + (hk * group + R % group) * HD + part * kPart);
+        for (int c = 0; c < kPart / 8; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(rd_umma::smem_u32(place(i, c))),
+                       "l"((const __nv_bfloat16*)a.q + from + eighth * kPart + c * 8), "r"(there)
+                       : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+      for (int i = 0; i < 8; ++i) {
+        float x[kPart], most = 0.f;
 #pragma unroll
-          for (int c = 0; c < kPart / 8; ++c) u[i][c] = R < rows ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < kPart / 8; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(place(i, c));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[8 * c + 2 * e] = __uint_as_float(w[e] << 16), x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
         }
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-          const int row = quarter * 32 + (i0 + i) * 4 + (lane >> 3);
-          float x[kPart];
+        for (int e = 0; e < kPart; ++e) most = fmaxf(most, fabsf(x[e]));
 #pragma unroll
-          for (int c = 0; c < kPart / 8; ++c) {
-            const uint32_t w[4] = {u[i][c].x, u[i][c].y, u[i][c].z, u[i][c].w};
+        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // the row's largest to [2^14, 2^15): see the few-rows kernel
+        const int e2 = most > 0.f && most < INFINITY ? (int)(__float_as_uint(most) >> 23) : 141;
+        const int up = 141 - e2, h1 = up / 2, h2 = up - h1;
+        const float f1 = __uint_as_float((uint32_t)(127 + h1) << 23), f2 = __uint_as_float((uint32_t)(127 + h2) << 23);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[8 * c + 2 * e] = __uint_as_float(w[e] << 16), x[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-          }
-          float most = 0.f;
+        for (int c = 0; c < kPart / 8; ++c) {
+          float y[8];
 #pragma unroll
-          for (int e = 0; e < kPart; ++e) most = fmaxf(most, fabsf(x[e]));
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          // the row's largest to [2^14, 2^15): see the few-rows kernel
-          const int e2 = most > 0.f && most < INFINITY ? (int)(__float_as_uint(most) >> 23) : 141;
-          const int up = 141 - e2, h1 = up / 2, h2 = up - h1;
-          const float f1 = __uint_as_float((uint32_t)(127 + h1) << 23), f2 = __uint_as_float((uint32_t)(127 + h2) << 23);
-#pragma unroll
-          for (int c = 0; c < kPart / 8; ++c) {
-            float y[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[order8<BITS>(k)] = x[8 * c + k] * f1 * f2;
-            const int chunk = part * (kPart / 8) + c;
-            *reinterpret_cast<uint4*>(myQ + (chunk >> 3) * (kManyRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-                make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7]));
-          }
-          if (part == 0)
-            units[tile * kManyRows + row] = a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
+          for (int k = 0; k < 8; ++k) y[order8<BITS>(k)] = x[8 * c + k] * f1 * f2;
+          *reinterpret_cast<uint4*>(place(i, c)) = make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[3]), pack_f16(y[4], y[5]), pack_f16(y[6], y[7]));
         }
+        if (eighth == 0)
+          units[tile * kManyRows + quarter * 32 + i * 4 + (lane >> 3)] =
+              a.scale * 1.44269504f * __uint_as_float((uint32_t)(127 - h1) << 23) * __uint_as_float((uint32_t)(127 - h2) << 23);
       }
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[tile]);
     }
     // ---------------- softmax: a thread a row ----------------
-    const int row = quarter * 32 + lane, R = q0 + tile * kManyRows + row;
-    const bool live = R < rows;
-    const int token = live ? R / group : 0;
     const float unit = units[tile * kManyRows + row];  // its own warp's
     const uint32_t taddr = tmem + tile * L::kCols + ((uint32_t)(quarter * 32) << 16);
     const int all_see = a.mode == RD_ATTN_CAUSAL ? min(kv_end, r.base + first_token + 1) : min(kv_end, r.base);
@@ -528,7 +545,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
     }
     if (ok) {
       rd_umma::fence_after();
-      const int64_t at = (int64_t)(r.start + token) * a.nh + hk * group + (live ? R % group : 0);
+      const int64_t at = (int64_t)(r.start + token) * a.nh + head;
       float* to = partial + (at * n_split + split) * (HD + 2);
       const float f = n_split > 1 ? ref : (l_run == 0.f ? 0.f : ref / l_run);  // the weights' 2^7 is in O and in l
 #pragma unroll 1
@@ -565,7 +582,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, QT == 1 ? 2 : 1)
   __syncthreads();
   if (warp == kIssue) {
     rd_umma::fence_after();
-    rd_umma::tmem_dealloc(tmem, L::kTmem);
+    rd_umma::tmem_dealloc(tmem_slot, L::kTmem);
   }
 }
 

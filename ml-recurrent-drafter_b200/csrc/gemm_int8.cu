@@ -574,30 +574,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   }
 }
 
-// Lets a kernel have its dynamic shared memory on the current device; once for each.
-template <auto Kernel>
-bool allow_smem(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return true;
-  const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err != cudaSuccess) {
-    rd_set_last_cuda_error((int)err);
-    return false;
-  }
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-int sm_count() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
-  }();
-  return n;
-}
-
 // How many CTAs of a kernel run at the same time in clusters of `shares`; asked once for each size of cluster and of shared memory.
 template <auto Kernel>
 int64_t resident_ctas(int shares, int threads, int smem, bool half) {
@@ -606,7 +582,7 @@ int64_t resident_ctas(int shares, int threads, int smem, bool half) {
   int n = here.load(std::memory_order_relaxed);
   if (n == 0) {
     if (shares == 1) {
-      n = sm_count() * (half ? 2 : 1);
+      n = rd_quant::sm_count() * (half ? 2 : 1);
     } else {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(shares);
@@ -637,7 +613,7 @@ struct ManyShape {
 };
 ManyShape many_shape(const Int8Args& a) {
   // features of a tile: the width with which the rounds of tiles take least, a tile of w features counting w + 64
-  const int64_t pairs = sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
+  const int64_t pairs = rd_quant::sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
   ManyShape sh{kMostWidth, 0, 0};
   int64_t best = INT64_MAX;
   for (int w = kMostWidth; w >= 64; w /= 2) {
@@ -653,7 +629,7 @@ int64_t few_shape(const Int8Args& a, FewShape& sh) {
   if (sh.tokens > kFewTokens) return INT64_MAX;
   // Weight rows of a CTA and shares of K: those with which an SM has the fewest bytes to bring in, all CTAs at the same time, one on an SM or two.
   // Fewer shares where that is the same.
-  const int sms = sm_count(), k_blocks = (a.K + kBlock - 1) / kBlock;
+  const int sms = rd_quant::sm_count(), k_blocks = (a.K + kBlock - 1) / kBlock;
   int64_t best = INT64_MAX;
   for (int shares = 1; shares <= kMostShares && shares <= k_blocks; ++shares)
     for (int half = 0; half < 2; ++half) {
@@ -697,11 +673,11 @@ int launch_few(const Int8Args& a, const FewShape& sh, int32_t* status, cudaStrea
 template <typename OutT, int EPI>
 int launch_many(const Int8Args& a, const ManyShape& sh, int32_t* status, cudaStream_t s) {
   constexpr auto kernel = int8_many_kernel<OutT, EPI>;
-  RD_REQUIRE(allow_smem<kernel>(ManySmem::kBytes), RD_ERR_LAUNCH);
+  RD_REQUIRE(rd_quant::allow_smem<kernel>(ManySmem::kBytes), RD_ERR_LAUNCH);
   ManyMaps maps;
   RD_REQUIRE(rd_umma::make_byte_map(&maps.a, a.A, a.m_max, a.K, a.lda, 128) && rd_umma::make_byte_map(&maps.w, a.W, a.N, a.K, a.ldw, sh.width / 2), RD_ERR_ARG);
   RD_REQUIRE(sh.tiles <= 0x7fffffff, RD_ERR_SIZE);
-  const int64_t pairs = sm_count() / 2;
+  const int64_t pairs = rd_quant::sm_count() / 2;
   const unsigned grid = 2 * (unsigned)(sh.tiles < pairs ? sh.tiles : pairs);
   cudaError_t err = rd::launch_chained(kernel, dim3(grid), dim3(kManyThreads), ManySmem::kBytes, s, 2, maps, a, sh.width, status);
   RD_CHECK_CHAINED(err);
@@ -736,7 +712,7 @@ int check_product(int out_dtype, const Int8Args& a, int epilogue) {
 int quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_codes, float* scales, int m_max, const int32_t* m_dev, int K, cudaStream_t s) {
   cudaError_t err;
   const bool vec = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (ldx * (dtype == RD_BF16 ? 2 : 4)) % 16 == 0;
-  const bool wide = m_max <= sm_count() && K > 2048;  // a block an SM: the row's latency is the kernel's
+  const bool wide = m_max <= rd_quant::sm_count() && K > 2048;  // a block an SM: the row's latency is the kernel's
   auto run = [&](auto kern, int threads, auto* zero) {
     using T = std::remove_pointer_t<decltype(zero)>;
     err = rd::launch_chained(kern, dim3(m_max), dim3(threads), 0, s, 1, (const T*)x, ldx, codes, ld_codes, scales, m_max, m_dev, K);
@@ -759,7 +735,7 @@ int product_of(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
   FewShape few;
   const ManyShape many = many_shape(a);
   constexpr auto few_kernel = int8_few_kernel<OutT, EPI>;
-  RD_REQUIRE(allow_smem<few_kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
+  RD_REQUIRE(rd_quant::allow_smem<few_kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
   if (few_shape<few_kernel>(a, few) > many.cost) return launch_many<OutT, EPI>(a, many, status, s);
   few.early = early;
   return launch_few<OutT, EPI>(a, few, status, s);

@@ -1,6 +1,7 @@
-// What the kernels of a cache in codes of 8 or 4 bits share.  A row's parameters are 32 bits: the bf16 pattern of its scale below, its
+// What the kernels of a cache in codes of 8 or 4 bits, and of products of 8-bit integers, share.  A row's parameters are 32 bits: the bf16 pattern of its scale below, its
 // zero (0 .. 255) above; see cache_quant.cu for what they mean.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "rd_common.cuh"
@@ -49,5 +50,31 @@ struct Divider {
   }
 };
 constexpr uint32_t kRintBias = 0x4b400000u;
+
+// Lets a kernel have its dynamic shared memory on the current device, and as many CTAs on an SM as fit into that; once for each.  (Without the
+// second attribute two CTAs of 99 KB were never placed on one SM.)
+template <auto Kernel>
+bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
+  if (err != cudaSuccess) {
+    rd_set_last_cuda_error((int)err);
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+inline int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+  }();
+  return n;
+}
 
 }  // namespace rd_quant
