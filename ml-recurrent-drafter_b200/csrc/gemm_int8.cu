@@ -182,10 +182,10 @@ __device__ __forceinline__ float gated(float gate, float up) {
 // row quantiser the first ring of weights is asked for before the codes of the tokens are there (`early`: the quantiser starts its
 // successors only when all before it is complete).
 constexpr int kFewTokens = 256, kMostShares = 8;
-constexpr int kFewRing = 200 * 1024, kFewHalfRing = 94 * 1024, kFewStagesMost = 16, kFewThreads = 192;  // one CTA on an SM, two
-constexpr int few_smem(int ring) { return 1024 + ring + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512; }
+constexpr int kFewRing = 200 * 1024, kFewStagesMost = 16, kFewThreads = 192;
+constexpr int kFewSmem = 1024 + kFewRing + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512;
 struct FewShape {
-  int slab, shares, tokens, blocks, stages, ring, tmem_cols, early;  // tokens: of m_max, a multiple of 16; blocks of K a stage
+  int slab, shares, tokens, blocks, stages, tmem_cols, early;  // slab: a multiple of 8; tokens: of m_max, a multiple of 16; blocks of K a stage
 };
 
 template <typename OutT, int EPI>
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kFewThreads)
     int8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Int8Args a, const FewShape sh, int32_t* status) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + sh.ring + 16 * 1024);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kFewRing + 16 * 1024);
   uint64_t* empty = full + kFewStagesMost;
   uint64_t* acc_full = empty + kFewStagesMost;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
@@ -574,15 +574,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   }
 }
 
-// How many CTAs of a kernel run at the same time in clusters of `shares`; asked once for each size of cluster and of shared memory.
+// How many CTAs of a kernel, one on an SM, run at the same time in clusters of `shares`; asked once for each size of cluster.
 template <auto Kernel>
-int64_t resident_ctas(int shares, int threads, int smem, bool half) {
-  static std::atomic<int> known[kMostShares + 1][2] = {};
-  std::atomic<int>& here = known[shares][half];
+int64_t resident_ctas(int shares, int threads, int smem) {
+  static std::atomic<int> known[kMostShares + 1] = {};
+  std::atomic<int>& here = known[shares];
   int n = here.load(std::memory_order_relaxed);
   if (n == 0) {
     if (shares == 1) {
-      n = rd_quant::sm_count() * (half ? 2 : 1);
+      n = rd_quant::sm_count();
     } else {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(shares);
@@ -616,7 +616,7 @@ ManyShape many_shape(const Int8Args& a) {
   const int64_t pairs = rd_quant::sm_count() / 2, t_tiles = (a.m_max + kTileTokens - 1) / kTileTokens;
   ManyShape sh{kMostWidth, 0, 0};
   int64_t best = INT64_MAX;
-  for (int w = kMostWidth; w >= 64; w /= 2) {
+  for (int w = kMostWidth; w >= 64; w -= 64) {
     const int64_t tiles = t_tiles * ((a.N + w - 1) / w), rounds = (tiles + pairs - 1) / pairs;
     if (rounds * (w + 64) < best) best = rounds * (w + 64), sh = ManyShape{w, rounds * (128 + w / 2) * ((a.K + kBlock - 1) / kBlock), tiles};
   }
@@ -627,31 +627,29 @@ template <auto kernel>
 int64_t few_shape(const Int8Args& a, FewShape& sh) {
   sh.tokens = (a.m_max + 15) / 16 * 16;
   if (sh.tokens > kFewTokens) return INT64_MAX;
-  // Weight rows of a CTA and shares of K: those with which an SM has the fewest bytes to bring in, all CTAs at the same time, one on an SM or two.
-  // Fewer shares where that is the same.
+  // Weight rows of a CTA and shares of K: those with which an SM has the fewest bytes to bring in, all CTAs at the same time.  Fewer shares where
+  // that is the same.
   const int sms = rd_quant::sm_count(), k_blocks = (a.K + kBlock - 1) / kBlock;
+  static_assert(kFewTokens * 512 <= kFewRing, "the sums");
   int64_t best = INT64_MAX;
-  for (int shares = 1; shares <= kMostShares && shares <= k_blocks; ++shares)
-    for (int half = 0; half < 2; ++half) {
-      const int ring = half ? kFewHalfRing : kFewRing;
-      if (sh.tokens * 512 > ring) continue;  // the sums
-      const int64_t most = resident_ctas<kernel>(shares, kFewThreads, few_smem(ring), half);
-      for (int slab = 128; slab >= 16; slab -= 16) {
-        const int64_t ctas = (int64_t)((a.N + slab - 1) / slab) * shares;
-        if (ctas > most) break;
-        const int64_t cost = (ctas + sms - 1) / sms * ((slab + sh.tokens) * ((k_blocks + shares - 1) / shares) + 8 * sh.tokens);
-        if (cost < best) best = cost, sh.slab = slab, sh.shares = shares, sh.ring = ring;
-      }
+  for (int shares = 1; shares <= kMostShares && shares <= k_blocks; ++shares) {
+    const int64_t most = resident_ctas<kernel>(shares, kFewThreads, kFewSmem);
+    for (int slab = 128; slab >= 16; slab -= 8) {
+      const int64_t ctas = (int64_t)((a.N + slab - 1) / slab) * shares;
+      if (ctas > most) break;
+      const int64_t cost = (slab + sh.tokens) * ((k_blocks + shares - 1) / shares) + 8 * sh.tokens;
+      if (cost < best) best = cost, sh.slab = slab, sh.shares = shares;
     }
+  }
   if (best == INT64_MAX) {  // more slabs than run at the same time
     if (sh.tokens > 128) return best;
-    sh.slab = 128, sh.shares = 1, sh.ring = kFewHalfRing;
+    sh.slab = 128, sh.shares = 1;
     best = ((a.N + 127) / 128 + sms - 1) / sms * ((128 + sh.tokens) * (int64_t)k_blocks + 8 * sh.tokens);
   }
   // four blocks of K a stage, 512 consecutive bytes of each row, where at least four such stages fit
   const int block = (sh.slab + sh.tokens) * kBlock;
-  sh.blocks = 16 * block <= sh.ring ? 4 : 8 * block <= sh.ring ? 2 : 1;
-  sh.stages = sh.ring / (sh.blocks * block);
+  sh.blocks = 16 * block <= kFewRing ? 4 : 8 * block <= kFewRing ? 2 : 1;
+  sh.stages = kFewRing / (sh.blocks * block);
   if (sh.stages > kFewStagesMost) sh.stages = kFewStagesMost;
   sh.tmem_cols = 32;
   while (sh.tmem_cols < sh.tokens) sh.tmem_cols *= 2;
@@ -665,7 +663,7 @@ int launch_few(const Int8Args& a, const FewShape& sh, int32_t* status, cudaStrea
   const int slabs = (a.N + sh.slab - 1) / sh.slab;
   CUtensorMap ma, mw;
   RD_REQUIRE(rd_umma::make_byte_map(&ma, a.A, a.m_max, a.K, a.lda, sh.tokens) && rd_umma::make_byte_map(&mw, a.W, a.N, a.K, a.ldw, sh.slab), RD_ERR_ARG);
-  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)(slabs * sh.shares)), dim3(kFewThreads), few_smem(sh.ring), s, sh.shares, ma, mw, a, sh, status);
+  cudaError_t err = rd::launch_chained(kernel, dim3((unsigned)(slabs * sh.shares)), dim3(kFewThreads), kFewSmem, s, sh.shares, ma, mw, a, sh, status);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
@@ -730,13 +728,15 @@ int quant_rows(int dtype, const void* x, int64_t ldx, int8_t* codes, int64_t ld_
 
 template <typename OutT, int EPI>
 int product_of(const Int8Args& a, bool early, int32_t* status, cudaStream_t s) {
-  // The kernel for few tokens where its SMs bring in less (one B200, row quantiser included, us, few against many: 11008 x 4096, 256
-  // tokens 30 : 35; 4096 x 12288, 110 tokens 23 : 28, 256 tokens 33 : 28; 4096 x 22016, 200 tokens 55 : 36; 2048 x 4096, 200 tokens 12.6 : 9.2).
+  // The kernel for few tokens up to 32 of them, and where it is expected to be sooner done.  Times fit 4.6 us + 1.45 ns x cost for many tokens, 5.5 us + 2.05 ns
+  // x cost for few within a tenth (one B200, row quantiser included, us, few against many: 12288 x 4096 features, 40 tokens 16 : 18, 110 tokens 21 : 18, 256
+  // tokens 33 : 19; 22016 x 4096, 16 tokens 27 : 32, 110 tokens 41 : 27; 4096 x 11008, 110 tokens 18 : 24, 256 tokens 24 : 25; 2048 x 2048, 64 tokens 7.8 : 7.3).
   FewShape few;
   const ManyShape many = many_shape(a);
   constexpr auto few_kernel = int8_few_kernel<OutT, EPI>;
-  RD_REQUIRE(rd_quant::allow_smem<few_kernel>(few_smem(kFewRing)), RD_ERR_LAUNCH);
-  if (few_shape<few_kernel>(a, few) > many.cost) return launch_many<OutT, EPI>(a, many, status, s);
+  RD_REQUIRE(rd_quant::allow_smem<few_kernel>(kFewSmem), RD_ERR_LAUNCH);
+  const int64_t cost = few_shape<few_kernel>(a, few);
+  if (cost == INT64_MAX || (a.m_max > 32 && 10 * (cost + 450) > 7 * many.cost)) return launch_many<OutT, EPI>(a, many, status, s);
   few.early = early;
   return launch_few<OutT, EPI>(a, few, status, s);
 }
