@@ -272,6 +272,17 @@ __global__ void __launch_bounds__(kFewThreads)
     rd::pdl_wait();
     const int M = rd::live_rows(a.m_dev, a.m_max), quarter = warp & 3;
     const int row = quarter * 32 + lane;
+    const int each = (M + sh.shares - 1) / sh.shares, t_end = min(M, (share + 1) * each);
+    const int f = row0 + lane * 4;
+    const bool mine = lane * 4 < sh.slab && f < a.N;  // rows of the product past the slab are the next slab's
+    constexpr bool kGated = EPI == RD_EPI_SWIGLU;
+    constexpr int kOut = kGated ? 2 : 4;
+    const int col = kGated ? f / 2 : f, wide = kGated ? a.N / 2 : a.N;
+    const bool vec = col + kOut <= wide && ((uintptr_t)a.C % (kOut * sizeof(OutT))) == 0 && a.ldc % kOut == 0 &&
+                     (EPI != RD_EPI_RES || (((uintptr_t)a.R % (kOut * sizeof(OutT))) == 0 && a.ldr % kOut == 0));
+    if (EPI == RD_EPI_RES && mine)  // on their way from memory to L2 meanwhile
+      for (int t = share * each + quarter; t < t_end; t += 4)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"((const OutT*)a.R + (int64_t)t * a.ldr + min(col, wide - 1)) : "memory");
     ok = warp_wait(acc_full, 0, stop);
     if (!ok) site = 3;
     rd_umma::fence_after();
@@ -287,14 +298,7 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     if (sh.shares > 1) cluster_sync_part();
     else asm volatile("bar.sync 1, 128;" ::: "memory");
-    const int each = (M + sh.shares - 1) / sh.shares, t1 = ok ? min(M, (share + 1) * each) : 0;
-    const int f = row0 + lane * 4;
-    const bool mine = lane * 4 < sh.slab && f < a.N;  // rows of the product past the slab are the next slab's
-    constexpr bool kGated = EPI == RD_EPI_SWIGLU;
-    constexpr int kOut = kGated ? 2 : 4;
-    const int col = kGated ? f / 2 : f, wide = kGated ? a.N / 2 : a.N;
-    const bool vec = col + kOut <= wide && ((uintptr_t)a.C % (kOut * sizeof(OutT))) == 0 && a.ldc % kOut == 0 &&
-                     (EPI != RD_EPI_RES || (((uintptr_t)a.R % (kOut * sizeof(OutT))) == 0 && a.ldr % kOut == 0));
+    const int t1 = ok ? t_end : 0;
     float sw[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) sw[e] = mine && f + e < a.N ? a.w_scales[f + e] : 0.f;
