@@ -98,11 +98,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Rounds of row b: its tiles (at multiples of KEYS slots) over the warps of a CTA.
+// Rounds of row b: its tiles (at multiples of KEYS slots) over the warps of a CTA; one where there are new tokens and no keys, for the zeros that they get.
 template <int KEYS>
 __device__ __forceinline__ int rounds_of(const Args& a, int b) {
   const Row r = row_of(a, b);
-  if (r.n_new <= 0 || r.end <= 0) return 0;
+  if (r.n_new <= 0) return 0;
+  if (r.end <= 0) return 1;
   const int tiles = (int)((uint32_t)(r.first + r.end + KEYS - 1) / KEYS - (uint32_t)r.first / KEYS);
   return (tiles + kFewWarps - 1) / kFewWarps;
 }
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
       }
       const int j0 = (from + warp + i * kFewWarps) * kKeys - r.first;  // key of the tile's first slot
       const uint32_t kt = codes_u32 + stage * 2 * kTileBytes, pt = params_u32 + stage * 512;
-      if (j0 >= 0 && j0 + kKeys <= r.base) tile(std::true_type(), kt, pt, j0);
+      if (j0 >= 0 && j0 + kKeys <= min(r.base, r.end)) tile(std::true_type(), kt, pt, j0);
       else tile(std::false_type(), kt, pt, j0);
       __syncwarp();  // every lane has read its part of the stage
       if (i + kFewStages < mine && rd::elect_one()) load(i + kFewStages);

@@ -214,3 +214,59 @@ def test_captured_calls_side_by_side():
                 graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(one[1][1], one[2]) and torch.equal(two[1][1], two[2])
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", [(4, 2, 128, 1), (4, 2, 64, 2), (4, 2, 128, 40), (2, 2, 40, 3)])
+@pytest.mark.parametrize("most", [0, 1, 63, 200])
+def test_keys_past_the_bound_are_left_out(heads, kv, dim, new, most):
+    """Rows with more keys than max_kv says: the first max_kv are seen; without any the output is zero."""
+    base = [300, 250]
+    cache = rd.kv_cache.QuantizedCache(2, 400, 1, kv, dim, 4, DEV)
+    fill(cache, 0, most)
+    q = torch.randn(2 * new, heads * dim, device=DEV).to(BF16)
+    out = torch.full_like(q, 4.0)
+    cache.attend(0, q, out, i32(starts([new, new])), i32([0, 5]), i32(base), new, most)
+    if most == 0:
+        assert (out == 0).all()
+        return
+    nothing = np.zeros((2 * new, 1 + (new - 1) // 32), np.int32)
+    want, bound = attention(cache, 0, wide(q), starts([new, new]), [0, 5], [most, most], TREE, nothing, 1 / np.sqrt(dim), 2.0 ** -8)
+    assert (np.abs(wide(out) - want) <= bound + 2.0 ** -8 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("new, dim", [(1, 128), (3, 64), (40, 128), (2, 40)])
+def test_rows_that_begin_past_the_cache_have_no_keys(new, dim):
+    cache = rd.kv_cache.QuantizedCache(2, 128, 1, 2, dim, 8, DEV)
+    fill(cache, 0, 1)
+    q = torch.randn(2 * new, 4 * dim, device=DEV).to(BF16)
+    out = torch.full_like(q, 4.0)
+    cache.attend(0, q, out, i32(starts([new, new])), i32([128, 100000]), i32([7, 0]), new, 100)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("new, dim", [(3, 128), (40, 128), (40, 64), (3, 40)])
+def test_tokens_past_the_bound_are_left_alone(new, dim):
+    cache = rd.kv_cache.QuantizedCache(1, 128, 1, 2, dim, 8, DEV)
+    fill(cache, 0, 1)
+    q = torch.randn(new, 4 * dim, device=DEV).to(BF16)
+    some, all_ = torch.full_like(q, 4.0), torch.full_like(q, 4.0)
+    cache.attend(0, q, all_, i32([0, new]), i32([0]), i32([70]), new, 128)
+    cache.attend(0, q, some, i32([0, new]), i32([0]), i32([70]), new - 1, 128)
+    assert (some[new - 1] == 4.0).all() and (some[: new - 1] != 4.0).any()
+    assert (wide(some[: new - 1]) - wide(all_[: new - 1])).__abs__().max() <= 2.0 ** -6 * np.abs(wide(all_)).max()
+
+
+@pytest.mark.parametrize("bits, dim", [(4, 128), (8, 64)])
+@pytest.mark.parametrize("mode", [CAUSAL, TREE])
+def test_more_chains_than_multiprocessors(bits, dim, mode):
+    """An odd number of (row, head) chains, many of them without new tokens or with a second tile of query rows."""
+    rng = np.random.default_rng(dim)
+    new = [int(x) for x in rng.choice([0, 1, 17, 60, 128, 140, 150], 33)]
+    base = [int(x) for x in rng.integers(0, 200, 33)]
+    check(bits, BF16, 5, 5, dim, new, base, mode=mode, seed=4)
+
+
+def test_no_tokens():
+    cache = rd.kv_cache.QuantizedCache(2, 128, 1, 2, 64, 8, DEV)
+    q = torch.empty(0, 256, dtype=BF16, device=DEV)
+    cache.attend(0, q, torch.empty_like(q), i32([0, 0, 0]), i32([0, 0]), i32([7, 0]), 0, 100)
