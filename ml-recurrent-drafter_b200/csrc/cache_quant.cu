@@ -214,14 +214,17 @@ __global__ void __launch_bounds__(kThreads / 2) cache_quant_commit_kernel(uint8_
   rd::pdl_launch_dependents();
   rd::pdl_wait();
   const int b = blockIdx.y;
-  const int32_t* u = unpacker + ((int64_t)b * W + seq_in_beam[b]) * Lb;
-  const int64_t first = (((int64_t)blockIdx.z * B + b) * nkv + blockIdx.x) * max_len + kv_begin[b] + base_len[b];
+  const int seq = seq_in_beam[b];
+  const int64_t slot0 = (int64_t)kv_begin[b] + base_len[b];
+  if (seq < 0 || seq >= W || slot0 < 0) return;
+  const int32_t* u = unpacker + ((int64_t)b * W + seq) * Lb;
+  const int64_t first = (((int64_t)blockIdx.z * B + b) * nkv + blockIdx.x) * max_len + slot0, places = max_len - slot0;  // slots outside the cache do not exist
   const int n = n_accepted[b], w = threadIdx.x;
   if (w > row_words) return;
   uint32_t* rows = w < row_words ? reinterpret_cast<uint32_t*>(codes) + first * row_words + w : params + first;
   const int64_t step = w < row_words ? row_words : 1;
   for (int j = 0; j <= n && j < Lb; ++j)
-    if (u[j] != j) rows[j * step] = rows[u[j] * step];
+    if (u[j] > j && u[j] < places) rows[j * step] = rows[u[j] * step];
 }
 
 int check_layout(int bits, int B, int nkv, int hd, int max_len) {

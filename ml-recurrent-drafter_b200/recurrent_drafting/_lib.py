@@ -199,7 +199,7 @@ def check(rc: int, what: str) -> None:
 # kernels enqueued per entry point where that is not one; `launches` counts the kernels this process has enqueued
 # through call() (a replayed CUDA graph adds the number of kernels captured in it, see count_replay)
 KERNELS_PER_CALL = {"rd_tree_pack": 2, "rd_gemm_bf16_tc_argmax": 2, "rd_attention_tc_split": 2, "rd_attention_tc_masked_split": 2, "rd_cache_unpack": 2,
-                    "rd_cache_unpack_static": 2, "rd_mlstm_chunk": 3, "rd_mlstm_tree": 2}
+                    "rd_cache_unpack_static": 2, "rd_mlstm_chunk": 3, "rd_mlstm_tree": 2, "rd_linear_int8": 2}
 launches = 0
 
 

@@ -252,6 +252,8 @@ class QuantizedCache:
             q.data_ptr(), ldq if m > 1 else width, *self._planes[layer], out.data_ptr(), starts, begins, bases, mask,
             0 if workspace is None else workspace.data_ptr(), max(need, 0), 0 if status is None else status.data_ptr(),
             code, self.bits, m, B, nh, heads, hd, capacity, max_new, max_kv, mode, words, hd ** -0.5 if scale is None else scale), _lib.stream())
+        if need > 0:
+            _lib.launches += 1  # shares of keys are summed by a kernel of their own
 
     def commit_draft(self, fp, n_accepted: torch.Tensor, seq_in_beam: torch.Tensor, beam_shape, kv_begin: torch.Tensor) -> None:
         """Moves the accepted tokens of a packed draft behind the rows' prefixes, in all layers."""

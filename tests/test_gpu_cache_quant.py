@@ -169,3 +169,37 @@ def test_commit_moves_the_accepted_path(bits, dim):
                 for j in range(acc[b] + 1):
                     c0[b, :, s + j], p0[b, :, s + j] = c0[b, :, s + unpacker[b, seq[b], j]], p0[b, :, s + unpacker[b, seq[b], j]]
             assert np.array_equal(host(c), c0) and np.array_equal(host(p), p0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_read_of_long_rows(bits, dtype):
+    """Rows that take many steps of a thread block, next to short and empty ones."""
+    B, heads, dim, length, begin = 4, 8, 64, [6000, 1, 0, 4097], [3, 0, 9, 1900]
+    cache = new(B, 6016, 1, heads, dim, bits)
+    fill(cache, 0, 5)
+    k, v = (torch.full((B, heads, 6001, dim), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    cache.read(0, i32(begin), i32(length), k, v)
+    layer = cache.layers[0]
+    for codes, params, got in ((layer.k_codes, layer.k_params, k), (layer.v_codes, layer.v_params, v)):
+        c = codes if bits == 8 else torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2)
+        want = params[..., 0:1].contiguous().view(torch.bfloat16).float() * (c.float() - params[..., 1:2].float())  # exact
+        for b in range(B):
+            assert torch.equal(got[b, :, : length[b]], want[b, :, begin[b] : begin[b] + length[b]].to(dtype))
+            assert (got[b, :, length[b] :] == 7.0).all()
+
+
+def test_commit_stays_inside_the_cache():
+    """A path whose tokens would lie past the last slot, and a sequence that there is not: nothing moves."""
+    cache = new(2, 64, 1, 2, 64, 8)
+    fill(cache, 0, 1)
+    before = [(host(c), host(p)) for c, p in planes(cache, 0)]
+
+    class Pack:
+        pass
+
+    fp = Pack()
+    fp.base_len, fp.unpacker = i32([62, 5]), i32(np.tile([0, 3, 6], (2, 2, 1)).reshape(-1).tolist())
+    cache.commit_draft(fp, i32([2, 2]), i32([1, 2]), rd.modeling_drafter.BeamShape(2, 3), i32([0, 0]))
+    for (c, p), (c0, p0) in zip(planes(cache, 0), before):
+        assert np.array_equal(host(c), c0) and np.array_equal(host(p), p0)
