@@ -2,8 +2,7 @@
 // K = scale_k (code - zero_k), V likewise, a scale and a zero for each token of a head.
 //
 // attention_quant_rows_kernel: one CTA per (new token, head), for 32-bit queries and heads that the other kernels do not have.  A warp
-// takes 32 keys at a time, a key each for the scores, then all of them together for the values, a lane some features; running
-// maximum and sum in fp32.  The score is scale_k (q . code - zero_k sum q), the value's weight p scale_v.
+// takes 32 keys at a time, a lane one or two words of a row's codes; running maximum and sum in fp32, a lane a key.  The score is scale_k (q . code - zero_k sum q), the value's weight p scale_v.
 #include <atomic>
 
 #include <cuda_fp16.h>
@@ -15,7 +14,7 @@ namespace {
 
 using namespace rd_quant;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kMaxHd = 256;
 
 struct Args {
@@ -53,42 +52,62 @@ __device__ __forceinline__ bool sees(const Args& a, const Row& r, int i, int j) 
   return (jn >> 5) < a.mask_words && ((a.tree_mask[(int64_t)(r.start + i) * a.mask_words + (jn >> 5)] >> (jn & 31)) & 1u);
 }
 
-template <typename T, int BITS>
-__global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const Args a) {
-  __shared__ float q[kMaxHd], o[kWarps][kMaxHd], stats[kWarps][2];
+// W: words of codes that a lane holds of a row; `lanes` lanes (a power of two) hold a row, 32 / lanes rows at a time.
+template <typename T, int BITS, int W>
+__global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const Args a, int lanes) {
+  constexpr int kPer = 32 / BITS, kBatch = 8;  // codes of a word; loads of a lane that are on their way together
+  __shared__ float o[kWarps][kMaxHd], stats[kWarps][2];
   rd::pdl_launch_dependents();
   rd::pdl_wait();
   const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const Row r = row_of(a, b);
   if (i >= r.n_new) return;
   const int hd = a.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int words = hd / kPer, part = lane & (lanes - 1), at_once = 32 / lanes, group = lane / lanes;
   const T* from = (const T*)a.q + (int64_t)(r.start + i) * a.ldq + (int64_t)h * hd;
-  for (int d = threadIdx.x; d < hd; d += kWarps * 32) q[d] = rd::Num<T>::to_f(from[d]);
-  __syncthreads();
-  float q_sum = 0.f;
-  for (int d = lane; d < hd; d += 32) q_sum += q[d];
-  q_sum = rd::warp_sum(q_sum);
+  float q[W][kPer], q_sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      q[w][e] = part + 32 * w < words ? rd::Num<T>::to_f(from[(part + 32 * w) * kPer + e]) : 0.f;
+      q_sum += q[w][e];
+    }
+  for (int x = lanes >> 1; x > 0; x >>= 1) q_sum += __shfl_xor_sync(0xffffffffu, q_sum, x);
   const int64_t plane = ((int64_t)b * a.nkv + h / (a.nh / a.nkv)) * a.max_len + r.first;
-  const int row_bytes = hd * BITS / 8;
-  constexpr int kPer = 8 / BITS;  // codes of a byte
-  float m = -INFINITY, l = 0.f, acc[kMaxHd / 32] = {};
+  // words of keys (or values) s * at_once + group of 32 from j0 on, s from s0 on
+  auto load = [&](const uint8_t* codes, int j0, int s0, uint32_t (&u)[kBatch][W]) {
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int j = j0 + (s0 + x) * at_once + group;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        u[x][w] = s0 + x < lanes && j < r.end && part + 32 * w < words ? reinterpret_cast<const uint32_t*>(codes + (plane + j) * (hd * BITS / 8))[part + 32 * w] : 0u;
+    }
+  };
+  float m = -INFINITY, l = 0.f, acc[W][kPer] = {};
   for (int j0 = warp * 32; j0 < r.end; j0 += kWarps * 32) {
     const int j = j0 + lane;
     const bool seen = j < r.end && (j < r.base || sees(a, r, i, j));
-    float s = -INFINITY, sv = 0.f, zv = 0.f;
-    if (seen) {
-      const uint32_t pk = a.k_params[plane + j], pv = a.v_params[plane + j];
-      const uint8_t* k = a.k_codes + (plane + j) * row_bytes;
-      float dot = 0.f;
-      for (int w = 0; w < row_bytes / 4; ++w) {
-        const uint32_t u = reinterpret_cast<const uint32_t*>(k)[w];
+    const uint32_t pk = seen ? a.k_params[plane + j] : 0u, pv = seen ? a.v_params[plane + j] : 0u;
+    float mine = 0.f;  // q . codes of key j
+    uint32_t u[kBatch][W];
+    for (int s0 = 0; s0 < lanes; s0 += kBatch) {
+      load(a.k_codes, j0, s0, u);
 #pragma unroll
-        for (int e = 0; e < 4 * kPer; ++e) dot = fmaf(q[w * 4 * kPer + e], code_as_float((u >> (BITS * e)) & ((1u << BITS) - 1)), dot);
+      for (int x = 0; x < kBatch; ++x) {
+        float dot = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) dot = fmaf(q[w][e], code_as_float((u[x][w] >> (BITS * e)) & ((1u << BITS) - 1)), dot);
+        for (int y = lanes >> 1; y > 0; y >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, y);
+        dot = __shfl_sync(0xffffffffu, dot, (lane & (at_once - 1)) * lanes);
+        if (lane / at_once == s0 + x) mine = dot;
       }
-      s = (dot - (float)param_zero(pk) * q_sum) * param_scale(pk) * a.scale;
-      sv = param_scale(pv);
-      zv = (float)param_zero(pv);
     }
+    const float s = seen ? (mine - (float)param_zero(pk) * q_sum) * param_scale(pk) * a.scale : -INFINITY;
+    load(a.v_codes, j0, 0, u);  // under way while the weights are formed
     const bool any_nan = __any_sync(0xffffffffu, s != s);
     const float top = any_nan ? __int_as_float(0x7fffffff) : fmaxf(m, rd::warp_max(s));
     if (top == -INFINITY) continue;
@@ -96,24 +115,33 @@ __global__ void __launch_bounds__(kWarps * 32) attention_quant_rows_kernel(const
     const float p = seen ? expf(s - top) : 0.f;
     l = l * keep + rd::warp_sum(p);
     m = top;
-    const float pw = seen ? p * sv : 0.f;
+    const float pw = seen ? p * param_scale(pv) : 0.f, zv = (float)param_zero(pv);
 #pragma unroll
-    for (int c = 0; c < kMaxHd / 32; ++c) acc[c] *= keep;
-    const int n = min(32, r.end - j0);
-    for (int x = 0; x < n; ++x) {
-      const float w = __shfl_sync(0xffffffffu, pw, x), z = __shfl_sync(0xffffffffu, zv, x);
-      if (w == 0.f) continue;
-      const uint8_t* v = a.v_codes + (plane + j0 + x) * row_bytes;
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-      for (int c = 0; c < kMaxHd / 32; ++c) {
-        const int d = c * 32 + lane;
-        if (d < hd) acc[c] = fmaf(w, code_as_float((v[d / kPer] >> (BITS * (d % kPer))) & ((1u << BITS) - 1)) - z, acc[c]);
+      for (int e = 0; e < kPer; ++e) acc[w][e] *= keep;
+    for (int s0 = 0; s0 < lanes; s0 += kBatch) {
+      if (s0 > 0) load(a.v_codes, j0, s0, u);
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        const int key = (s0 + x) * at_once + group;  // past 31 where lanes < kBatch: nothing
+        const float weight = __shfl_sync(0xffffffffu, pw, key & 31), zero = __shfl_sync(0xffffffffu, zv, key & 31);
+        if (key > 31) continue;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[w][e] = fmaf(weight, code_as_float((u[x][w] >> (BITS * e)) & ((1u << BITS) - 1)) - zero, acc[w][e]);
       }
     }
   }
-  if (lane == 0) stats[warp][0] = m, stats[warp][1] = l;
 #pragma unroll
-  for (int c = 0; c < kMaxHd / 32; ++c) o[warp][c * 32 + lane] = acc[c];
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      for (int x = lanes; x < 32; x <<= 1) acc[w][e] += __shfl_xor_sync(0xffffffffu, acc[w][e], x);
+      if (group == 0 && part + 32 * w < words) o[warp][(part + 32 * w) * kPer + e] = acc[w][e];
+    }
+  if (lane == 0) stats[warp][0] = m, stats[warp][1] = l;
   __syncthreads();
   float top = -INFINITY;
   bool nan = false;
@@ -280,9 +308,17 @@ extern "C" int rd_attention_quant(const rd_attention_quant_desc* desc, void* str
   }
   const dim3 grid(max_new, nh, B);
   cudaError_t err;
-  auto run = [&](auto kern) { err = rd::launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
-  if (dtype == RD_BF16) bits == 4 ? run(attention_quant_rows_kernel<__nv_bfloat16, 4>) : run(attention_quant_rows_kernel<__nv_bfloat16, 8>);
-  else bits == 4 ? run(attention_quant_rows_kernel<float, 4>) : run(attention_quant_rows_kernel<float, 8>);
+  const int words = hd * bits / 32;
+  int lanes = 1;
+  while (lanes < words && lanes < 32) lanes *= 2;
+  auto run = [&](auto kern) { err = rd::launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a, lanes); };
+  auto pick = [&](auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    if (bits == 4) run(attention_quant_rows_kernel<T, 4, 1>);
+    else words <= 32 ? run(attention_quant_rows_kernel<T, 8, 1>) : run(attention_quant_rows_kernel<T, 8, 2>);
+  };
+  if (dtype == RD_BF16) pick((__nv_bfloat16*)nullptr);
+  else pick((float*)nullptr);
   RD_CHECK_CHAINED(err);
   return RD_OK;
 }
