@@ -19,6 +19,11 @@
 // (16 bytes of 8 keys) and of V (4 to 16 bytes of 4 keys) touch every bank once.
 //
 // Work is cut on the device, where the rows' lengths are known: chains (row, key/value head) in chunks of equal length.
+//
+// Measured on one B200: 16 rows of 105000 keys in all, 32 heads of 128 features with keys of their own, 8 bits, 138 us, 5.4 TB/s of codes (a copy reaches
+// 6.6): schedulers issue in 57 % of the cycles, the vector pipes are busy for 47, memory for 69.  One row of 131072 keys, 8 heads of 4 bits, four query heads
+// each: 42 us, 3.4 TB/s, of which some 8 until the first products and 3 for the sum of the chunks.  One row of 1001 keys: 9.6 us, trips to memory one
+// after another (lengths, codes, queries, chunks) and two launches.
 
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;

@@ -19,6 +19,12 @@
 // take the same order, the output undoes it.  QT = 2 unpacks half as often; with QT = 1 an SM works at two of these at once all the same.
 // With n_split > 1 a CTA walks its share of the tiles and leaves its sums for attention_quant_merge_shares_kernel.
 //
+// Measured on one B200: 2048 new tokens on 6144 before, 32 heads on 8 of 128, 8 bits, 302 us, 0.82 PFLOP/s (bf16 products of the library reach 1.64): a step of 256
+// rows and 64 keys takes some 2350 cycles, of which the tensor cores are busy for 42 % (products 1024 wide, with their operands' way through shared memory
+// 1280), exponentials for 42, shared memory for 71, and the last of 1.7 rounds of tiles leaves SMs idle.  Eight draft trees of 64 to 140 tokens on some 400, 32
+// heads, 4 bits: 31 us, ten steps of 1.3 us each, the way to the first of them and out of the last.  Tried and slower: tiles of 128 keys with one buffer of
+// scores (418 us), two tiles of rows taking turns (367); no different: scores of the next tile read before this one's weights are stored, 64 columns a load.
+//
 // Every wait is bounded; on give-up the kernel records a code in *status, frees its TMEM and returns.
 
 constexpr int kManyRows = 128, kManyKeys = 64;

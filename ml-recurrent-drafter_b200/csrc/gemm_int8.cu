@@ -11,8 +11,8 @@ namespace {
 
 
 // One block a row, 8 values of a thread at a time; rows of up to kQuantHeld * 8 * THREADS values stay in registers between the maximum and the
-// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows: these have blocks of 1024 threads.  VEC: rows on
-// 16-byte boundaries, K a multiple of 8.
+// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows: these have blocks of 1024 threads (one row of 4096 values 2.0 us, 110
+// of 11008 2.6, 4095 of 4096 19.5 us: 2.6 TB/s, its quotients' instructions).  VEC: rows on 16-byte boundaries, K a multiple of 8.
 
 template <bool Bits8>
 __device__ __forceinline__ uint32_t int8_code(float x, const rd_quant::Divider<Bits8>& by) {
@@ -180,7 +180,8 @@ __device__ __forceinline__ float gated(float gate, float up) {
 // of the weight, a share of K and all tokens; the weight rows ride the products' M, the tokens their N.  The CTAs of a slab are a
 // cluster: their sums, integers, meet in shared memory, and each finishes a part of the tokens.  In a chain that begins with the
 // row quantiser the first ring of weights is asked for before the codes of the tokens are there (`early`: the quantiser starts its
-// successors only when all before it is complete).
+// successors only when all before it is complete).  On one B200, quantiser included: one token x 12288 x 4096 13.7 us (3.7 TB/s of weights, some 3 us of them
+// before the first block of the tokens, 2 after the last product), 110 x 4096 x 11008 with a residual 19.3 us, 32000 x 4096 27.9 us (4.7 TB/s).
 constexpr int kFewTokens = 256, kMostShares = 8;
 constexpr int kFewRing = 200 * 1024, kFewStagesMost = 16, kFewThreads = 192;
 constexpr int kFewSmem = 1024 + kFewRing + 16 * 1024 /* a product reads 128 rows from a slab's first */ + 512;
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(kFewThreads)
 //   warp 1     of the leader: issues the products into one of two accumulators;
 //   warps 2-5  epilogue, a token to a lane: scales, gate; 32 output features at a time through shared memory, from where rows go out
 //              (and residual rows come in) in 16-byte pieces of consecutive addresses.
+// 4095 tokens x 22016 x 4096 with a gate on one B200: 199 us, 3.7 POP/s, the tensor cores busy for 95 % of the cycles.
 constexpr int kManyStages = 6, kManyThreads = 192, kTileTokens = 256, kMostWidth = 256;
 struct ManySmem {
   static constexpr int kTokens = 128 * kBlock, kFeatures = kMostWidth / 2 * kBlock;
