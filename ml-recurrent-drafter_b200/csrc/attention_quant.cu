@@ -227,9 +227,17 @@ ManyPlan many_plan(int dtype, int B, int nh, int nkv, int hd, int max_new, int m
   if (chains * ((rows + 2 * kManyRows - 1) / (2 * kManyRows)) >= rd_quant::sm_count() && rows > (B == 1 ? kManyRows : kManyRows * 3 / 2)) p.tiles = 2;
   // Shares of the keys where the query tiles leave CTAs idle: enough to fill two to an SM, each of at least four tiles of keys.
   const int64_t ctas = chains * ((rows + p.tiles * kManyRows - 1) / (p.tiles * kManyRows)), slots = 2 * rd_quant::sm_count() / p.tiles;
-  if (2 * ctas >= slots) return p;
-  const int64_t by_fill = slots / ctas, by_length = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys / 4;
+  const int64_t key_tiles = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys, by_fill = 2 * ctas < slots ? slots / ctas : 1, by_length = key_tiles / 4;
   int64_t n = by_fill < by_length ? by_fill : by_length;
+  // Of several rows one may be much longer than the others, which is not known here: then shares that would fill the SMs one and a half times, of at
+  // least twelve tiles, where rows have as many new tokens as the longest on average.  Four rows of 11 to 147 new tokens on 2 to 2554, 32 heads: 77 us
+  // in one piece, 50 in shares.  Twice as many shares cost more than they gave where rows are alike: 8 x 128 tokens on 4000, 143 us in one piece, 176 in two.
+  if (B > 1) {
+    int64_t expected = chains * rows / (p.tiles * kManyRows);
+    expected = expected < chains ? chains : expected;
+    const int64_t by_spread = 3 * slots / (2 * expected), spread = by_spread < key_tiles / 12 ? by_spread : key_tiles / 12;
+    n = n < spread ? spread : n;
+  }
   n = n < kManyMaxSplit ? n : kManyMaxSplit;
   p.n_split = n > 1 ? (int)n : 1;
   return p;
@@ -265,7 +273,7 @@ extern "C" int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m
   const FewPlan p = few_plan(dtype, bits, B, nh, nkv, hd, max_new, max_kv);
   if (p.rows && few_cut(p, B, nkv)) return kFewHeader + p.items * few_item_floats(hd, p.rows) * 4;
   const ManyPlan q = many_plan(dtype, B, nh, nkv, hd, max_new, max_kv);
-  if (q.here && q.n_split > 1) return (int64_t)m_max * nh * q.n_split * (hd + 2) * 4;
+  if (q.here && q.n_split > 1) return (int64_t)m_max * nh * q.n_split * (hd == 64 ? kShareFloats<64> : kShareFloats<128>) * 4;
   return 0;
 }
 

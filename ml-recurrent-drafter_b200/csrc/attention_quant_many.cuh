@@ -29,6 +29,8 @@
 
 constexpr int kManyRows = 128, kManyKeys = 64;
 constexpr int kManyMaxSplit = 16;
+template <int HD>
+constexpr int kShareFloats = HD + 4;  // of a share of a row: O, then maximum and sum; 16-byte pieces
 constexpr float kWeightBits = 7.f;        // weights are 2^7 p
 constexpr float kMostWeights = 32768.f;   // of a tile of a row: none is more, and fp16 holds it
 
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
     if (ok) {
       rd_umma::fence_after();
       const int64_t at = (int64_t)(r.start + token) * a.nh + head;
-      float* to = partial + (at * n_split + split) * (HD + 2);
+      float* to = partial + (at * n_split + split) * kShareFloats<HD>;
       const float f = n_split > 1 ? ref : (l_run == 0.f ? 0.f : ref / l_run);  // the weights' 2^7 is in O and in l
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
         if (!live) continue;
         if (n_split > 1) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(to + c * 32 + 2 * i) = make_float2(y[2 * i], y[2 * i + 1]);
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(to + c * 32 + 4 * i) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
         } else {
           uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + at * HD + c * 32);
 #pragma unroll
@@ -603,13 +605,13 @@ __global__ void __launch_bounds__(256) attention_quant_merge_shares_kernel(const
   const Row r = row_of(a, b);
   if (token >= r.n_new) return;
   const int64_t at = (int64_t)r.start * a.nh + unit;
-  const float* p = partial + at * n_split * (HD + 2);
-  const float mine = lane < n_split ? p[lane * (HD + 2) + HD] : -INFINITY;
+  const float* p = partial + at * n_split * kShareFloats<HD>;
+  const float mine = lane < n_split ? p[lane * kShareFloats<HD> + HD] : -INFINITY;
   const float top = rd::warp_max(mine);
   float sum = 0.f, v[HD / 32] = {};
 #pragma unroll 4
   for (int c = 0; c < n_split; ++c) {
-    const float* x = p + c * (HD + 2);
+    const float* x = p + c * kShareFloats<HD>;
     const float mc = x[HD], f = mc == -INFINITY ? 0.f : ex2(mc - top);
     sum += f * x[HD + 1];
 #pragma unroll
