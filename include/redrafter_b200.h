@@ -676,7 +676,8 @@ RD_API int rd_cache_quant_commit(int bits, uint8_t* codes, void* params, int pla
 
 /* Attention over such a cache: as rd_attention in modes RD_ATTN_CAUSAL and RD_ATTN_TREE (the new tokens' keys and values are in the
  * cache), with scores multiplied by `scale`.  q: head h of token t at q + t*ldq + h*hd; out [m_max, nh*hd], rows past the last new token
- * are left as they were.  A token that sees no key gets zeros.  max_len a multiple of 16; q, out and ldq 16-byte aligned.  max_new and
+ * are left as they were.  A token that sees no key gets zeros.  With 16-bit queries of heads of 64 or 128 features, weights, and for more than 16
+ * query rows to a key/value head keys and values too, are rounded to fp16's 11 bits; sums, maxima and scores are fp32.  max_len a multiple of 16; q, out and ldq 16-byte aligned.  max_new and
  * max_kv bound the new tokens of a row and its keys.  workspace: rd_attention_quant_workspace_bytes() of device memory, 16-byte aligned
  * (NULL if that is 0); calls that may run at the same time need one each. */
 RD_API int64_t rd_attention_quant_workspace_bytes(int dtype, int bits, int m_max, int B, int nh, int nkv, int hd, int max_new, int max_kv);

@@ -5,8 +5,6 @@
 // takes 32 keys at a time, a lane one or two words of a row's codes; running maximum and sum in fp32, a lane a key.  The score is scale_k (q . code - zero_k
 // sum q), the value's weight p scale_v.  Bound by its instructions (unpacking, and the sums over lanes): eight rows of 4096 keys, 32 heads on 8 of 128
 // features, fp32 queries take 357 us at 8 bits and 179 at 4 on one B200; one row of 300 keys, 8 heads of 64, 12 us.
-#include <atomic>
-
 #include <cuda_fp16.h>
 
 #include "quant.cuh"

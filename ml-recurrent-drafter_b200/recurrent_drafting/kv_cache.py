@@ -188,6 +188,8 @@ class QuantizedCache:
         tok, head = (s[0] if m > 1 else 0), (s[1] if heads > 1 else 0)
         if s[2] != 1 or u[2] != 1 or (m > 1 and u[0] != tok) or (heads > 1 and u[1] != head):
             raise _lib.RedrafterError("keys and values need the same strides, and their features one after another")
+        if m_dev is not None and m_dev.dtype is not torch.int32:
+            raise _lib.RedrafterError("m_dev is an int32 count")
         dev = self._on_device()
         if k.get_device() != dev or v.get_device() != dev or (m_dev is not None and m_dev.get_device() != dev):
             self._elsewhere(k=k, v=v, m_dev=m_dev)
@@ -228,6 +230,8 @@ class QuantizedCache:
         ldq, step = q.stride()
         if step != 1:
             raise _lib.RedrafterError("the features of a query lie one after another")
+        if status is not None and status.dtype is not torch.int32:
+            raise _lib.RedrafterError("status is int32")
         dev = self._on_device()
         if q.get_device() != dev or out.get_device() != dev or (status is not None and status.get_device() != dev):
             self._elsewhere(q=q, out=out, status=status)

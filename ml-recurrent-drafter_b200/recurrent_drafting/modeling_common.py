@@ -284,6 +284,8 @@ class Int8Linear:
         may be c).  Rows may lie any stride apart."""
         rows, width = a.shape
         m = rows if m_max is None else m_max
+        if (m_dev is not None and m_dev.dtype is not torch.int32) or (status is not None and status.dtype is not torch.int32):
+            raise _lib.RedrafterError("m_dev and status are int32")
         wide = self.out_features // 2 if epilogue == _lib.EPI_SWIGLU else self.out_features
         crows, cwidth = c.shape
         if rows < m or width != self.in_features or crows < m or cwidth != wide:

@@ -148,3 +148,17 @@ def test_workspace_sizes_are_host_calls():
     lib = _lib.load()
     assert lib.rd_attention_quant_workspace_bytes(1, 4, 1, 1, 32, 8, 128, 1, 100000) >= 0
     assert ctypes.c_int64(lib.rd_attention_quant_workspace_bytes(1, 7, 1, 1, 32, 8, 128, 1, 100000)).value < 0
+
+
+def test_counts_and_status_are_int32():
+    """Said before the device is looked at."""
+    cache = rd.kv_cache.QuantizedCache(1, 16, 1, 2, 64, 8, torch.device("cpu"))
+    k, index, wrong = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(_lib.RedrafterError, match="int32"):
+        cache.append(0, k, k, index, index, wrong)
+    with pytest.raises(_lib.RedrafterError, match="int32"):
+        cache.attend(0, k.reshape(3, 128), torch.zeros(3, 128), index, index, index, 3, 16, status=wrong)
+    linear = rd.modeling_common.Int8Linear.from_codes(torch.zeros(16, 64, dtype=torch.int8), torch.ones(16))
+    for kw in (dict(m_dev=wrong), dict(status=wrong)):
+        with pytest.raises(_lib.RedrafterError, match="int32"):
+            linear(torch.zeros(2, 64), torch.zeros(2, 16), **kw)
