@@ -427,9 +427,11 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
         float top = fmaxf(most, ref);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float back = ref / fmaxf(top, 0x1p-100f);
+        // not below 2^-112, so that its inverse stays finite; at that the weights of a value whose scale is 2^-126 are still p
+        top = fmaxf(top, 0x1p-112f);
+        const float back = ref / top;
         ref = top;
-        inv_ref = 16384.f / fmaxf(ref, 0x1p-100f);
+        inv_ref = 16384.f / ref;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float f[2];
