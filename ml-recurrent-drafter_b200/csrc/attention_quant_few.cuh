@@ -551,8 +551,7 @@ __global__ void __launch_bounds__(kFewThreads, NT == 1 ? 2 : 1)
           dst[g * (HD / 8) + 2 * k + 1] = o[n][k][2 + c] * kBack * ref;
         }
         if (g == 0) {
-          // A maximum of -inf says that there is nothing to add; scores that are all NaN leave it at that, too, and are to show
-          ss[(warp * kRows + row) * 2] = m[n][c] != -INFINITY ? m[n][c] * unit[n][c] : sum != sum ? 0.f : -INFINITY;
+          ss[(warp * kRows + row) * 2] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * unit[n][c];
           ss[(warp * kRows + row) * 2 + 1] = sum;
         }
       }

@@ -582,8 +582,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
           }
         }
       }
-      // a maximum of -inf: nothing to add; scores that are all NaN leave it at that, too, and are to show
-      if (n_split > 1 && live) to[HD] = m_run == -INFINITY && l_run != l_run ? 0.f : m_run, to[HD + 1] = l_run;
+      if (n_split > 1 && live) to[HD] = m_run, to[HD + 1] = l_run;
     }
   }
   if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 420 + site);
