@@ -93,6 +93,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
         self.gemm_status: Optional[torch.Tensor] = None
         self.cache_bits: Optional[int] = None  # of the caches that new_cache() makes; None: the model's type
         self._int8: Optional[Dict[str, List[Int8Linear]]] = None
+        self._int8_begun: Dict[str, List[Int8Linear]] = {}  # of a conversion that has not come to its end
         self._stage: Optional[Dict[str, torch.Tensor]] = None
 
     # ----------------------------------------------------------------- reference-compatible surface
@@ -128,16 +129,16 @@ class LlamaForCausalLM(LMHead, nn.Module):
     def hold_weights_in_int8(self) -> "LlamaForCausalLM":
         """Replaces the projections of all layers by 8-bit integers with a scale for each output feature, and gives their memory back; at
         each call the rows that they are applied to become 8-bit integers too.  Embedding, norms and the language-model head stay.  The weights
-        as they were are gone: the model can be neither saved nor moved afterwards, and load_state_dict() needs a new one."""
+        as they were are gone: the model can be neither saved nor moved afterwards, and load_state_dict() needs a new one.  A call that fails
+        on its way (no memory left) keeps what it has converted, and the next one goes on from there; until then the model does not run."""
         if self._int8 is None:
-            self._int8 = {}
-            self._linears = None
+            self._invalidate()  # nothing refers to a weight any more
             for name, weights in (("qkv", self.wqkv), ("o", self.wo), ("gu", self.wgu), ("down", self.wdown)):
-                self._int8[name] = []
-                for w in weights:
-                    self._int8[name].append(Int8Linear(w.detach()))
+                done = self._int8_begun.setdefault(name, [])
+                for w in list(weights)[len(done):]:
+                    done.append(Int8Linear(w.detach()))
                     w.data = torch.empty(0, dtype=w.dtype, device=w.device)
-            self._invalidate()
+            self._int8, self._int8_begun = self._int8_begun, {}
         return self
 
     def new_cache(self, batch_size: int, max_length: int, draft_tokens: int = 0, device=None) -> Union[kv_cache.Cache, kv_cache.QuantizedCache]:
@@ -241,7 +242,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
         return sd
 
     def _weights_as_they_were(self) -> None:
-        if self._int8 is not None:
+        if self._int8 is not None or any(self._int8_begun.values()):
             raise _lib.RedrafterError("the projections of this model are held in 8-bit integers: its weights cannot be loaded, saved or moved any more")
 
     def _apply(self, fn, *args, **kwargs):
@@ -314,6 +315,8 @@ class LlamaForCausalLM(LMHead, nn.Module):
 
     # ----------------------------------------------------------------- kernels
     def _lin(self):
+        if any(self._int8_begun.values()):
+            raise _lib.RedrafterError("hold_weights_in_int8() did not come to its end: call it again")
         if self._linears is None:
             self._linears = dict(self._int8, head=_Linear(self.lm_head.weight)) if self._int8 is not None else {
                 "qkv": [_Linear(w) for w in self.wqkv],

@@ -1,0 +1,59 @@
+"""What a Llama model in 8-bit integers can be asked for, and what is left of one whose conversion fails: runs without a GPU."""
+import pytest
+import torch
+from gpu_helpers import llama_config
+
+import recurrent_drafting as rd
+from recurrent_drafting import modeling_llama
+
+CONFIG = dict(hidden_size=32, num_attention_heads=2, num_key_value_heads=1, num_hidden_layers=2, intermediate_size=48, vocab_size=40, rms_norm_eps=1e-6,
+              rope_theta=10000.0)
+
+
+class Held:
+    """In the place of Int8Linear: refuses the calls after the first `left`."""
+
+    left = 0
+
+    def __init__(self, weight):
+        if Held.left == 0:
+            raise rd._lib.RedrafterError("no memory left")
+        Held.left -= 1
+        self.sum = float(weight.double().sum())
+
+
+def model():
+    return modeling_llama.LlamaForCausalLM(llama_config(CONFIG)).init_random(0.1, 3)
+
+
+def sums(llm):
+    return {name: [float(w.double().sum()) for w in ws] for name, ws in (("qkv", llm.wqkv), ("o", llm.wo), ("gu", llm.wgu), ("down", llm.wdown))}
+
+
+def test_a_refused_conversion_changes_nothing():
+    llm = model()
+    before = sums(llm)
+    for _ in range(2):
+        with pytest.raises(rd._lib.RedrafterError, match="CPU"):
+            llm.hold_weights_in_int8()
+    assert sums(llm) == before and len(llm._lin()["qkv"]) == 2
+    assert llm.to(torch.bfloat16).wqkv[1].dtype is torch.bfloat16
+    assert "model.layers.1.mlp.down_proj.weight" in llm.reference_state_dict()
+
+
+@pytest.mark.parametrize("first", [1, 3, 5, 7])
+def test_a_conversion_goes_on_where_it_failed(monkeypatch, first):
+    monkeypatch.setattr(modeling_llama, "Int8Linear", Held)
+    llm = model()
+    before = sums(llm)
+    Held.left = first
+    with pytest.raises(rd._lib.RedrafterError, match="memory"):
+        llm.hold_weights_in_int8()
+    for refused in (llm._lin, llm.reference_state_dict, lambda: llm.to(torch.bfloat16), lambda: llm.load_state_dict({})):
+        with pytest.raises(rd._lib.RedrafterError, match="hold_weights_in_int8|8-bit"):
+            refused()
+    Held.left = 8 - first  # each weight once
+    assert llm.hold_weights_in_int8() is llm and Held.left == 0
+    assert {name: [lin.sum for lin in lins] for name, lins in llm._lin().items() if name != "head"} == before
+    assert all(w.numel() == 0 for w in llm.wqkv) and all(w.numel() == 0 for w in llm.wdown)
+    assert llm.hold_weights_in_int8() is llm  # a second time changes nothing
