@@ -129,8 +129,9 @@ class LlamaForCausalLM(LMHead, nn.Module):
     def hold_weights_in_int8(self) -> "LlamaForCausalLM":
         """Replaces the projections of all layers by 8-bit integers with a scale for each output feature, and gives their memory back; at
         each call the rows that they are applied to become 8-bit integers too.  Embedding, norms and the language-model head stay.  The weights
-        as they were are gone: the model can be neither saved nor moved afterwards, and load_state_dict() needs a new one.  A call that fails
-        on its way (no memory left) keeps what it has converted, and the next one goes on from there; until then the model does not run."""
+        as they were are gone: the model can be neither saved nor moved afterwards, and load_state_dict() and init_random()
+        need a new one.  A call that fails on its way (no memory left) keeps what it has converted, and the next one goes on from there; until
+        then the model does not run."""
         if self._int8 is None:
             self._invalidate()  # nothing refers to a weight any more
             for name, weights in (("qkv", self.wqkv), ("o", self.wo), ("gu", self.wgu), ("down", self.wdown)):
@@ -162,6 +163,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
 
     def init_random(self, std: float = 0.02, seed: int = 0) -> "LlamaForCausalLM":
         """Random-init weights in place (normal(0, std); norm weights 1), on the current device."""
+        self._weights_as_they_were()
         g = torch.Generator(device=self.device).manual_seed(seed)
         for prm in self.parameters():
             if prm.ndim == 1:
@@ -222,6 +224,10 @@ class LlamaForCausalLM(LMHead, nn.Module):
         """config.json + model.safetensors with the HF names."""
         checkpoint.save_directory(path, self.config, self.reference_state_dict())
 
+    def state_dict(self, *args, **kwargs):
+        self._weights_as_they_were()
+        return super().state_dict(*args, **kwargs)
+
     def reference_state_dict(self) -> Dict[str, torch.Tensor]:
         """The weights under the HF / reference names."""
         self._weights_as_they_were()
@@ -243,7 +249,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
 
     def _weights_as_they_were(self) -> None:
         if self._int8 is not None or any(self._int8_begun.values()):
-            raise _lib.RedrafterError("the projections of this model are held in 8-bit integers: its weights cannot be loaded, saved or moved any more")
+            raise _lib.RedrafterError("the projections of this model are held in 8-bit integers: its weights cannot be set, loaded, saved or moved any more")
 
     def _apply(self, fn, *args, **kwargs):
         self._weights_as_they_were()

@@ -57,3 +57,21 @@ def test_a_conversion_goes_on_where_it_failed(monkeypatch, first):
     assert {name: [lin.sum for lin in lins] for name, lins in llm._lin().items() if name != "head"} == before
     assert all(w.numel() == 0 for w in llm.wqkv) and all(w.numel() == 0 for w in llm.wdown)
     assert llm.hold_weights_in_int8() is llm  # a second time changes nothing
+
+
+def held(monkeypatch):
+    monkeypatch.setattr(modeling_llama, "Int8Linear", Held)
+    Held.left = 8
+    return model().hold_weights_in_int8()
+
+
+def test_no_checkpoint_without_projections(monkeypatch):
+    """Also as a part of a larger module, and with weights made anew: the projections in integers would stay the old ones."""
+    llm = held(monkeypatch)
+    embedding = llm.model.embed_tokens.weight.clone()
+    both = torch.nn.ModuleDict({"llm": llm})
+    for refused in (llm.state_dict, both.state_dict, llm.init_random, lambda: llm.save_pretrained("/nonexistent")):
+        with pytest.raises(rd._lib.RedrafterError, match="8-bit"):
+            refused()
+    assert torch.equal(llm.model.embed_tokens.weight, embedding)
+    assert set(torch.nn.ModuleDict({"llm": model()}).state_dict()) >= {"llm.wqkv.0", "llm.lm_head.weight"}
