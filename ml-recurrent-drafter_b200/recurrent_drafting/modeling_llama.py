@@ -252,6 +252,11 @@ class LlamaForCausalLM(LMHead, nn.Module):
             raise _lib.RedrafterError("the projections of this model are held in 8-bit integers: its weights cannot be set, loaded, saved or moved any more")
 
     def _apply(self, fn, *args, **kwargs):
+        if self._int8 is not None:
+            # a move to where the model is, as a larger module makes it of all its parts; the smallest first, which show others at no cost
+            with torch.no_grad():
+                if all(fn(t) is t for t in sorted(self.parameters(), key=torch.numel)):
+                    return self
         self._weights_as_they_were()
         out = super()._apply(fn, *args, **kwargs)
         self._invalidate()

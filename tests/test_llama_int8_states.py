@@ -75,3 +75,17 @@ def test_no_checkpoint_without_projections(monkeypatch):
             refused()
     assert torch.equal(llm.model.embed_tokens.weight, embedding)
     assert set(torch.nn.ModuleDict({"llm": model()}).state_dict()) >= {"llm.wqkv.0", "llm.lm_head.weight"}
+
+
+def test_moves_that_change_nothing(monkeypatch):
+    """As RecurrentDrafting(llm, drafter).to(device) asks of a model that is there already."""
+    llm = held(monkeypatch)
+    drafter = rd.modeling_drafter.Drafter(rd.configuration_drafter.DrafterConfig(vocab_size=40, hidden_size=32, exit_dim=64, num_draft_layers=1, rnn=True))
+    both = rd.RecurrentDrafting(llm, drafter)
+    weights = [p.data_ptr() for p in llm.parameters()]
+    assert both.to("cpu") is both and both.float() is both and llm.to("cpu", torch.float32) is llm and llm.cpu() is llm
+    assert [p.data_ptr() for p in llm.parameters()] == weights and len(llm._lin()["qkv"]) == 2
+    for moved in (lambda: both.to(torch.bfloat16), lambda: llm.to("meta"), llm.double, lambda: llm.to_empty(device="cpu")):
+        with pytest.raises(rd._lib.RedrafterError, match="8-bit"):
+            moved()
+    assert [p.data_ptr() for p in llm.parameters()] == weights and llm.dtype is torch.float32
