@@ -499,10 +499,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int t0 = tile % t_tiles * kTileTokens + (int)rank * 128 + quarter * 32, f0 = tile / t_tiles * width;
       float* sw = s_scale + (local & 1) * kMostWidth;
       for (int i = threadIdx.x - 64; i < width; i += kEpiWarps * 32) sw[i] = f0 + i < a.N ? a.w_scales[f0 + i] : 0.f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
       const float sa = t0 + lane < M ? a.a_scales[t0 + lane] : 0.f;
       const int acc = local & 1;
-      if (!warp_wait(&acc_full[acc], (local >> 1) & 1, stop)) {
+      // the scales are there for all four warps, and they leave together
+      if (!rd::epilogue_agrees(warp_wait(&acc_full[acc], (local >> 1) & 1, stop))) {
         ok = false, site = 4;
         break;
       }

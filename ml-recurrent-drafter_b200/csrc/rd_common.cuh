@@ -192,6 +192,17 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Named barrier 1 of the four epilogue warps, which also tells each thread whether `ok` holds for all 128: warps that meet again at that barrier
+// go on, or leave, together.  (One that left by itself after a bounded wait would have the others wait for it without a bound.)
+__device__ __forceinline__ bool epilogue_agrees(bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.aligned.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(all)
+               : "r"((uint32_t)ok)
+               : "memory");
+  return all != 0;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster_x,
                                   Args&&... args) {
