@@ -146,7 +146,7 @@ __device__ __forceinline__ bool rows_epilogue(const EpiArgs& epi, const RowsShap
     asm volatile("bar.sync 1, 128;" ::: "memory");  // the staged entries are visible
     RopeRows cs;
     if (sh.rows == BM) cs.request(epi, s_pos, quarter, lane, 0, M, is_v);  // on its way while the products run
-    if (!mbar_wait(acc_full, on ^ 1, abort_flag)) return false;
+    if (!rd::epilogue_agrees(mbar_wait(acc_full, on ^ 1, abort_flag))) return false;  // the four warps meet again below
     tc_fence_after();
     if (sh.rows < BM) return true;  // the rest is the cluster's
 #pragma unroll 1
@@ -197,9 +197,9 @@ __device__ __forceinline__ bool rows_epilogue(const EpiArgs& epi, const RowsShap
         if (kRes && u < units && aligned && n_warp0 + 32 <= N) res.load(epi, u / groups * 32, kGlu<EPI> ? (n_warp0 >> 1) : n_warp0, M, lane);
       };
       prepare(quarter);
-      if (!mbar_wait(acc_full, on ^ 1, abort_flag)) return false;
+      const bool got = __all_sync(0xffffffffu, mbar_wait(acc_full, on ^ 1, abort_flag));
       tc_fence_after();
-      if (quarter * 16 < sh.rows) {
+      if (got && quarter * 16 < sh.rows) {
         const int f = quarter * 16 + lane;
 #pragma unroll 1
         for (int i = 0; i < units / groups; ++i) {
@@ -213,7 +213,7 @@ __device__ __forceinline__ bool rows_epilogue(const EpiArgs& epi, const RowsShap
           __syncwarp();
         }
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (!rd::epilogue_agrees(got)) return false;
 #pragma unroll 1
       for (int u = quarter; u < units; u += 4) {
         const int n_warp0 = row0 + 32 * (u % groups);

@@ -988,12 +988,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
           res_next.request(epi, tok_base, out0, tok_limit, lane, res_buf, 0u);
       }
-      if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag)) {
-        ok = false;
-        break;
-      }
+      // Where the four warps meet inside a tile they also give up together; then the staged entries are visible, too
+      ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+      if (EPI == kEpiQkvRope || norm_in || (kRes && !OUT_F32 && epi.gamma != nullptr)) ok = rd::epilogue_agrees(ok);
+      else ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
-      if (EPI == kEpiQkvRope || norm_in) asm volatile("bar.sync 1, 128;" ::: "memory");  // the staged entries are visible
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kMaxChunk;
 #pragma unroll 1
       for (int c = 0; c < cols; c += 32) {
@@ -1325,12 +1325,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
           res_next.request(epi, tok_base, out0, tok_limit, lane, res_buf, 0u);
       }
-      if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag)) {
-        ok = false;
-        break;
-      }
+      // Where the four warps meet inside a tile they also give up together; then the staged entries are visible, too
+      ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+      if (EPI == kEpiQkvRope || norm_in || (kRes && !OUT_F32 && epi.gamma != nullptr)) ok = rd::epilogue_agrees(ok);
+      else ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
-      if (EPI == kEpiQkvRope || norm_in) asm volatile("bar.sync 1, 128;" ::: "memory");  // the staged entries are visible
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kMaxChunk;
 #pragma unroll 1
       for (int c = 0; c < cols; c += 32) {

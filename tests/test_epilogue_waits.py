@@ -37,7 +37,7 @@ def left_alone(body):
     return [m.group(0) for m in re.finditer(r"if \(([^;{}]*wait[^;{}]*)\) \{[^{}]*\b(?:break|return)\b[^{}]*\}", body) if "epilogue_agrees(" not in m.group(1)]
 
 
-@pytest.mark.parametrize("name", ["gemm_int8.cu"])
+@pytest.mark.parametrize("name", ["gemm_int8.cu", "gemm_tc.cu"])
 def test_epilogue_warps_leave_a_loop_together(name):
     with open(os.path.join(CSRC, name)) as f:
         source = f.read()
