@@ -389,10 +389,10 @@ class LlamaForCausalLM(LMHead, nn.Module):
         self._drop_attn_plans()
 
     def _stage_of(self, m_max: int) -> Dict[str, torch.Tensor]:
-        """Where the keys and values of m_max new tokens lie between their projection and a cache in codes: [1, heads, m_max, head_dim] each, token t
-        at slot t of row 0."""
+        """Where the keys and values of at least m_max new tokens lie between their projection and a cache in codes: [1, heads, slots, head_dim] each,
+        token t at slot t of row 0.  One grow-only set, as workspace() keeps it: portions of other sizes neither allocate nor make other plans."""
         st = self._stage
-        if st is None or st["slot"].shape[0] != m_max:
+        if st is None or st["slot"].shape[0] < m_max:
             kv = dict(dtype=self.dtype, device=self.device)
             st = self._stage = {
                 "k": torch.empty(1, self.n_kv_heads, m_max, self.head_dim, **kv), "v": torch.empty(1, self.n_kv_heads, m_max, self.head_dim, **kv),
@@ -416,7 +416,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
             if mode == _lib.ATTN_DENSE:
                 raise _lib.RedrafterError("a cache in codes is attended to causally or through a prefix tree, not through an explicit mask")
             stage = self._stage_of(m_max)
-            row_of, slot_of, max_len = stage["row"], stage["slot"], m_max
+            row_of, slot_of, max_len = stage["row"], stage["slot"], stage["k"].shape[2]
         else:
             row_of, slot_of, max_len = tok_row, tok_slot, cache_tensor.shape[4]
         int8 = self._int8 is not None
@@ -475,7 +475,7 @@ class LlamaForCausalLM(LMHead, nn.Module):
                           _lib.ptr(tok_pos), _lib.ptr(slot_of), _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], m_max, md, nh, nkv,
                           hd, max_len, st)
             if codes is not None:
-                codes.append(l, kc[0].transpose(0, 1), vc[0].transpose(0, 1), tok_row, tok_slot, m_dev)
+                codes.append(l, kc[0, :, :m_max].transpose(0, 1), vc[0, :, :m_max].transpose(0, 1), tok_row, tok_slot, m_dev)
                 codes.attend(l, q, attn, row_start, kv_begin, base_len, max_new, max_kv, mode, tree_mask, status=self.gemm_status)
             else:
                 self._attention(code, q, kc, vc, attn, row_start, kv_begin, base_len, batch, m_max, max_new, max_kv, mode, tree_mask,
