@@ -134,12 +134,23 @@ class QuantizedCache:
         capacity = (max_length + self.SLOTS - 1) // self.SLOTS * self.SLOTS
         self._codes = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, head_dim * bits // 8, dtype=torch.uint8, device=device)
         self._params = torch.zeros(n_layers, 2, batch_size, n_heads, capacity, 2, dtype=torch.int16, device=device)
-        self.layers = [LayerCodes(c[0], p[0], c[1], p[1]) for c, p in zip(self._codes, self._params)]
-        # what every call needs of them
-        self._planes = [tuple(t.data_ptr() for t in l) for l in self.layers]
         self._shape = (batch_size, n_heads, capacity, head_dim)
-        self._device: int = self._codes.get_device()
         self._workspace_bytes: Dict[Tuple, int] = {}
+        self._describe()
+
+    def _describe(self) -> None:
+        """What every call needs of the storage: layers, addresses, device."""
+        self.layers = [LayerCodes(c[0], p[0], c[1], p[1]) for c, p in zip(self._codes, self._params)]
+        self._planes = [tuple(t.data_ptr() for t in l) for l in self.layers]
+        self._device: int = self._codes.get_device()
+
+    # copies (copy.deepcopy, pickle) have storage, and so addresses, of their own
+    def __getstate__(self) -> Dict:
+        return {k: v for k, v in self.__dict__.items() if k not in ("layers", "_planes", "_device")}
+
+    def __setstate__(self, state: Dict) -> None:
+        self.__dict__.update(state)
+        self._describe()
 
     @property
     def storage(self) -> "QuantizedCache":

@@ -275,6 +275,13 @@ class Int8Linear:
         # what every call needs of them
         self._k16, self._codes_ptr, self._scales_ptr, self._device = codes.shape[1], codes.data_ptr(), scales.data_ptr(), codes.get_device()
 
+    # copies (copy.deepcopy, pickle) have codes, and so addresses, of their own
+    def __getstate__(self):
+        return self.codes, self.scales, self.in_features
+
+    def __setstate__(self, state) -> None:
+        self._hold(*state)
+
     def drop_plans(self) -> None:
         """Nothing is kept between calls."""
 
