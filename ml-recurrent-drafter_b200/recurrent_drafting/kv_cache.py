@@ -199,7 +199,7 @@ class QuantizedCache:
         tok, head = (s[0] if m > 1 else 0), (s[1] if heads > 1 else 0)
         if s[2] != 1 or u[2] != 1 or (m > 1 and u[0] != tok) or (heads > 1 and u[1] != head):
             raise _lib.RedrafterError("keys and values need the same strides, and their features one after another")
-        if m_dev is not None and m_dev.dtype is not torch.int32:
+        if m_dev is not None and (m_dev.dtype is not torch.int32 or m_dev.numel() < 1):
             raise _lib.RedrafterError("m_dev is an int32 count")
         dev = self._on_device()
         if k.get_device() != dev or v.get_device() != dev or (m_dev is not None and m_dev.get_device() != dev):
@@ -241,8 +241,8 @@ class QuantizedCache:
         ldq, step = q.stride()
         if step != 1:
             raise _lib.RedrafterError("the features of a query lie one after another")
-        if status is not None and status.dtype is not torch.int32:
-            raise _lib.RedrafterError("status is int32")
+        if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
+            raise _lib.RedrafterError("status is an int32 number")
         dev = self._on_device()
         if q.get_device() != dev or out.get_device() != dev or (status is not None and status.get_device() != dev):
             self._elsewhere(q=q, out=out, status=status)
@@ -273,11 +273,17 @@ class QuantizedCache:
     def commit_draft(self, fp, n_accepted: torch.Tensor, seq_in_beam: torch.Tensor, beam_shape, kv_begin: torch.Tensor) -> None:
         """Moves the accepted tokens of a packed draft behind the rows' prefixes, in all layers."""
         n_layers, _, B, heads, capacity, _ = self._codes.shape
+        W, L = beam_shape.width, beam_shape.length
+        unpacker = fp.unpacker
+        if unpacker.dtype is not torch.int32 or unpacker.numel() < B * W * L or not unpacker.is_contiguous():
+            raise _lib.RedrafterError(f"unpacker is a contiguous int32 tensor of {B} * {W} * {L} elements")
+        if unpacker.get_device() != self._device:
+            self._elsewhere(unpacker=unpacker)
+        begin, base, accepted, seq = (self._index(name, t, B) for name, t in (("kv_begin", kv_begin), ("base_len", fp.base_len),
+                                                                             ("n_accepted", n_accepted), ("seq_in_beam", seq_in_beam)))
         self._on_device()
-        self._elsewhere(kv_begin=kv_begin, n_accepted=n_accepted, seq_in_beam=seq_in_beam)
-        _lib.call("rd_cache_quant_commit", self.bits, _lib.ptr(self._codes), _lib.ptr(self._params), 2 * n_layers, B, heads, capacity, self.head_dim,
-                  _lib.ptr(kv_begin), _lib.ptr(fp.base_len), _lib.ptr(fp.unpacker), beam_shape.width, beam_shape.length, _lib.ptr(n_accepted),
-                  _lib.ptr(seq_in_beam), _lib.stream())
+        _lib.call("rd_cache_quant_commit", self.bits, self._codes.data_ptr(), self._params.data_ptr(), 2 * n_layers, B, heads, capacity, self.head_dim,
+                  begin, base, unpacker.data_ptr(), W, L, accepted, seq, _lib.stream())
 
 
 @dataclass(frozen=True)

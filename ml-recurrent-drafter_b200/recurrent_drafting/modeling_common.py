@@ -291,8 +291,9 @@ class Int8Linear:
         may be c).  Rows may lie any stride apart."""
         rows, width = a.shape
         m = rows if m_max is None else m_max
-        if (m_dev is not None and m_dev.dtype is not torch.int32) or (status is not None and status.dtype is not torch.int32):
-            raise _lib.RedrafterError("m_dev and status are int32")
+        if (m_dev is not None and (m_dev.dtype is not torch.int32 or m_dev.numel() < 1)) or (
+                status is not None and (status.dtype is not torch.int32 or status.numel() < 1)):
+            raise _lib.RedrafterError("m_dev and status are int32 numbers")
         wide = self.out_features // 2 if epilogue == _lib.EPI_SWIGLU else self.out_features
         crows, cwidth = c.shape
         if rows < m or width != self.in_features or crows < m or cwidth != wide:
@@ -331,8 +332,10 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, m_
         raise _lib.RedrafterError(f"codes: contiguous int8 [{m}, a multiple of 16 from {k} on] is wanted")
     if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] < m or not scales.is_contiguous() or (k > 1 and x.stride(1) != 1):
         raise _lib.RedrafterError("scales: contiguous fp32, one for each row; the values of a row lie one after another")
-    if x.is_cuda and (x.device != codes.device or x.device != scales.device or x.device.index != torch._C._cuda_getDevice()):
-        raise _lib.RedrafterError("rows, codes and scales lie on the current device")
+    if m_dev is not None and (m_dev.dtype is not torch.int32 or m_dev.numel() < 1):
+        raise _lib.RedrafterError("m_dev is an int32 count")
+    if x.is_cuda and (any(t is not None and t.device != x.device for t in (codes, scales, m_dev)) or x.device.index != torch._C._cuda_getDevice()):
+        raise _lib.RedrafterError("rows, codes, scales and m_dev lie on the current device")
     _lib.call("rd_quant_rows", _lib.dtype_code(x.dtype), _lib.ptr(x), x.stride(0) if m > 1 else k, _lib.ptr(codes), codes.shape[1], _lib.ptr(scales), m,
               _lib.ptr(m_dev), k, _lib.stream())
 
