@@ -9,7 +9,7 @@
 //               over a power of two, fp16, into swizzled shared-memory tiles of 64 keys, two or four stages each for K and V.  For keys that power
 //               is of the tile and goes into the scores' unit; for values it is r, that of the largest scale so far;
 //   QT warps    issue S = Q K^T (both from shared memory) and O += W V (W from TMEM, V as an MN-major operand).
-// Keys, values and weights are thus rounded to fp16's 11 bits, each by at most 2^-12 of itself, an eighth of what a bf16 cache costs.  With the
+// Keys, values and weights are thus rounded to fp16's 11 bits, each by at most 2^-11 of itself, an eighth of what a bf16 cache costs.  With the
 // scales left to the softmax instead (codes alone are exact) its 64 x 128 scores cost four instructions for two where they now take
 // two and a half, which bounded the kernel: a tile of 256 rows 2560 cycles.
 // S has two buffers, W of a tile takes the place of its S: QK of the next two tiles run under the softmax of this one.  A tile is read from TMEM once,
