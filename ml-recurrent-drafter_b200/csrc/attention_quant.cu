@@ -228,13 +228,16 @@ ManyPlan many_plan(int dtype, int B, int nh, int nkv, int hd, int max_new, int m
   const int64_t key_tiles = ((int64_t)max_kv + kManyKeys - 1) / kManyKeys, by_fill = 2 * ctas < slots ? slots / ctas : 1, by_length = key_tiles / 4;
   int64_t n = by_fill < by_length ? by_fill : by_length;
   // Of several rows one may be much longer than the others, which is not known here: then shares that would fill the SMs one and a half times, of at
-  // least twelve tiles, where rows have as many new tokens as the longest on average.  Four rows of 11 to 147 new tokens on 2 to 2554, 32 heads: 77 us
-  // in one piece, 50 in shares.  Twice as many shares cost more than they gave where rows are alike: 8 x 128 tokens on 4000, 143 us in one piece, 176 in two.
+  // least twelve tiles, where rows have as many new tokens as the longest on average; a multiple of those above, so that rows that are alike take
+  // whole rounds.  This pays where rows differ and costs where they do not (one B200, 32 heads on 8 of 128, 8 bits, us, with these shares against only those
+  // that fill the SMs): 11 to 147 new tokens on 2 to 2554 49 : 93, 5 to 147 on 30 to 6000 85 : 197, 64 and 200 on 4000 and 100 53 : 84; but 4 x 128 on 3968 in
+  // four shares 106, in two 89 (in three 125: two rounds of a third), 2 x 128 on 8000 110 : 88, 8 x 128 on 3872 139 either way.
   if (B > 1) {
     int64_t expected = chains * rows / (p.tiles * kManyRows);
     expected = expected < chains ? chains : expected;
-    const int64_t by_spread = 3 * slots / (2 * expected), spread = by_spread < key_tiles / 12 ? by_spread : key_tiles / 12;
-    n = n < spread ? spread : n;
+    const int64_t by_spread = 3 * slots / (2 * expected), most = key_tiles / 12, spread = by_spread < most ? by_spread : most;
+    const int64_t rounded = (spread + by_fill - 1) / by_fill * by_fill;
+    if (n < spread && rounded <= most) n = rounded;
   }
   n = n < kManyMaxSplit ? n : kManyMaxSplit;
   p.n_split = n > 1 ? (int)n : 1;
