@@ -75,18 +75,6 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
   return y;
 }
-__device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  if (rd_umma::mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (;;) {
-    if (rd_umma::mbar_try(bar, parity)) return true;
-    if (*stop || clock64() - t0 > (1ll << 31)) return false;
-  }
-}
-// by all lanes of a warp, the same answer for all
-__device__ __forceinline__ bool warp_wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  return __all_sync(0xffffffffu, mbar_wait_or(bar, parity, stop));
-}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(rd_umma::smem_u32(bar)) : "memory");
 }
@@ -279,7 +267,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
     auto unpack = [&](int t, auto set) {
       constexpr int S = decltype(set)::value;
       const int st = t % kSt;
-      if (t >= kSt && !warp_wait_or(&k_empty[st], (t / kSt - 1) & 1, stop)) {
+      if (t >= kSt && !rd_umma::warp_wait(&k_empty[st], (t / kSt - 1) & 1, stop)) {
         ok = false, site = 1;
         return;
       }
@@ -301,7 +289,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
       rd_umma::fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[st]);
-      if (t >= kSt && !warp_wait_or(&v_empty[st], (t / kSt - 1) & 1, stop)) {
+      if (t >= kSt && !rd_umma::warp_wait(&v_empty[st], (t / kSt - 1) & 1, stop)) {
         ok = false, site = 2;
         return;
       }
@@ -332,7 +320,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
       // S of tile t: its buffer held W of tile t - 2, whose product has been issued before; products run in that order
       auto scores = [&](int t) {
         const int st = t % kSt;
-        if (!mbar_wait_or(&k_full[st], (t / kSt) & 1, stop)) return false;
+        if (!rd_umma::wait_or(&k_full[st], (t / kSt) & 1, stop)) return false;
         rd_umma::fence_after();
         const uint32_t k = rd_umma::smem_u32(sK + st * L::kTile);
 #pragma unroll
@@ -344,11 +332,11 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
         rd_umma::commit(&k_empty[st]);
         return true;
       };
-      ok = mbar_wait_or(&q_full[x], 0, stop);
+      ok = rd_umma::wait_or(&q_full[x], 0, stop);
       for (int t = 0; ok && t < 2 && t < n_tiles; ++t) ok = scores(t);
       for (int t = 0; ok && t < n_tiles; ++t) {
         const int st = t % kSt;
-        ok = mbar_wait_or(&p_full[2 * x + (t & 1)], (t >> 1) & 1, stop) && mbar_wait_or(&v_full[st], (t / kSt) & 1, stop);
+        ok = rd_umma::wait_or(&p_full[2 * x + (t & 1)], (t >> 1) & 1, stop) && rd_umma::wait_or(&v_full[st], (t / kSt) & 1, stop);
         if (!ok) break;
         rd_umma::fence_after();
         const uint32_t v = rd_umma::smem_u32(sV + st * L::kTile);
@@ -477,7 +465,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
       return top;
     };
     for (int t = 0; t < n_tiles; ++t) {
-      if (!warp_wait_or(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
+      if (!rd_umma::warp_wait(&s_full[2 * tile + (t & 1)], (t >> 1) & 1, stop)) {
         ok = false, site = 4;
         break;
       }
@@ -524,7 +512,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
         ref = ref_t;
         if (t == 0) continue;
         // O has to be quiet
-        if (!warp_wait_or(&o_full[2 * tile + ((t - 1) & 1)], ((t - 1) >> 1) & 1, stop)) {
+        if (!rd_umma::warp_wait(&o_full[2 * tile + ((t - 1) & 1)], ((t - 1) >> 1) & 1, stop)) {
           ok = false, site = 5;
           break;
         }
@@ -548,7 +536,7 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
       if (lane == 0) mbar_arrive(&p_full[2 * tile + (t & 1)]);
     }
     if (ok && n_tiles > 0) {
-      ok = warp_wait_or(&o_full[2 * tile + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, stop);
+      ok = rd_umma::warp_wait(&o_full[2 * tile + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, stop);
       if (!ok) site = 6;
     }
     if (ok) {

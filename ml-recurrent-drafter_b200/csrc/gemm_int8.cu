@@ -133,18 +133,6 @@ __device__ __forceinline__ void mma_int8(uint32_t d, uint64_t a, uint64_t b, uin
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  if (rd_umma::mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (;;) {
-    if (rd_umma::mbar_try(bar, parity)) return true;
-    if (*stop || clock64() - t0 > (1ll << 31)) return false;
-  }
-}
-// by all lanes of a warp, the same answer for all
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  return __all_sync(0xffffffffu, wait_or(bar, parity, stop));
-}
 __device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int* v) {
   float f[32];
   rd_umma::tmem_ld32(taddr, f);
@@ -239,7 +227,7 @@ __global__ void __launch_bounds__(kFewThreads)
       if (sh.early) rd::pdl_wait();
       for (int i = 0; i < ahead; ++i) load(i, false);
       for (int i = ahead; i < steps; ++i) {
-        if (!wait_or(&empty[i % sh.stages], (i / sh.stages - 1) & 1, stop)) {
+        if (!rd_umma::wait_or(&empty[i % sh.stages], (i / sh.stages - 1) & 1, stop)) {
           ok = false, site = 1;
           break;
         }
@@ -254,7 +242,7 @@ __global__ void __launch_bounds__(kFewThreads)
       const uint32_t idesc = int8_idesc(128, max(16, (M + 15) / 16 * 16));
       for (int i = 0; i < steps; ++i) {
         const int s = i % sh.stages, n = min(sh.blocks, k_blocks - i * sh.blocks);
-        if (!wait_or(&full[s], (i / sh.stages) & 1, stop)) {
+        if (!rd_umma::wait_or(&full[s], (i / sh.stages) & 1, stop)) {
           ok = false, site = 2;
           break;
         }
@@ -284,7 +272,7 @@ __global__ void __launch_bounds__(kFewThreads)
     if (EPI == RD_EPI_RES && mine)  // on their way from memory to L2 meanwhile
       for (int t = share * each + quarter; t < t_end; t += 4)
         asm volatile("prefetch.global.L2 [%0];" ::"l"((const OutT*)a.R + (int64_t)t * a.ldr + min(col, wide - 1)) : "memory");
-    ok = warp_wait(acc_full, 0, stop);
+    ok = rd_umma::warp_wait(acc_full, 0, stop);
     if (!ok) site = 3;
     rd_umma::fence_after();
     // Sums go to shared memory, [token][128 features], where the ring was; then a warp takes a token at a time, a lane four features.  Short
@@ -448,7 +436,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       for (int tile = pair; ok && tile < tiles; tile += n_pairs) {
         const int t0 = tile % t_tiles * kTileTokens + (int)rank * 128, f0 = tile / t_tiles * width + (int)rank * (width / 2);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!wait_or(&empty[stage], phase ^ 1, stop)) {
+          if (!rd_umma::wait_or(&empty[stage], phase ^ 1, stop)) {
             ok = false, site = 1;
             break;
           }
@@ -467,13 +455,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       uint32_t phase = 0;
       for (int tile = pair; ok && tile < tiles; tile += n_pairs, ++local) {
         const int acc = local & 1;
-        if (!wait_or(&acc_empty[acc], ((local >> 1) & 1) ^ 1, stop)) {
+        if (!rd_umma::wait_or(&acc_empty[acc], ((local >> 1) & 1) ^ 1, stop)) {
           ok = false, site = 2;
           break;
         }
         rd_umma::fence_after();
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!wait_or(&full[stage], phase, stop)) {
+          if (!rd_umma::wait_or(&full[stage], phase, stop)) {
             ok = false, site = 3;
             break;
           }
@@ -502,7 +490,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const float sa = t0 + lane < M ? a.a_scales[t0 + lane] : 0.f;
       const int acc = local & 1;
       // the scales are there for all four warps, and they leave together
-      if (!rd::epilogue_agrees(warp_wait(&acc_full[acc], (local >> 1) & 1, stop))) {
+      if (!rd::epilogue_agrees(rd_umma::warp_wait(&acc_full[acc], (local >> 1) & 1, stop))) {
         ok = false, site = 4;
         break;
       }

@@ -32,6 +32,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     if (clock64() - t0 > (1ll << 31)) return false;
   }
 }
+// the same, given up early where another role has set *stop
+__device__ __forceinline__ bool wait_or(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (mbar_try(bar, parity)) return true;
+    if (*stop || clock64() - t0 > (1ll << 31)) return false;
+  }
+}
+// by all lanes of a warp, the same answer for all
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, wait_or(bar, parity, stop));
+}
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
