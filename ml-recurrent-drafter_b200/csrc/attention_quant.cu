@@ -4,7 +4,8 @@
 // attention_quant_rows_kernel: one CTA per (new token, head), for 32-bit queries and heads that the other kernels do not have.  A warp
 // takes 32 keys at a time, a lane one or two words of a row's codes; running maximum and sum in fp32, a lane a key.  The score is scale_k (q . code - zero_k
 // sum q), the value's weight p scale_v.  Bound by its instructions (unpacking, and the sums over lanes): eight rows of 4096 keys, 32 heads on 8 of 128
-// features, fp32 queries take 357 us at 8 bits and 179 at 4 on one B200; one row of 300 keys, 8 heads of 64, 12 us.
+// features, fp32 queries take 322 us at 8 bits and 181 at 4 on one B200; one row of 300 keys, 8 heads of 64, 12 us.  Keys are never cut, and the
+// query heads of a group unpack the same codes each: one row of 131072 keys takes 6.9 ms, a prompt of 512 tokens 1.1.
 #include <cuda_fp16.h>
 
 #include "quant.cuh"

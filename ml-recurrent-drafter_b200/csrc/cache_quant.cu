@@ -97,8 +97,8 @@ struct Planes {
 };
 
 // A unit is one head of one token, its key and its value, by hd / VEC lanes (rounded up to a power of two).  Bound by memory for fp32 rows (20235 tokens of
-// 8 heads of 128 at 8 bits: 38 us, 5.5 TB/s) and by instructions for bf16 ones (31.5 us, 4.0 TB/s; at 4 bits 30): two a quotient, one for its cut, one to
-// put its code in place.  CTAs that go through several units each with the next one's rows under way: 63 to 125 us instead of 57, appended and read.
+// 8 heads of 128 at 8 bits: 38 us, 5.5 TB/s) and by instructions for bf16 ones (31.5 us, 4.0 TB/s; at 4 bits 30; issue slots 74 %, the integer pipe 60, memory
+// 34): two a quotient, one for its cut, one to put its code in place.  CTAs that go through several units each with the next one's rows under way: 63 to 125 us instead of 57, appended and read.
 template <typename T, int BITS, int VEC>
 __global__ void __launch_bounds__(kThreads) cache_quant_append_kernel(const T* k, const T* v, int64_t tok_stride, int64_t head_stride, Planes to,
                                                                       const int32_t* tok_row, const int32_t* tok_slot, int m_max,

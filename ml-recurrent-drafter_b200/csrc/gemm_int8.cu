@@ -11,8 +11,9 @@ namespace {
 
 
 // One block a row, 8 values of a thread at a time; rows of up to kQuantHeld * 8 * THREADS values stay in registers between the maximum and the
-// codes, what is longer is read again.  Bound by memory, or by a trip to it for a few rows: these have blocks of 1024 threads (one row of 4096 values 2.0 us, 110
-// of 11008 2.6, 4095 of 4096 19.5 us: 2.6 TB/s, its quotients' instructions).  VEC: rows on 16-byte boundaries, K a multiple of 8.
+// codes, what is longer is read again.  A few rows are bound by a trip to memory: these have blocks of 1024 threads (one row of 4096 values 2.0 us, 110
+// of 11008 2.6).  Many are bound by how little is asked for at once: what is held, as fp32, takes 89 registers a thread, so that two blocks are on an SM (4095 of
+// 4096 values 19.5 us, 2.6 TB/s: issue slots 40 %, memory 14, warps wait for their loads).  VEC: rows on 16-byte boundaries, K a multiple of 8.
 
 template <bool Bits8>
 __device__ __forceinline__ uint32_t int8_code(float x, const rd_quant::Divider<Bits8>& by) {

@@ -187,8 +187,8 @@ class QuantizedCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, tok_row: torch.Tensor, tok_slot: torch.Tensor,
                m_dev: Optional[torch.Tensor] = None) -> None:
-        """Writes the keys and values [tokens, heads, head_dim] of new tokens (bf16 or fp32; any strides of tokens and heads, the same in
-        both) to slots tok_slot of batch rows tok_row.  Two tokens must not have the same place."""
+        """Writes the keys and values [tokens, heads, head_dim] of new tokens (bf16 or fp32; tokens and heads any multiples of 16 bytes
+        apart, the same in both) to slots tok_slot of batch rows tok_row.  Two tokens must not have the same place."""
         B, heads, capacity, hd = self._shape
         dims = k.shape
         if len(dims) != 3 or dims[1] != heads or dims[2] != hd or v.shape != dims or k.dtype is not v.dtype:
@@ -229,7 +229,7 @@ class QuantizedCache:
                max_new: int, max_kv: int, mode: int = _lib.ATTN_CAUSAL, tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                status: Optional[torch.Tensor] = None) -> None:
         """Attention of new tokens, whose keys and values have been appended.  q [tokens, query heads * head_dim] (bf16 or fp32; rows any
-        stride apart), out the same, contiguous; row b of the batch has tokens row_start[b] .. row_start[b + 1] - 1, its keys are slots
+        multiple of 16 bytes apart), out the same, contiguous; row b of the batch has tokens row_start[b] .. row_start[b + 1] - 1, its keys are slots
         kv_begin[b] .. + base_len[b] (all visible) and its new tokens' own, visible causally or through tree_mask [tokens, words] (ATTN_TREE).
         max_new, max_kv: upper bounds of a row's new tokens and keys; what exceeds them is left out.  scale: of the scores, 1 / sqrt(head_dim) unless
         given."""
