@@ -576,6 +576,8 @@ __global__ void __launch_bounds__(Many<HD, QT>::kThreads, 1)
   if (!ok && atomicCAS((int*)stop, 0, 1) == 0 && status) atomicExch(status, 420 + site);
   rd_umma::fence_before();
   __syncthreads();
+  if (*stop)
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // products in flight read and write shared memory and TMEM
   if (warp == kIssue) {
     rd_umma::fence_after();
     rd_umma::tmem_dealloc(tmem_slot, L::kTmem);

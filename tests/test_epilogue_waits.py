@@ -50,3 +50,12 @@ def test_the_reading_finds_one_that_leaves_alone():
     good = "for (;;) { stage(); if (!rd::epilogue_agrees(warp_wait(&full, 0, stop))) { ok = false; break; } use(); }"
     bad = 'for (int t = 0; t < n; ++t) { asm volatile("bar.sync 1, 128;" ::: "memory"); if (!warp_wait(&full, 0, stop)) { ok = false; break; } use(); }'
     assert not any(left_alone(b) for b in blocks(good)) and any(left_alone(b) for b in blocks(bad))
+
+
+@pytest.mark.parametrize("name, kernels", [("gemm_int8.cu", 2), ("attention_quant_many.cuh", 1)])
+def test_a_kernel_that_gave_up_lets_its_work_land(name, kernels):
+    """Copies and products in flight have time to land before tensor memory is given back and the CTA leaves its shared memory."""
+    with open(os.path.join(CSRC, name)) as f:
+        source = f.read()
+    ends = re.findall(r"__syncthreads\(\);\n  if \(\*stop\)\n    for \(int i = 0; i < 2000; \+\+i\) __nanosleep\(1000\);[^}]*?dealloc", source)
+    assert len(ends) == len(re.findall(r"tmem_dealloc\(|tcgen05\.dealloc", source)) == kernels
