@@ -11,7 +11,9 @@
 //                 keep fp16's 11 bits down to 2^-28 of the largest.  What the zeros come to, sum W zero, is one number for a row of
 //                 queries and is taken off its features every eight tiles: until then O's fp32 holds at most some 2000 codes too much.
 //                 Codes of 4 bits are all taken four bits up here: the tensor core cuts a sum some 24 bits below what its factors' exponents allow for,
-//                 and with factors of code * 2^-24 that was 2^-19 of the largest value, unmoved that is 2^-23.
+//                 and with factors of code * 2^-24 that was 2^-19 of the largest value, moved that is 2^-23, as for codes of 8 bits.  Each
+//                 of the n keys is cut there: where one key has nearly all the weight and a value near 0, the others' part is off by up to n 2^-24 of the
+//                 largest value (22 keys against one of weight 0.99995: 6 10^-7 of it).
 // The accumulators' layouts fit: a lane holds the same query columns in S^T and in O^T, so the running maximum and sum need no
 // exchange but the maximum's over the 8 lanes of a column, and only where some lane's exceeds it; the weights become a B operand by
 // movmatrix.

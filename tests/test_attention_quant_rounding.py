@@ -24,7 +24,8 @@ def exact(cache, q, new, base, scale, many, plant=None):
     Scores: products with one feature and with zero * sum q, 5 roundings of 2^-23 of at most 2 |x| (2^bits - 1) scale_k; 2^-22 of the score for the
     exponent's argument; where keys are rounded, 2^-11 |x k|.  They count twice, in a weight and in the sum.  e^x: 2^-20.  Sums of n weights: n 2^-23.
     Weights (few rows: p s / r 2^14) and values (many rows) in fp16: 2^-11 of each product p |v|, the sum of weights is that of the unrounded ones.
-    fp16's smallest step and what is taken off for the zeros: see quant_helpers.attention."""
+    fp16's smallest step: see quant_helpers.attention.  What W code and W zero come to apart (few rows) is at most r = R (2^bits - 1) times the weights' share;
+    a tensor core cuts each addend of a product of 16 keys at 2^-24 of the largest, all n of them, and the two sums and their difference round."""
     l = cache.layers[0]
     hd, bits = cache.head_dim, cache.bits
     k, v = (values(host(c), host(p), bits)[0] for c, p in ((l.k_codes, l.k_params), (l.v_codes, l.v_params)))
@@ -51,7 +52,7 @@ def exact(cache, q, new, base, scale, many, plant=None):
             both = 2.0 ** -20 + 2 * err + n * 2.0 ** -23
             weight = both + FP16 * (2.001 if many else 1.0)
             r = vs[g, : base + new].max() * top
-            bound[i, h] = weight * (p @ np.abs(v[g, :n])) + both * np.abs(out[i, h]) + (n * 2.0 ** -32 + (n / 128 + 2) * 2.0 ** -22) * r
+            bound[i, h] = weight * (p @ np.abs(v[g, :n])) + both * np.abs(out[i, h]) + (n * 2.0 ** -32 + (0.0 if many else n * 2.0 ** -24 + 2.0 ** -21)) * r
     return out, bound + 2.0 ** -8 * np.abs(out)
 
 
