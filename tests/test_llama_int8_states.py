@@ -1,4 +1,4 @@
-"""What a Llama model in 8-bit integers can be asked for, and what is left of one whose conversion fails: runs without a GPU."""
+"""What a Llama model in 8-bit integers can be asked for, and what is left of one whose conversion fails."""
 import pytest
 import torch
 from gpu_helpers import llama_config
@@ -89,3 +89,18 @@ def test_moves_that_change_nothing(monkeypatch):
         with pytest.raises(rd._lib.RedrafterError, match="8-bit"):
             moved()
     assert [p.data_ptr() for p in llm.parameters()] == weights and llm.dtype is torch.float32
+
+
+@pytest.mark.gpu
+def test_on_the_device():
+    """The same of a real conversion, and the model goes on as before."""
+    llm = model().to("cuda", torch.bfloat16).hold_weights_in_int8()
+    ids, counts = torch.arange(3, 12, device="cuda"), [9]
+    before = rd.session.Session(llm, 1, 32).extend(ids, counts).clone()
+    drafter = rd.modeling_drafter.Drafter(rd.configuration_drafter.DrafterConfig(vocab_size=40, hidden_size=32, exit_dim=64, num_draft_layers=1, rnn=True))
+    both = rd.RecurrentDrafting(llm, drafter)
+    assert both.to("cuda") is both and both.to(torch.device("cuda", 0), torch.bfloat16) is both and llm.cuda() is llm
+    for refused in (llm.state_dict, both.state_dict, llm.init_random, llm.cpu, llm.float, llm.reference_state_dict):
+        with pytest.raises(rd._lib.RedrafterError, match="8-bit"):
+            refused()
+    assert torch.equal(rd.session.Session(llm, 1, 32).extend(ids, counts), before)
